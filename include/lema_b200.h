@@ -309,6 +309,99 @@ LEMA_API int lema_attn_bwd(const void* q, int64_t ldq, const void* k, int64_t ld
  * restores the default. A wait that runs out records device error 0x105. */
 LEMA_API int lema_attn_set_wait_budget(int64_t cycles);
 
+/* ---- losses over vocabulary logits (post-training objectives) --------------- */
+/* What stands beside the reference's shifted cross entropy (src/lema/_trainer.py:
+ * 151-157) in a trainer that aligns or distils a model; the reference has no such
+ * loss. Logits are n0 sequences of n1 rows of V values, bf16 (x_f32 = 0) or fp32,
+ * row (b, t) at x + b*ld0 + t*ld1 elements, unit stride along V, any alignment.
+ * targets [n0, n1] int64: a row whose target is ignore_index is not read, counts
+ * for nothing and gets a zero gradient row. A target (or a teacher index with a
+ * weight) outside [0, V) records device error 0x106 and makes its row's outputs
+ * NaN. q = softmax(x / temperature). Sums of exponentials are fp32, per-token
+ * terms and sums over tokens fp64, every output is rounded once. Gradients dx have
+ * the logits' type, row (b, t) at dx + b*ldd0 + t*ldd1, and may be written over x
+ * itself (same pointer and strides); they may not overlap it otherwise. NULL dx
+ * computes no gradient. grad_scale multiplies the gradient alone. `upstream` (may
+ * be NULL) is one fp32 device value that multiplies the gradient. `ws` is a
+ * 16-byte aligned scratch of lema_loss_workspace_bytes(n0, n1) bytes that no other
+ * call in flight uses; it needs no initial value. With no counted row a loss is 0.
+ * 1e-6 <= temperature <= 1e6. */
+
+/* Scratch bytes of the loss calls on n0 sequences of n1 rows (-1: too many rows). */
+LEMA_API int64_t lema_loss_workspace_bytes(int64_t n0, int64_t n1);
+
+/* logps[b,t] (fp32) = log q[target], 0 for ignored rows; stats (may be NULL)
+ * [n0, n1, 2] fp32 receives each row's maximum and reciprocal sum of
+ * exp((x - max) / temperature), the backward's input. */
+LEMA_API int lema_token_logprobs(const void* x, int32_t x_f32, int64_t n0, int64_t n1,
+                                 int64_t ld0, int64_t ld1, int64_t V, const int64_t* targets,
+                                 int64_t ignore_index, double temperature, float* logps,
+                                 float* stats, void* stream);
+
+/* dx = dlogps[b,t] * upstream / temperature * (onehot(target) - q), from the
+ * forward's stats. */
+LEMA_API int lema_token_logprobs_bwd(const void* x, int32_t x_f32, int64_t n0, int64_t n1,
+                                     int64_t ld0, int64_t ld1, int64_t V, const int64_t* targets,
+                                     int64_t ignore_index, double temperature,
+                                     const float* stats, const float* dlogps,
+                                     const float* upstream, void* dx, int64_t ldd0, int64_t ldd1,
+                                     void* stream);
+
+/* Preference loss of paired sequences: b < n0/2 chosen, b + n0/2 its rejected one.
+ *   R_b = sum_t logps[b,t] - ref_logps[b,t];  h = beta * (R_chosen - R_rejected)
+ *   loss = mean over pairs of (1 - e) * softplus(-h) + e * softplus(h), e = label_smoothing
+ * ref_logps [n0, n1] fp32 (NULL: 0; not read on ignored rows). Also returns
+ * rewards [n0] = beta * R_b, logps [n0, n1], stats [n0, n1, 2] and coef [n0, n1]
+ * = dloss/dlogps (the inputs of lema_token_logprobs_bwd at temperature 1). */
+LEMA_API int lema_preference_loss(const void* x, int32_t x_f32, int64_t n0, int64_t n1,
+                                  int64_t ld0, int64_t ld1, int64_t V, const int64_t* targets,
+                                  int64_t ignore_index, const float* ref_logps, double beta,
+                                  double label_smoothing, double grad_scale, void* ws,
+                                  int64_t ws_bytes, float* logps, float* stats, float* coef,
+                                  float* loss, float* rewards, void* dx, int64_t ldd0,
+                                  int64_t ldd1, void* stream);
+
+/* Clipped policy loss with a KL term, over counted tokens:
+ *   r = exp(logps - old_logps) (old_logps NULL: r = 1, on-policy),  d = ref_logps - logps
+ *   loss = sum_t w * ( -min(r * A, clip(r, 1 - clip_lo, 1 + clip_hi) * A)
+ *                      + kl_coef * (exp(d) - 1 - d) )
+ *   kl   = sum_t w * (exp(d) - 1 - d)                       (ref_logps NULL: 0)
+ * w = 1 / counted tokens, or with per_sequence 1 / (n0 * counted tokens of the
+ * sequence). A of row (b, t) is advantages[b*adv_s0 + t*adv_s1]. coef (may be NULL)
+ * receives dloss/dlogps, stats (may be NULL) the backward's statistics. */
+LEMA_API int lema_policy_loss(const void* x, int32_t x_f32, int64_t n0, int64_t n1, int64_t ld0,
+                              int64_t ld1, int64_t V, const int64_t* targets,
+                              int64_t ignore_index, double temperature, const float* old_logps,
+                              const float* advantages, int64_t adv_s0, int64_t adv_s1,
+                              const float* ref_logps, double clip_lo, double clip_hi,
+                              double kl_coef, int32_t per_sequence, double grad_scale, void* ws,
+                              int64_t ws_bytes, float* logps, float* stats, float* coef,
+                              float* loss, float* kl, void* dx, int64_t ldd0, int64_t ldd1,
+                              void* stream);
+
+/* Distillation from the teacher's K (1..1024) logits of each row, p = softmax over
+ * them of teacher_logits / temperature:
+ *   loss = temperature^2 * mean over counted rows of sum_k p_k (log p_k - log q[id_k])
+ * teacher_ids [n0, n1, K] int64 (ids_i32: int32), teacher_logits [n0, n1, K] bf16
+ * (tl_f32 = 0) or fp32, mask [n0, n1] bytes (0: row not counted; NULL: all count).
+ * Entries of logit -inf have no weight, whatever their index; a row of them alone
+ * contributes 0. An index that repeats adds its weights. stats / coef (may be NULL):
+ * the inputs of lema_distill_loss_bwd. */
+LEMA_API int lema_distill_loss(const void* x, int32_t x_f32, int64_t n0, int64_t n1, int64_t ld0,
+                               int64_t ld1, int64_t V, const void* teacher_ids, int32_t ids_i32,
+                               const void* teacher_logits, int32_t tl_f32, int64_t K,
+                               const uint8_t* mask, double temperature, double grad_scale,
+                               void* ws, int64_t ws_bytes, float* stats, float* coef, float* loss,
+                               void* dx, int64_t ldd0, int64_t ldd1, void* stream);
+
+/* dx of lema_distill_loss from its stats and coef. */
+LEMA_API int lema_distill_loss_bwd(const void* x, int32_t x_f32, int64_t n0, int64_t n1,
+                                   int64_t ld0, int64_t ld1, int64_t V, const void* teacher_ids,
+                                   int32_t ids_i32, const void* teacher_logits, int32_t tl_f32,
+                                   int64_t K, const uint8_t* mask, double temperature,
+                                   const float* stats, const float* coef, const float* upstream,
+                                   void* dx, int64_t ldd0, int64_t ldd1, void* stream);
+
 /* ---- K6: grouped W8A8 GEMM (MoE experts) -------------------------------- */
 /* Tokens are pre-sorted by expert: rows [offsets[e], offsets[e+1]) of xq/sx/y
  * belong to expert e, whose weights are wq + e*N*ldw, sw + e*N and

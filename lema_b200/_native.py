@@ -19,6 +19,10 @@ i64 = C.c_int64
 i32 = C.c_int32
 vp = C.c_void_p
 sz = C.c_size_t
+f64 = C.c_double
+
+# x, x_f32, n0, n1, ld0, ld1, V: the logits of the loss entry points
+_LOGITS = [vp, i32, i64, i64, i64, i64, i64]
 
 JOB_FN = C.CFUNCTYPE(None, vp)
 
@@ -66,6 +70,17 @@ _SIGNATURES: dict[str, list] = {
     "lema_attn_bwd": [vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp,
                       i64, vp, i64, i64, i64, i64, i64, i64, C.c_float, vp],
     "lema_attn_set_wait_budget": [i64],
+    "lema_loss_workspace_bytes": [i64, i64],
+    "lema_token_logprobs": _LOGITS + [vp, i64, f64, vp, vp, vp],
+    "lema_token_logprobs_bwd": _LOGITS + [vp, i64, f64, vp, vp, vp, vp, i64, i64, vp],
+    "lema_preference_loss": _LOGITS + [vp, i64, vp, f64, f64, f64, vp, i64, vp, vp, vp, vp, vp,
+                                       vp, i64, i64, vp],
+    "lema_policy_loss": _LOGITS + [vp, i64, f64, vp, vp, i64, i64, vp, f64, f64, f64, i32, f64,
+                                   vp, i64, vp, vp, vp, vp, vp, vp, i64, i64, vp],
+    "lema_distill_loss": _LOGITS + [vp, i32, vp, i32, i64, vp, f64, f64, vp, i64, vp, vp, vp, vp,
+                                    i64, i64, vp],
+    "lema_distill_loss_bwd": _LOGITS + [vp, i32, vp, i32, i64, vp, f64, vp, vp, vp, vp, i64, i64,
+                                        vp],
     "lema_ckpt_save": [vp, vp, sz, i32, vp, vp, vp],
     "lema_ckpt_restore": [vp, vp, sz, vp, vp, vp],
     "lema_mm_create": [i64, i64, i32, C.POINTER(vp)],
@@ -89,7 +104,8 @@ _SIGNATURES: dict[str, list] = {
     "lema_mm_is_layer_in_ram": [vp, i64, C.POINTER(i32)],
     "lema_mm_copy_stream": [vp, C.POINTER(vp)],
 }
-_RESTYPES = {"lema_last_error": C.c_char_p, "lema_version": C.c_char_p}
+_RESTYPES = {"lema_last_error": C.c_char_p, "lema_version": C.c_char_p,
+             "lema_loss_workspace_bytes": i64}
 
 # Status codes (enum lema_status).
 LEMA_OK = 0
@@ -146,7 +162,9 @@ KERNELS_PER_CALL = {
     "lema_grouped_w8a8_dgrad": 2, "lema_rmsnorm_quant": 1, "lema_rmsnorm_bwd": 1,
     "lema_rope": 1, "lema_rope_qkv": 1, "lema_swiglu_quant": 1, "lema_swiglu_bwd": 1,
     "lema_adamw_requant_rows": 1, "lema_device_error_async": 1, "lema_attn_fwd": 1,
-    "lema_attn_bwd": 3,
+    "lema_attn_bwd": 3, "lema_token_logprobs": 1, "lema_token_logprobs_bwd": 1,
+    "lema_preference_loss": 3, "lema_policy_loss": 3, "lema_distill_loss": 3,
+    "lema_distill_loss_bwd": 1,
 }
 # Running count of this library's kernel launches issued by this process.
 kernel_launches = 0
@@ -203,6 +221,7 @@ DEVICE_ERROR_NAMES = {
     0x103: "a GEMM's epilogue timed out waiting for accumulators",
     0x104: "a split GEMM tile's partial accumulators never arrived",
     0x105: "an attention kernel timed out waiting for a tile, a score buffer or P",
+    0x106: "a loss was given a target or teacher index outside the vocabulary",
 }
 
 

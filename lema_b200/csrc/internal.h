@@ -40,6 +40,7 @@ enum DeviceErr : int32_t {
   kDevErrEpilogueTimeout = 0x103,
   kDevErrSplitTimeout = 0x104,  // a split tile's partial accumulators never arrived
   kDevErrAttnTimeout = 0x105,   // an attention kernel's wait ran out
+  kDevErrIndex = 0x106,         // a loss's target or teacher index lies outside the vocabulary
 };
 
 // While alive, GEMMs issued by this thread run every tile whole (no split-K

@@ -12,6 +12,14 @@ adapters/_llama.py:245-250), wrapped by ``LoRAWrapper.forward``
                          backward dx = dy . (wq * sw) through ``w8a8_dgrad``
 * ``grouped_w8a8_gemm``  the same per expert over pre-sorted token ranges
 
+and of the losses over the head's logits (each with a ``*_grad`` form that returns the
+logits' gradient in the same call):
+
+* ``token_logprobs``     log-probability of each target token, differentiable
+* ``preference_loss``    pairs of chosen / rejected sequences
+* ``policy_loss``        clipped policy ratios with a KL term
+* ``distill_loss``       a teacher's top logits
+
 All tensors must live on a CUDA device; there is no CPU fallback. Calls run
 on the current torch stream of the tensors' device.
 """
@@ -824,3 +832,418 @@ class AttentionFn(torch.autograd.Function):
         q2d, k2d, v2d, o, lse = ctx.saved_tensors
         dq, dk, dv = attention_bwd(q2d, k2d, v2d, o, lse, do, *ctx.meta)
         return dq, dk, dv, None, None, None, None, None
+
+
+# ---------------------------------------------------------------------------
+# Losses over vocabulary logits: token log-probabilities, preference pairs,
+# clipped policy, distillation from a teacher's top logits
+# ---------------------------------------------------------------------------
+
+class _Logits:
+    """Logits [..., V] as the sequences of rows the kernels address, with the
+    checks every loss makes. Copies only when the last stride is not 1 or the
+    leading dimensions cannot be seen as [sequences, rows]."""
+
+    __slots__ = ("t", "dev", "lead", "n0", "n1", "ld0", "ld1", "V", "args")
+
+    def __init__(self, logits: torch.Tensor):
+        if not logits.is_cuda:
+            _require_cuda(logits)
+        if logits.dtype not in (torch.bfloat16, torch.float32):
+            raise TypeError(f"logits must be bf16 or fp32, got {logits.dtype}")
+        if logits.dim() < 2:
+            raise ValueError(f"logits must be [..., V], got shape {tuple(logits.shape)}")
+        self.lead = logits.shape[:-1]
+        self.V = logits.shape[-1]
+        if self.V < 1:
+            raise ValueError("logits need at least one vocabulary entry")
+        self.dev = logits.device
+        t = logits
+        if t.dim() > 3:
+            t = t.reshape(-1, t.shape[-2], self.V)
+        elif t.dim() == 2:
+            t = t[None]
+        if t.stride(2) != 1 and self.V > 1:
+            t = t.contiguous()
+        self.t = t
+        self.n0, self.n1 = t.shape[0], t.shape[1]
+        self.ld0, self.ld1 = t.stride(0), t.stride(1)
+        self.args = (t.data_ptr(), int(t.dtype == torch.float32), self.n0, self.n1, self.ld0,
+                     self.ld1, self.V)
+
+    def per_row(self, t: torch.Tensor | None, name: str, dtype: torch.dtype):
+        """A contiguous [rows] companion of the logits, on their device."""
+        if t is None:
+            return None
+        if t.device != self.dev:
+            raise RuntimeError(f"{name} on {t.device}, logits on {self.dev}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if t.shape != self.lead:
+            raise ValueError(f"{name} must have shape {tuple(self.lead)}, got {tuple(t.shape)}")
+        if t.requires_grad:
+            raise ValueError(f"{name} is a constant of the loss: detach it")
+        return t.contiguous()
+
+    def grad_out(self, logits: torch.Tensor, out: torch.Tensor | None):
+        """(gradient tensor, its [sequences, rows, V] view)."""
+        if out is None:
+            out = torch.empty(logits.shape, dtype=logits.dtype, device=self.dev)
+        else:
+            if out.shape != logits.shape or out.dtype != logits.dtype or out.device != self.dev:
+                raise ValueError("out must have the logits' shape, type and device")
+            if out.requires_grad:
+                raise ValueError("out must not require grad: detach it")
+            same = (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride())
+            if out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr() \
+                    and out.numel() and not same:
+                raise ValueError("out shares the logits' storage without being the logits")
+            if not _rows_disjoint(out):
+                raise ValueError("out needs a unit last stride and rows that do not overlap")
+            if same and self.t.data_ptr() != logits.data_ptr():
+                raise ValueError("out: these logits have to be copied, so out cannot be they")
+            torch.autograd.graph.increment_version(out)
+        view = out
+        if out.dim() > 3:
+            view = out.view(-1, out.shape[-2], self.V)
+        elif out.dim() == 2:
+            view = out[None]
+        return out, view
+
+    def workspace(self):
+        n = N.lib().lema_loss_workspace_bytes(self.n0, self.n1)
+        if n < 0:
+            raise ValueError("more than 2^31 - 1 rows of logits")
+        return torch.empty(n, dtype=torch.uint8, device=self.dev), n
+
+    def call(self, name: str, *args) -> None:
+        """One entry point on the logits' device and its current stream."""
+        if torch.cuda.current_device() != self.dev.index:
+            with torch.cuda.device(self.dev):
+                N.call(name, *self.args, *args, _stream(self.dev))
+        else:
+            N.call(name, *self.args, *args, _stream(self.dev))
+
+
+def _rows_disjoint(t: torch.Tensor) -> bool:
+    """Unit stride along the last dimension and no two elements at one address."""
+    if t.numel() == 0:
+        return True
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        return False
+    extent = t.shape[-1]
+    for size, stride in sorted(((t.shape[d], t.stride(d)) for d in range(t.dim() - 1)
+                                if t.shape[d] > 1), key=lambda p: p[1]):
+        if stride < extent:
+            return False
+        extent = stride * (size - 1) + extent
+    return True
+
+
+def _targets(x: _Logits, targets: torch.Tensor) -> torch.Tensor:
+    return x.per_row(targets, "targets", torch.int64)
+
+
+def _logprobs_bwd(x: _Logits, logits, targets, ignore_index, temperature, stats, dlogps,
+                  upstream=None) -> torch.Tensor:
+    dx, view = x.grad_out(logits, None)
+    x.call("lema_token_logprobs_bwd", targets.data_ptr(), ignore_index, temperature,
+           stats.data_ptr(), dlogps.data_ptr(), _ptr(upstream), view.data_ptr(), view.stride(0),
+           view.stride(1))
+    return dx
+
+
+def _logprobs_fwd(logits, targets, temperature, ignore_index, want_stats):
+    x = _Logits(logits)
+    targets = _targets(x, targets)
+    logps = torch.empty(x.lead, dtype=torch.float32, device=x.dev)
+    stats = (torch.empty(x.n0, x.n1, 2, dtype=torch.float32, device=x.dev) if want_stats
+             else None)
+    x.call("lema_token_logprobs", targets.data_ptr(), ignore_index, temperature,
+           logps.data_ptr(), _ptr(stats))
+    return logps, targets, stats
+
+
+class _TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, temperature, ignore_index):
+        logps, targets, stats = _logprobs_fwd(logits, targets, temperature, ignore_index, True)
+        ctx.save_for_backward(logits, targets, stats)
+        ctx.meta = (temperature, ignore_index)
+        return logps
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dlogps):
+        logits, targets, stats = ctx.saved_tensors
+        temperature, ignore_index = ctx.meta
+        return _logprobs_bwd(_Logits(logits), logits, targets, ignore_index, temperature, stats,
+                             dlogps.contiguous()), None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, *, temperature: float = 1.0,
+                   ignore_index: int = -100) -> torch.Tensor:
+    """log softmax(logits / temperature) at ``targets``: logits [..., V] bf16 or
+    fp32, targets [...] int64 -> fp32 [...] (0 where the target is ``ignore_index``;
+    those rows are not read). Differentiable in the logits. ``targets`` are aligned
+    with the logits: position t holds the token the row predicts."""
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _TokenLogprobsFn.apply(logits, targets, float(temperature), int(ignore_index))
+    return _logprobs_fwd(logits, targets, float(temperature), int(ignore_index), False)[0]
+
+
+def _preference(logits, targets, ref_logps, beta, label_smoothing, ignore_index, grad_scale, out,
+                want_dx):
+    x = _Logits(logits)
+    if logits.dim() != 3 or x.n0 % 2 or x.n0 == 0:
+        raise ValueError("preference_loss takes logits [2 P, S, V]: P chosen sequences, then "
+                         "their P rejected ones")
+    targets = _targets(x, targets)
+    ref = x.per_row(ref_logps, "ref_logps", torch.float32)
+    ws, n = x.workspace()
+    f = torch.empty(2 + 4 * x.n0 * x.n1 + x.n0, dtype=torch.float32, device=x.dev)
+    T = x.n0 * x.n1
+    stats, logps, coef = f[:2 * T], f[2 * T:3 * T], f[3 * T:4 * T]
+    rewards, loss = f[4 * T:4 * T + x.n0], f[4 * T + x.n0]
+    dx = view = None
+    if want_dx:
+        dx, view = x.grad_out(logits, out)
+    x.call("lema_preference_loss", targets.data_ptr(), int(ignore_index), _ptr(ref), float(beta),
+           float(label_smoothing), float(grad_scale), ws.data_ptr(), n, logps.data_ptr(),
+           stats.data_ptr(), coef.data_ptr(), loss.data_ptr(), rewards.data_ptr(), _ptr(view),
+           view.stride(0) if want_dx else 0, view.stride(1) if want_dx else 0)
+    if want_dx and T:
+        N.kernel_launches += 1  # the gradient rows
+    return x, targets, loss, rewards, stats, coef, dx
+
+
+class _PreferenceFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, ref_logps, beta, label_smoothing, ignore_index):
+        _, targets, loss, rewards, stats, coef, _ = _preference(
+            logits, targets, ref_logps, beta, label_smoothing, ignore_index, 1.0, None, False)
+        ctx.save_for_backward(logits, targets, stats, coef)
+        ctx.ignore_index = ignore_index
+        ctx.mark_non_differentiable(rewards)
+        return loss, rewards
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss, _drewards):
+        logits, targets, stats, coef = ctx.saved_tensors
+        return (_logprobs_bwd(_Logits(logits), logits, targets, ctx.ignore_index, 1.0, stats, coef,
+                              dloss.float()), None, None, None, None, None)
+
+
+def preference_loss(logits: torch.Tensor, targets: torch.Tensor,
+                    ref_logps: torch.Tensor | None = None, *, beta: float = 0.1,
+                    label_smoothing: float = 0.0, ignore_index: int = -100):
+    """Preference loss of paired sequences over their summed log ratios.
+
+    logits [2 P, S, V] (bf16 or fp32): the P chosen sequences, then their rejected
+    ones in the same order; targets [2 P, S] int64, ``ignore_index`` on prompts and
+    padding; ref_logps [2 P, S] fp32, the frozen reference model's
+    ``token_logprobs`` (None: 0). Returns (loss, rewards): the mean over pairs of
+    (1 - e) softplus(-h) + e softplus(h), h the chosen reward less the rejected
+    one, e = ``label_smoothing``, and rewards [2 P] = beta * sum of log ratios
+    (no gradient). Differentiable in the logits."""
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _PreferenceFn.apply(logits, targets, ref_logps, beta, label_smoothing, ignore_index)
+    _, _, loss, rewards, *_ = _preference(logits, targets, ref_logps, beta, label_smoothing,
+                                          ignore_index, 1.0, None, False)
+    return loss, rewards
+
+
+def preference_loss_grad(logits: torch.Tensor, targets: torch.Tensor,
+                         ref_logps: torch.Tensor | None = None, *, beta: float = 0.1,
+                         label_smoothing: float = 0.0, ignore_index: int = -100,
+                         grad_scale: float = 1.0, out: torch.Tensor | None = None):
+    """``preference_loss`` and its gradient in one call: (loss, rewards, dlogits).
+    dlogits = grad_scale * dloss/dlogits, written into ``out`` when given (which
+    may be ``logits`` itself)."""
+    _, _, loss, rewards, _, _, dx = _preference(logits, targets, ref_logps, beta, label_smoothing,
+                                                ignore_index, grad_scale, out, True)
+    return loss, rewards, dx
+
+
+def _policy(logits, targets, old_logps, advantages, ref_logps, clip, kl_coef, temperature,
+            reduction, ignore_index, grad_scale, out, want_dx, want_saved):
+    x = _Logits(logits)
+    if reduction not in ("token", "sequence"):
+        raise ValueError(f"reduction must be 'token' or 'sequence', not {reduction!r}")
+    clip_lo, clip_hi = clip
+    targets = _targets(x, targets)
+    old = x.per_row(old_logps, "old_logps", torch.float32)
+    ref = x.per_row(ref_logps, "ref_logps", torch.float32)
+    adv = advantages
+    if adv.shape == x.lead:
+        adv = x.per_row(adv, "advantages", torch.float32)
+        s0, s1 = x.n1, 1
+    elif logits.dim() == 3 and adv.shape == x.lead[:1]:
+        if adv.device != x.dev or adv.dtype != torch.float32 or adv.requires_grad:
+            raise ValueError("advantages must be fp32 constants on the logits' device")
+        adv = adv.contiguous()
+        s0, s1 = 1, 0
+    else:
+        raise ValueError(f"advantages must have shape {tuple(x.lead)}, or one per sequence")
+    ws, n = x.workspace()
+    T = x.n0 * x.n1
+    logps = torch.empty(x.lead, dtype=torch.float32, device=x.dev)
+    f = torch.empty(2 + (3 * T if want_saved else 0), dtype=torch.float32, device=x.dev)
+    loss, kl = f[0], f[1]
+    stats, coef = (f[2:2 + 2 * T], f[2 + 2 * T:]) if want_saved else (None, None)
+    dx = view = None
+    if want_dx:
+        dx, view = x.grad_out(logits, out)
+    x.call("lema_policy_loss", targets.data_ptr(), int(ignore_index), float(temperature),
+           _ptr(old), adv.data_ptr(), s0, s1, _ptr(ref), float(clip_lo), float(clip_hi),
+           float(kl_coef), int(reduction == "sequence"), float(grad_scale), ws.data_ptr(), n,
+           logps.data_ptr(), _ptr(stats), _ptr(coef), loss.data_ptr(), kl.data_ptr(), _ptr(view),
+           view.stride(0) if want_dx else 0, view.stride(1) if want_dx else 0)
+    return targets, loss, logps, kl, stats, coef, dx
+
+
+class _PolicyFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, old_logps, advantages, ref_logps, clip, kl_coef, temperature,
+                reduction, ignore_index):
+        targets, loss, logps, kl, stats, coef, _ = _policy(
+            logits, targets, old_logps, advantages, ref_logps, clip, kl_coef, temperature,
+            reduction, ignore_index, 1.0, None, False, True)
+        ctx.save_for_backward(logits, targets, stats, coef)
+        ctx.meta = (ignore_index, float(temperature))
+        ctx.mark_non_differentiable(logps, kl)
+        return loss, logps, kl
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss, _dlogps, _dkl):
+        logits, targets, stats, coef = ctx.saved_tensors
+        ignore_index, temperature = ctx.meta
+        dx = _logprobs_bwd(_Logits(logits), logits, targets, ignore_index, temperature, stats,
+                           coef, dloss.float())
+        return (dx,) + (None,) * 9
+
+
+def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logps: torch.Tensor | None,
+                advantages: torch.Tensor, ref_logps: torch.Tensor | None = None, *,
+                clip: tuple[float, float] = (0.2, 0.2), kl_coef: float = 0.0,
+                temperature: float = 1.0, reduction: str = "token", ignore_index: int = -100):
+    """Clipped policy loss with a KL term.
+
+    logits [B, S, V] or [T, V]; targets (the sampled tokens, aligned with the rows
+    that predict them), old_logps (the sampling policy's, None: on-policy, ratio
+    1) and ref_logps (the KL's reference, None: no KL) of shape [B, S] / [T];
+    advantages of that shape, or [B]. With r = exp(lp - old), d = ref - lp:
+    loss = sum w (-min(r A, clip(r, 1 - clip[0], 1 + clip[1]) A) + kl_coef
+    (exp(d) - 1 - d)), w = 1 / counted tokens ("token") or the mean over sequences
+    of their tokens' means ("sequence"). Returns (loss, logps, kl): logps fp32, kl
+    the weighted sum of exp(d) - 1 - d (neither with a gradient). Differentiable in
+    the logits; every other argument is a constant."""
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _PolicyFn.apply(logits, targets, old_logps, advantages, ref_logps, clip, kl_coef,
+                               temperature, reduction, ignore_index)
+    _, loss, logps, kl, *_ = _policy(logits, targets, old_logps, advantages, ref_logps, clip,
+                                     kl_coef, temperature, reduction, ignore_index, 1.0, None,
+                                     False, False)
+    return loss, logps, kl
+
+
+def policy_loss_grad(logits: torch.Tensor, targets: torch.Tensor, old_logps: torch.Tensor | None,
+                     advantages: torch.Tensor, ref_logps: torch.Tensor | None = None, *,
+                     clip: tuple[float, float] = (0.2, 0.2), kl_coef: float = 0.0,
+                     temperature: float = 1.0, reduction: str = "token",
+                     ignore_index: int = -100, grad_scale: float = 1.0,
+                     out: torch.Tensor | None = None):
+    """``policy_loss`` and its gradient in one pass over the logits: (loss, logps,
+    kl, dlogits). dlogits = grad_scale * dloss/dlogits, written into ``out`` when
+    given (which may be ``logits`` itself)."""
+    _, loss, logps, kl, _, _, dx = _policy(logits, targets, old_logps, advantages, ref_logps, clip,
+                                           kl_coef, temperature, reduction, ignore_index,
+                                           grad_scale, out, True, False)
+    return loss, logps, kl, dx
+
+
+def _teacher(x: _Logits, ids: torch.Tensor, logits: torch.Tensor, mask):
+    if ids.device != x.dev or logits.device != x.dev:
+        raise RuntimeError("teacher tensors must be on the logits' device")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"teacher_ids must be int32 or int64, got {ids.dtype}")
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"teacher_logits must be bf16 or fp32, got {logits.dtype}")
+    if ids.shape != logits.shape or ids.shape[:-1] != x.lead or ids.dim() != len(x.lead) + 1:
+        raise ValueError(f"teacher_ids and teacher_logits must be {tuple(x.lead)} + (K,)")
+    if logits.requires_grad:
+        raise ValueError("teacher_logits are constants of the loss: detach them")
+    mask = x.per_row(mask, "mask", torch.bool)
+    return ids.contiguous(), logits.contiguous(), mask
+
+
+def _distill(logits, teacher_ids, teacher_logits, mask, temperature, grad_scale, out, want_dx,
+             want_saved):
+    x = _Logits(logits)
+    ids, tl, mask = _teacher(x, teacher_ids, teacher_logits, mask)
+    ws, n = x.workspace()
+    T = x.n0 * x.n1
+    # the loss, then the statistics (pairs: 8-byte aligned) and the coefficients
+    f = torch.empty(2 + (3 * T if want_saved else 0), dtype=torch.float32, device=x.dev)
+    stats, coef = (f[2:2 + 2 * T], f[2 + 2 * T:]) if want_saved else (None, None)
+    dx = view = None
+    if want_dx:
+        dx, view = x.grad_out(logits, out)
+    x.call("lema_distill_loss", ids.data_ptr(), int(ids.dtype == torch.int32), tl.data_ptr(),
+           int(tl.dtype == torch.float32), ids.shape[-1], _ptr(mask), float(temperature),
+           float(grad_scale), ws.data_ptr(), n, _ptr(stats), _ptr(coef), f.data_ptr(), _ptr(view),
+           view.stride(0) if want_dx else 0, view.stride(1) if want_dx else 0)
+    return ids, tl, mask, f[0], stats, coef, dx
+
+
+class _DistillFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, teacher_ids, teacher_logits, mask, temperature):
+        ids, tl, mask, loss, stats, coef, _ = _distill(logits, teacher_ids, teacher_logits, mask,
+                                                       temperature, 1.0, None, False, True)
+        ctx.save_for_backward(logits, ids, tl, mask, stats, coef)
+        ctx.temperature = float(temperature)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        logits, ids, tl, mask, stats, coef = ctx.saved_tensors
+        x = _Logits(logits)
+        dx, view = x.grad_out(logits, None)
+        up = dloss.float()
+        x.call("lema_distill_loss_bwd", ids.data_ptr(), int(ids.dtype == torch.int32),
+               tl.data_ptr(), int(tl.dtype == torch.float32), ids.shape[-1], _ptr(mask),
+               ctx.temperature, stats.data_ptr(), coef.data_ptr(), up.data_ptr(),
+               view.data_ptr(), view.stride(0), view.stride(1))
+        return dx, None, None, None, None
+
+
+def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                 mask: torch.Tensor | None = None, *, temperature: float = 1.0) -> torch.Tensor:
+    """Distillation from the K (at most 1024) best logits a teacher gave for each row:
+    temperature^2 * mean over counted rows of KL(p || q), p the softmax over
+    the teacher's K entries and q the student's over the whole vocabulary, both at
+    ``temperature``. logits [..., V] bf16 or fp32; teacher_ids [..., K] int32 or
+    int64; teacher_logits [..., K] bf16 or fp32 (-inf: no entry, whatever its
+    index; an index that repeats adds its weights); mask [...] bool, False rows
+    are not read. Differentiable in the logits."""
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _DistillFn.apply(logits, teacher_ids, teacher_logits, mask, temperature)
+    _, _, _, loss, *_ = _distill(logits, teacher_ids, teacher_logits, mask, temperature, 1.0, None,
+                                 False, False)
+    return loss
+
+
+def distill_loss_grad(logits: torch.Tensor, teacher_ids: torch.Tensor,
+                      teacher_logits: torch.Tensor, mask: torch.Tensor | None = None, *,
+                      temperature: float = 1.0, grad_scale: float = 1.0,
+                      out: torch.Tensor | None = None):
+    """``distill_loss`` and its gradient in one pass over the logits: (loss, dlogits).
+    dlogits = grad_scale * dloss/dlogits, written into ``out`` when given (which may
+    be ``logits`` itself)."""
+    *_, loss, _, _, dx = _distill(logits, teacher_ids, teacher_logits, mask, temperature,
+                                  grad_scale, out, True, False)
+    return loss, dx

@@ -1,0 +1,96 @@
+"""Host-side behaviour of the losses over vocabulary logits: every bad argument is an
+error before anything is launched, and no operator runs on CPU tensors."""
+import pytest
+import torch
+
+from lema_b200 import _native as N
+from lema_b200 import ops
+
+FAKE = 4096          # a non-null, aligned address that is never dereferenced
+ROWS = (FAKE, 0, 2, 3, 300, 100, 100)
+
+
+def logprobs(rows=ROWS, targets=FAKE, tau=1.0, logps=FAKE):
+    return N.lib().lema_token_logprobs(*rows, targets, -100, tau, logps, None, None)
+
+
+def test_rows():
+    assert logprobs((None, 0, 0, 3, 300, 100, 100)) == N.LEMA_OK       # no rows: nothing to do
+    assert logprobs((None, 0, 2, 0, 300, 100, 100)) == N.LEMA_OK
+    for rows in ((None, 0, 2, 3, 300, 100, 100), (FAKE, 0, -1, 3, 300, 100, 100),
+                 (FAKE, 0, 2, -3, 300, 100, 100), (FAKE, 0, 2, 3, -1, 100, 100),
+                 (FAKE, 0, 2, 3, 300, -1, 100), (FAKE, 0, 2, 3, 300, 100, 0),
+                 (FAKE, 0, 2, 3, 300, 100, (1 << 30) + 1)):
+        assert logprobs(rows) == N.LEMA_ERR_INVALID_ARGUMENT, rows
+    assert logprobs((FAKE, 0, 1 << 20, 1 << 20, 1, 1, 1)) == N.LEMA_ERR_UNSUPPORTED
+    assert logprobs(targets=None) == N.LEMA_ERR_INVALID_ARGUMENT
+    assert logprobs(logps=None) == N.LEMA_ERR_INVALID_ARGUMENT
+    for tau in (0.0, -1.0, float("nan"), float("inf"), 1e-7, 1e7):
+        assert logprobs(tau=tau) == N.LEMA_ERR_INVALID_ARGUMENT
+        assert "temperature" in N.last_error()
+
+
+def test_workspace_bytes():
+    size = N.lib().lema_loss_workspace_bytes
+    assert size(-1, 4) == -1 and size(4, -1) == -1 and size(1 << 20, 1 << 20) == -1
+    assert 0 < size(0, 0) <= size(2, 3) <= size(8, 512)
+
+
+def preference(n0=2, ws=FAKE, n=1 << 20, beta=0.1, e=0.0, out=(None, 0, 0), loss=FAKE):
+    return N.lib().lema_preference_loss(FAKE, 0, n0, 3, 300, 100, 100, FAKE, -100, None, beta, e,
+                                        1.0, ws, n, FAKE, FAKE, FAKE, loss, FAKE, *out, None)
+
+
+def policy(ws=FAKE, n=1 << 20, clip=(0.2, 0.2), kl=0.0, adv=FAKE, out=(None, 0, 0)):
+    return N.lib().lema_policy_loss(FAKE, 0, 2, 3, 300, 100, 100, FAKE, -100, 1.0, None, adv, 3, 1,
+                                    None, *clip, kl, 0, 1.0, ws, n, FAKE, None, None, FAKE, FAKE,
+                                    *out, None)
+
+
+def distill(K=3, ids=FAKE, ws=FAKE, n=1 << 20, out=(None, 0, 0)):
+    return N.lib().lema_distill_loss(FAKE, 0, 2, 3, 300, 100, 100, ids, 0, FAKE, 1, K, None, 1.0,
+                                     1.0, ws, n, None, None, FAKE, *out, None)
+
+
+def test_losses_refuse():
+    bad = N.LEMA_ERR_INVALID_ARGUMENT
+    need = N.lib().lema_loss_workspace_bytes(2, 3)
+    for f in (preference, policy, distill):
+        assert f(ws=None) == bad and "workspace" in N.last_error()
+        assert f(ws=FAKE + 4) == bad
+        assert f(n=need - 1) == bad
+        assert f(out=(FAKE, 300, 99)) == bad and "overlap" in N.last_error()
+        assert f(out=(FAKE, 299, 100)) == bad
+        assert f(out=(FAKE, -300, 100)) == bad
+    assert preference(n0=3) == bad and preference(n0=0) == bad
+    for kw in ({"beta": 0.0}, {"beta": -1.0}, {"beta": float("inf")}, {"e": 0.5}, {"e": -0.1},
+               {"e": float("nan")}, {"loss": None}):
+        assert preference(**kw) == bad, kw
+    for kw in ({"clip": (1.1, 0.2)}, {"clip": (-0.1, 0.2)}, {"clip": (0.2, float("nan"))},
+               {"kl": -0.5}, {"kl": float("inf")}, {"adv": None}):
+        assert policy(**kw) == bad, kw
+    assert distill(K=0) == N.LEMA_ERR_UNSUPPORTED and distill(K=1025) == N.LEMA_ERR_UNSUPPORTED
+    assert distill(ids=None) == bad
+
+
+@pytest.mark.parametrize("name", ["token_logprobs", "preference_loss", "preference_loss_grad",
+                                  "policy_loss", "policy_loss_grad", "distill_loss",
+                                  "distill_loss_grad"])
+def test_no_cpu_fallback(name):
+    x = torch.zeros(2, 3, 8, dtype=torch.bfloat16)
+    t = torch.zeros(2, 3, dtype=torch.int64)
+    ids = torch.zeros(2, 3, 4, dtype=torch.int64)
+    args = {"token_logprobs": (t,), "preference_loss": (t,), "policy_loss": (t, None, torch.ones(2)),
+            "distill_loss": (ids, ids.float())}[name.replace("_grad", "")]
+    for v in (x, x.clone().requires_grad_(True)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            getattr(ops, name)(v, *args)
+
+
+def test_rows_that_overlap_are_found():
+    base = torch.zeros(4, 6, 8)
+    assert ops._rows_disjoint(base) and ops._rows_disjoint(base.transpose(0, 1))
+    assert ops._rows_disjoint(base[:, ::2, :5]) and ops._rows_disjoint(base[:0])
+    assert not ops._rows_disjoint(base[:1].expand(4, 6, 8))
+    assert not ops._rows_disjoint(base.transpose(1, 2))
+    assert not ops._rows_disjoint(base.as_strided((4, 6, 8), (48, 7, 1)))

@@ -1,0 +1,660 @@
+"""The losses over vocabulary logits (token log-probabilities, preference, clipped
+policy, distillation) and their gradients against their formulas in fp64.
+
+Tolerances. u = 2^-24. An exponential 2^((x - max) c) carries the fp32 roundings of the
+difference, of c and of the product (3 u of the exponent a, so 3 u a ln 2 of the value)
+and ex2.approx's 2^-22: relative 4 u + 2.1 u a. In the row's sum the exponents
+average at most log2 V (the entropy bound), and V / 512 + 16 additions round once each:
+    rel_s = (4 + 2.1 log2 V + V / 512 + 16) u
+which is the absolute error of a log-probability before its own rounding, u |lp|.
+A probability has rel_q = rel_s + (4 + 2.1 a_max) u. A gradient k (onehot - q) then
+is off by |k| q rel_q + 8 u |k (onehot - q)| + 2 u |k| onehot, and by half a step of its type.
+Losses move with the log-probabilities by at most sum |dloss/dlp| times their error."""
+import math
+
+import pytest
+import torch
+
+from lema_b200 import _native, ops
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
+IGN = -100
+
+
+def rel_s(V):
+    return (20 + 2.1 * math.log2(max(V, 2)) + V / 512) * U
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def make(dev, B, S, V, dtype, seed=0, ignore=0.3):
+    g = torch.Generator(device=dev).manual_seed(seed + 7 * V + S)
+    x = (torch.randn(B, S, V, device=dev, generator=g) * 2).to(DT[dtype])
+    t = torch.randint(0, V, (B, S), device=dev, generator=g)
+    up = torch.rand(B, S, 1, device=dev, generator=g) * 8
+    x.scatter_(-1, t[..., None], (x.gather(-1, t[..., None]).float() + up).to(x.dtype))
+    if ignore:
+        t[torch.rand(B, S, device=dev, generator=g) < ignore] = IGN
+    return x, t, g
+
+
+def ref_logps(x, t, tau=1.0):
+    """fp64 log-probabilities (0 where ignored) and probabilities of every row."""
+    z = x.double() / tau
+    lsm = torch.log_softmax(z, -1)
+    lp = lsm.gather(-1, t.clamp(min=0)[..., None])[..., 0]
+    return torch.where(t == IGN, torch.zeros_like(lp), lp), lsm.exp()
+
+
+def check_logps(got, want, V):
+    assert got.dtype == torch.float32
+    err = (got.double() - want).abs()
+    assert (err <= rel_s(V) + U * want.abs()).all(), err.max().item()
+
+
+def check_dx(got, x, q, k, mass, tau=1.0):
+    """got = k (mass - q): k [rows] fp64, mass the row's point masses."""
+    k = k[..., None]
+    want = k * (mass - q)
+    a_max = (x.double().amax(-1) - torch.where(x.isinf(), 0.0, x.double()).amin(-1)).max().item() \
+        / tau * 1.4427
+    rel_q = rel_s(x.shape[-1]) + (4 + 2.1 * min(a_max, 150.0)) * U
+    tol = (half_step(got.dtype) + 8 * U) * want.abs() + k.abs() * (q * rel_q + 2 * U * mass) + 1e-37
+    err = (got.double() - want).abs()
+    assert (err <= tol).all(), (err - tol).max().item()
+
+
+def onehot(t, V):
+    m = torch.zeros(*t.shape, V, dtype=torch.float64, device=t.device)
+    m.scatter_(-1, t.clamp(min=0)[..., None], 1.0)
+    return torch.where((t == IGN)[..., None], 0.0, m)
+
+
+SHAPES = [(1, 1, 1), (1, 1, 2), (2, 3, 7), (1, 5, 31), (3, 17, 512), (2, 9, 4097), (2, 5, 32000),
+          (1, 7, 32768), (1, 3, 32776), (2, 2, 50257), (1, 3, 65544), (1, 2, 128256),
+          (1, 1, 151937), (1, 2, 262144), (1, 1, 300001), (40, 64, 130), (300, 1, 1000)]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("B,S,V", SHAPES)
+def test_token_logprobs(cuda_device, B, S, V, dtype):
+    for tau in (1.0, 0.7):
+        x, t, g = make(cuda_device, B, S, V, dtype)
+        if B * S > 1:
+            t.view(-1)[0] = V - 1
+            t.view(-1)[-1] = 0
+        x.requires_grad_(True)
+        lp = ops.token_logprobs(x, t, temperature=tau)
+        want, q = ref_logps(x.detach(), t, tau)
+        check_logps(lp.detach(), want, V)
+        assert torch.equal(ops.token_logprobs(x.detach(), t, temperature=tau), lp.detach())
+        up = torch.randn(B, S, device=cuda_device, generator=g)
+        (dx,) = torch.autograd.grad(lp, x, up)
+        assert dx.shape == x.shape and dx.dtype == x.dtype
+        k = torch.where(t == IGN, 0.0, up.double() / tau)
+        check_dx(dx, x.detach(), q, k, onehot(t, V), tau)
+
+
+def _layouts(dev, dtype):
+    x, t, _ = make(dev, 3, 12, 1000, dtype)
+    big = torch.zeros(3, 12, 1100, dtype=x.dtype, device=dev)
+    for off in (0, 1, 8):
+        view = big.clone()[:, :, off:off + 1000]
+        view.copy_(x)
+        yield f"rows of a wider buffer, offset {off}", view, t
+    yield "without the last position", x[:, :-1], t[:, :-1]
+    yield "every second position", x[:, ::2], t[:, ::2]
+    yield "positions outermost", x.transpose(0, 1).contiguous().transpose(0, 1), t
+    yield "vocabulary outermost", x.permute(2, 0, 1).contiguous().permute(1, 2, 0), t
+    yield "one row for all", x[:1, :1].expand(3, 12, 1000), t
+    yield "two-dimensional", x.view(36, 1000), t.view(36)
+    yield "four-dimensional", x.view(3, 4, 3, 1000), t.view(3, 4, 3)
+    yield "four-dimensional, permuted", x.view(3, 4, 3, 1000).transpose(1, 2), \
+        t.view(3, 4, 3).transpose(1, 2)
+    odd = torch.zeros(3 * 12 * 1000 + 3, dtype=x.dtype, device=dev)[3:].view(3, 12, 1000)
+    odd.copy_(x)
+    yield "base off by three elements", odd, t
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_layouts(cuda_device, dtype):
+    for name, x, t in _layouts(cuda_device, dtype):
+        want, q = ref_logps(x, t)
+        x = x.detach().requires_grad_(True)
+        lp = ops.token_logprobs(x, t)
+        check_logps(lp.detach(), want, 1000)
+        (dx,) = torch.autograd.grad(lp.sum(), x)
+        check_dx(dx, x.detach(), q, torch.where(t == IGN, 0.0, 1.0).double(), onehot(t, 1000))
+        adv = torch.ones_like(want, dtype=torch.float32)
+        loss, lps, _, dx2 = ops.policy_loss_grad(x.detach(), t, None, adv)
+        n = (t != IGN).sum().double()
+        check_logps(lps, want, 1000)
+        check_dx(dx2, x.detach(), q, torch.where(t == IGN, 0.0, -1.0).double() / n, onehot(t, 1000))
+        assert abs(loss.item() + 1.0) <= 2 * U, name
+
+
+def test_ignored_rows_are_not_read(cuda_device):
+    for dtype in DT:
+        x, t, _ = make(cuda_device, 2, 24, 5000, dtype, ignore=0.5)
+        clean = ops.preference_loss_grad(x, t)
+        x2 = x.clone()
+        x2[t == IGN] = float("nan")
+        ref = torch.where(t == IGN, float("nan"), 0.0)
+        for a, b in zip(clean, ops.preference_loss_grad(x2, t, ref)):
+            assert torch.equal(a, b)
+        assert (clean[2][t == IGN] == 0).all()
+        adv = torch.where(t == IGN, float("inf"), 1.5)
+        old = torch.where(t == IGN, float("nan"), ops.token_logprobs(x, t))
+        loss, lps, kl, dx = ops.policy_loss_grad(x2, t, old, adv, ref)
+        assert torch.isfinite(loss) and torch.isfinite(kl) and torch.isfinite(dx.float()).all()
+        assert (lps[t == IGN] == 0).all() and (dx[t == IGN] == 0).all()
+        ids = torch.zeros(2, 24, 3, dtype=torch.int64, device=cuda_device)
+        ids[t == IGN] = 10 ** 12
+        tl = torch.where((t == IGN)[..., None], float("nan"), 1.0).expand(2, 24, 3)
+        loss, dx = ops.distill_loss_grad(x2, ids, tl, t != IGN)
+        assert torch.isfinite(loss) and (dx[t == IGN] == 0).all()
+
+
+@pytest.mark.parametrize("V", [130, 9001])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_infinities_and_lowest_values(cuda_device, dtype, V):
+    low = torch.finfo(DT[dtype]).min
+    x, t, _ = make(cuda_device, 1, 8, V, dtype, ignore=0)
+    t[:] = 3
+    x[0, 0, 10:] = float("-inf")         # most of the vocabulary masked
+    x[0, 1, :] = low                     # masked whole by the lowest value: uniform
+    x[0, 2, :] = low
+    x[0, 2, 3] = 0.0                     # one token left
+    x[0, 3, 3] = float("-inf")           # the target itself masked
+    x[0, 4, :] = float("-inf")           # nothing left: NaN, as log_softmax gives
+    x[0, 5, 7] = float("nan")
+    x[0, 6, 5] = float("inf")
+    for tau in (1.0, 0.5):
+        xr = x.clone().requires_grad_(True)
+        lp = ops.token_logprobs(xr, t, temperature=tau)
+        # lowest values overflow when divided by a temperature below 1: subtract the maximum first
+        z = x.double()
+        z = torch.log_softmax((z - z.amax(-1, keepdim=True)) / tau, -1)
+        want = z[..., 3]
+        got = lp.detach().double()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+        assert want.isnan().tolist()[0] == [False] * 4 + [True] * 3 + [False]
+        ok = torch.isfinite(want)
+        assert ((got - want).abs()[ok] <= (rel_s(V) + U * want.abs())[ok]).all()
+        (dx,) = torch.autograd.grad(lp, xr, torch.ones_like(lp))
+        assert dx[0, 4:7].isnan().all()
+        for r in (0, 1, 2, 3, 7):
+            q = z[0, r].exp()
+            mass = torch.zeros_like(q)
+            mass[3] = 1
+            err = (dx[0, r].double() - (mass - q) / tau).abs()
+            tol = (half_step(x.dtype) + 8 * U) * (mass - q).abs() / tau \
+                + (q * (rel_s(V) + 300 * U) + 2 * U * mass) / tau + 1e-37
+            assert (err <= tol).all(), (r, err.max())
+
+
+def ref_preference(x, t, ref, beta, e):
+    lp, q = ref_logps(x, t)
+    keep = (t != IGN)
+    d = torch.where(keep, lp - (0 if ref is None else ref.double()), 0.0)
+    P = x.shape[0] // 2
+    R = beta * d.sum(1)
+    h = R[:P] - R[P:]
+    sp = torch.nn.functional.softplus
+    loss = ((1 - e) * sp(-h) + e * sp(h)).mean()
+    dh = (e * torch.sigmoid(h) - (1 - e) * torch.sigmoid(-h)) * beta / P
+    k = torch.cat([dh, -dh])[:, None] * keep
+    return loss, R, k, q
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("P,S,V,beta,e", [(1, 1, 5, 0.1, 0.0), (1, 40, 1000, 0.1, 0.1),
+                                          (3, 33, 4099, 0.5, 0.0), (2, 70, 32000, 0.1, 0.2),
+                                          (1, 5, 128256, 5.0, 0.0), (160, 2, 300, 0.3, 0.1)])
+def test_preference(cuda_device, P, S, V, beta, e, dtype):
+    x, t, g = make(cuda_device, 2 * P, S, V, dtype)
+    if S > 1:
+        t[0, :] = IGN                    # a chosen sequence without a counted token
+    lp, _ = ref_logps(x, t)
+    refs = [None, (lp + torch.randn(lp.shape, device=x.device, generator=g,
+                                    dtype=torch.float64) * 0.2).float()]
+    for ref in refs:
+        loss, rewards, dx = ops.preference_loss_grad(x, t, ref, beta=beta, label_smoothing=e)
+        want, R, k, q = ref_preference(x, t, ref, beta, e)
+        n = (t != IGN).sum(1)
+        lp_err = rel_s(V) + U * lp.abs().amax(1)      # the log-probabilities pass through fp32
+        r_err = beta * n * lp_err
+        assert ((rewards.double() - R).abs() <= r_err + U * R.abs() + 1e-30).all()
+        h_err = (r_err[:P] + r_err[P:])
+        assert abs(loss.item() - want.item()) <= h_err.mean() + 2 * U * abs(want.item())
+        # sigma moves by at most its value times the error of h
+        slack = 1 + 2 * torch.cat([h_err, h_err])[:, None]
+        for scale in (1.0, 0.25):
+            got = dx if scale == 1.0 else ops.preference_loss_grad(
+                x, t, ref, beta=beta, label_smoothing=e, grad_scale=scale)[2]
+            a = k * scale
+            mass = onehot(t, V)
+            wantx = a[..., None] * (mass - q)
+            tol = (half_step(x.dtype) + 8 * U) * wantx.abs() \
+                + a.abs()[..., None] * (q * (rel_s(V) + 90 * U) + 2 * U * mass) \
+                + (slack - 1)[..., None] * (k.abs().amax() * scale) * (mass - q).abs() + 1e-37
+            assert ((got.double() - wantx).abs() <= tol).all()
+        xr = x.clone().requires_grad_(True)
+        l2, rw2 = ops.preference_loss(xr, t, ref, beta=beta, label_smoothing=e)
+        assert torch.equal(l2.detach(), loss) and torch.equal(rw2, rewards)
+        assert not rw2.requires_grad
+        (gx,) = torch.autograd.grad(l2, xr, torch.tensor(1.0, device=x.device))
+        assert torch.equal(gx, dx)
+
+
+def ref_policy(x, t, old, adv, ref, clip, kl_coef, tau, reduction):
+    lp, q = ref_logps(x, t, tau)
+    keep = t != IGN
+    A = adv.double() if adv.dim() == t.dim() else adv.double()[:, None].expand(t.shape)
+    n = keep.sum() if reduction == "token" else t.shape[0] * keep.sum(-1, keepdim=True)
+    w = torch.where(keep, 1.0 / n.clamp(min=1).double(), 0.0)
+    r = torch.exp(lp - old.double()) if old is not None else torch.ones_like(lp)
+    bent = r.clamp(1 - clip[0], 1 + clip[1])
+    surr = -torch.minimum(r * A, bent * A)
+    k = torch.where(r * A <= bent * A, -r * A, 0.0)
+    kl = torch.zeros_like(lp)
+    if ref is not None:
+        d = ref.double() - lp
+        kl = torch.expm1(d) - d
+        k = k - kl_coef * torch.expm1(d)
+    return (w * (surr + kl_coef * kl)).sum(), lp, (w * kl).sum(), w * k, q
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("B,S,V,tau,kl,reduction", [
+    (1, 1, 4, 1.0, 0.0, "token"), (3, 29, 777, 1.0, 0.1, "token"),
+    (4, 31, 4096, 0.8, 0.05, "sequence"), (2, 40, 32000, 1.0, 0.0, "token"),
+    (2, 6, 100277, 1.3, 0.2, "sequence"), (200, 3, 128, 1.0, 0.04, "sequence")])
+def test_policy(cuda_device, B, S, V, tau, kl, reduction, dtype):
+    x, t, g = make(cuda_device, B, S, V, dtype)
+    if B > 1:
+        t[1, :] = IGN                    # a sequence without a counted token
+    lp, _ = ref_logps(x, t, tau)
+    clip = (0.2, 0.3)
+    d = torch.randn(B, S, device=x.device, generator=g, dtype=torch.float64) * 0.2
+    for edge in (math.log(0.8), math.log(1.3)):   # the gradient jumps there
+        d = torch.where((d - edge).abs() < 1e-3, edge + 2e-3, d)
+    old = (lp - d).float()
+    ref = (lp + torch.randn(B, S, device=x.device, generator=g, dtype=torch.float64) * 0.3).float()
+    adv2 = torch.randn(B, S, device=x.device, generator=g)
+    adv1 = torch.randn(B, device=x.device, generator=g)
+    for o, adv, r in ((old, adv2, ref), (old, adv1, None), (None, adv1, ref)):
+        kw = dict(clip=clip, kl_coef=kl, temperature=tau, reduction=reduction)
+        loss, lps, klv, dx = ops.policy_loss_grad(x, t, o, adv, r, **kw)
+        want, wlp, wkl, k, q = ref_policy(x, t, o, adv, r, clip, kl, tau, reduction)
+        check_logps(lps, wlp, V)
+        # per token: |d loss / d lp| <= |coef|, second order below; kl's slope is |e^d - 1|
+        e_lp = rel_s(V)
+        s_abs = ref_policy(x, t, o, adv.abs(), r, (1.0, 1e6), kl, tau, reduction)
+        bound = 4 * e_lp * (s_abs[3].abs().sum() + 1e-3) + 2 * U * abs(want.item()) \
+            + 4 * U * s_abs[0].abs()
+        assert abs(loss.item() - want.item()) <= bound
+        assert abs(klv.item() - wkl.item()) <= bound + 2 * e_lp
+        a_max = (x.double().amax(-1) - x.double().amin(-1)).max().item() / tau * 1.4427
+        rel_q = rel_s(V) + (4 + 2.1 * a_max) * U
+        mass = onehot(t, V)
+        kk = (k / tau)[..., None]
+        # a coefficient moves by its token's |A| r + kl e^d times the log-probability's error
+        wobble = 4 * e_lp * (torch.where(t == IGN, 0.0, 1.0).double() * 4 * (adv.abs().max() + kl)
+                             / (tau * max(1, int((t != IGN).sum()) if reduction == "token"
+                                          else B)))[..., None]
+        wantx = kk * (mass - q)
+        tol = (half_step(x.dtype) + 8 * U) * wantx.abs() + (kk.abs() + wobble) * (q * rel_q) \
+            + wobble * (mass - q).abs() + 2 * U * kk.abs() * mass + 1e-37
+        assert ((dx.double() - wantx).abs() <= tol).all()
+        xr = x.clone().requires_grad_(True)
+        l2, lp2, kl2 = ops.policy_loss(xr, t, o, adv, r, **kw)
+        assert torch.equal(l2.detach(), loss) and torch.equal(lp2, lps) and torch.equal(kl2, klv)
+        (g1,) = torch.autograd.grad(l2, xr, torch.tensor(0.5, device=x.device))
+        err = (g1.double() - 0.5 * wantx).abs()
+        assert (err <= 0.5 * tol + 1e-37).all()
+
+
+def ref_distill(x, ids, tl, mask, tau):
+    V = x.shape[-1]
+    keep = mask.clone() if mask is not None else torch.ones(x.shape[:-1], dtype=torch.bool,
+                                                            device=x.device)
+    z = tl.double() / tau
+    empty = torch.isinf(tl).all(-1) & (tl < 0).all(-1)
+    lt = torch.log_softmax(torch.where(empty[..., None], 0.0, z), -1)
+    p = lt.exp() * ~empty[..., None]
+    _, q = ref_logps(x, torch.zeros(x.shape[:-1], dtype=torch.int64, device=x.device), tau)
+    lq = torch.log_softmax(x.double() / tau, -1).gather(-1, ids.clamp(0, V - 1).long())
+    terms = torch.where(p > 0, p * (lt - lq), 0.0).sum(-1)
+    n = max(1, int(keep.sum()))
+    loss = tau * tau * (terms * keep).sum() / n
+    mass = torch.zeros_like(q).scatter_add_(-1, ids.clamp(0, V - 1).long(), p)
+    k = (keep & ~empty).double() * (-tau / n)
+    return loss, k, mass, q
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("B,S,V,K,tau", [(1, 1, 3, 1, 1.0), (2, 9, 100, 7, 2.0),
+                                         (1, 20, 4099, 64, 1.0), (2, 16, 32000, 64, 2.0),
+                                         (1, 4, 50257, 1024, 4.0), (1, 2, 128256, 100, 1.0),
+                                         (70, 4, 96, 96, 3.0)])
+def test_distill(cuda_device, B, S, V, K, tau, dtype):
+    x, _, g = make(cuda_device, B, S, V, dtype)
+    noisy = x.float() + torch.randn(x.shape, device=x.device, generator=g)
+    tl, ids = torch.topk(noisy, min(K, V), -1)
+    mask = torch.rand(B, S, device=x.device, generator=g) > 0.3
+    mask.view(-1)[0] = True
+    cases = [(ids, tl, mask), (ids.int(), tl.bfloat16(), None)]
+    if K > 4:
+        dup, gone = ids.clone(), tl.clone()
+        dup[..., 2] = dup[..., 0]        # an index twice, one three times
+        dup[..., 3] = dup[..., 1]
+        dup[..., 4] = dup[..., 1]
+        gone[..., 5:] = float("-inf")    # short lists: padded with no entries
+        bad = dup.clone()
+        bad[..., 5:] = -1                # whatever index those hold
+        gone.view(-1, gone.shape[-1])[-1] = float("-inf")   # a row without any entry
+        cases += [(dup, tl, mask), (bad, gone, None)]
+    for i, v, m in cases:
+        loss, dx = ops.distill_loss_grad(x, i, v, m, temperature=tau)
+        want, k, mass, q = ref_distill(x, i, v, m, tau)
+        # weights p are rounded to fp32 once, log q carries rel_s; both enter times tau^2
+        assert abs(loss.item() - want.item()) <= tau * tau * (rel_s(V) + 60 * U) \
+            + 2 * U * abs(want.item())
+        a_max = (x.double().amax(-1) - x.double().amin(-1)).max().item() / tau * 1.4427
+        rel_q = rel_s(V) + (4 + 2.1 * a_max) * U
+        kk = k[..., None]
+        wantx = kk * (mass - q)
+        # masses of a repeated index add K roundings
+        tol = (half_step(x.dtype) + 8 * U) * wantx.abs() \
+            + kk.abs() * (q * rel_q + (4 + K) * U * mass) + 1e-37
+        assert ((dx.double() - wantx).abs() <= tol).all()
+        xr = x.clone().requires_grad_(True)
+        l2 = ops.distill_loss(xr, i, v, m, temperature=tau)
+        assert torch.equal(l2.detach(), loss)
+        (g1,) = torch.autograd.grad(l2 * 3.0, xr)
+        assert ((g1.double() - 3 * wantx).abs() <= 3 * tol).all()
+
+
+def test_gradients_against_differences(cuda_device):
+    """Central differences along a direction d, |d| <= 1: the third derivative of a
+    log-probability along it is at most 1 (a third cumulant of a variable in [-1, 1])
+    and the second at most 1, the first at most 2; with step e the quotient is off by e^2 / 6 of the
+    loss's third derivative and by 2 u |loss| / e."""
+    e = 2.0 ** -6
+    x, t, g = make(cuda_device, 2, 6, 333, "fp32", ignore=0.2)
+    d = torch.rand(x.shape, device=x.device, generator=g) * 2 - 1
+    d = (d * 64).round() / 64
+    x = (x * 1024).round() / 1024                     # x +- e d is exact
+    w = torch.randn(2, 6, device=x.device, generator=g).double()
+    old = ops.token_logprobs(x, t)
+    adv = torch.randn(2, 6, device=x.device, generator=g)
+    tl, ids = torch.topk(x + torch.randn(x.shape, device=x.device, generator=g), 9, -1)
+    n = int((t != IGN).sum())
+
+    def lp_sum(v):
+        return (ops.token_logprobs(v, t).double() * w).sum()
+
+    def pref(v):
+        return ops.preference_loss(v, t, beta=0.05)[0]
+
+    def pol(v):
+        return ops.policy_loss(v, t, old, adv, old - 0.1, clip=(1.0, 100.0), kl_coef=0.3)[0]
+
+    def dist(v):
+        return ops.distill_loss(v, ids, tl)
+
+    bt = 0.05 * n
+    third = {"lp": w.abs().sum().item(),
+             "pref": 0.1 * (2 * bt) ** 3 + 3 * 0.25 * 2 * bt * bt + bt,
+             "pol": (adv.abs().max().item() * 1.2 + 0.3 * 1.2) * (8 + 6 + 1),
+             "dist": 1.0}
+    for name, f in (("lp", lp_sum), ("pref", pref), ("pol", pol), ("dist", dist)):
+        xr = x.clone().requires_grad_(True)
+        loss = f(xr)
+        (gx,) = torch.autograd.grad(loss, xr)
+        slope = (gx.double() * d.double()).sum().item()
+        hi, lo = f(x + e * d).item(), f(x - e * d).item()
+        size = max(abs(hi), abs(lo)) if name != "lp" else w.abs().sum().item() * 20
+        # the gradient's own fp32 roundings: 60 u of each |entry|
+        own = 60 * U * (gx.double() * d.double()).abs().sum().item() + 10 * rel_s(333)
+        tol = e * e / 6 * third[name] + (2 * U * size + 2 * rel_s(333) * third[name]) / e + own
+        assert abs((hi - lo) / (2 * e) - slope) <= tol, (name, (hi - lo) / (2 * e), slope, tol)
+
+
+def test_no_counted_row(cuda_device):
+    x, t, _ = make(cuda_device, 2, 5, 400, "bf16")
+    t[:] = IGN
+    loss, lps, kl, dx = ops.policy_loss_grad(x, t, None, torch.ones(2, device=x.device))
+    assert loss.item() == 0 and kl.item() == 0 and not lps.any() and not dx.any()
+    ids = torch.zeros(2, 5, 3, dtype=torch.int64, device=x.device)
+    loss, dx = ops.distill_loss_grad(x, ids, ids.float(), torch.zeros_like(t, dtype=torch.bool))
+    assert loss.item() == 0 and not dx.any()
+    loss, rewards, dx = ops.preference_loss_grad(x, t)
+    assert abs(loss.item() - math.log(2)) <= U and not rewards.any() and not dx.any()
+    # no rows at all
+    x0, t0 = x[:, :0], t[:, :0]
+    assert ops.token_logprobs(x0, t0).shape == (2, 0)
+    assert ops.policy_loss_grad(x0, t0, None, torch.ones(2, device=x.device))[0].item() == 0
+    assert ops.distill_loss_grad(x0, ids[:, :0], ids[:, :0].float())[0].item() == 0
+    assert abs(ops.preference_loss_grad(x0, t0)[0].item() - math.log(2)) <= U
+    xr = x0.clone().requires_grad_(True)
+    (g,) = torch.autograd.grad(ops.token_logprobs(xr, t0).sum(), xr)
+    assert g.shape == x0.shape
+
+
+def test_out_of_range_index_is_an_error(cuda_device):
+    for bad in (400, -1, 2 ** 40):
+        x, t, _ = make(cuda_device, 2, 5, 400, "bf16", ignore=0)
+        t[0, 1] = bad
+        lp = ops.token_logprobs(x, t)
+        assert _native.device_error() == 0x106
+        assert lp[0, 1].isnan() and torch.isfinite(lp).sum() == 9
+        loss, _, dx = ops.preference_loss_grad(x, t)
+        assert _native.device_error() == 0x106 and loss.isnan() and dx[0].isnan().all()
+        loss, _, _, dx = ops.policy_loss_grad(x, t, None, torch.ones(2, device=x.device))
+        assert _native.device_error() == 0x106 and loss.isnan() and dx[0, 1].isnan().all()
+        assert torch.isfinite(dx[0, 0].float()).all()
+        ids = torch.zeros(2, 5, 3, dtype=torch.int64, device=x.device)
+        ids[0, 1, 2] = bad
+        loss, dx = ops.distill_loss_grad(x, ids, torch.ones(2, 5, 3, device=x.device))
+        assert _native.device_error() == 0x106 and loss.isnan() and dx[0, 1].isnan().all()
+        assert torch.isfinite(dx[0, 0].float()).all()
+
+
+def test_out_argument(cuda_device):
+    for dtype, V in (("bf16", 32000), ("bf16", 5003), ("fp32", 50257), ("bf16", 300001)):
+        x, t, _ = make(cuda_device, 2, 9, V, dtype)
+        adv = torch.ones(2, device=x.device)
+        tl, ids = torch.topk(x.float(), 8, -1)
+        for f in (lambda v, o: ops.policy_loss_grad(v, t, None, adv, out=o),
+                  lambda v, o: ops.preference_loss_grad(v, t, out=o),
+                  lambda v, o: ops.distill_loss_grad(v, ids, tl, t != IGN, out=o)):
+            want = f(x, None)
+            y = x.clone()
+            version = y._version
+            got = f(y, y)
+            assert got[-1] is y and y._version > version
+            for a, b in zip(want, got):
+                assert torch.equal(a, b)
+            guard = torch.full((2, 9, V + 5), 7.0, dtype=x.dtype, device=x.device)
+            f(x, guard[..., 3:3 + V])
+            assert torch.equal(guard[..., 3:3 + V], want[-1])
+            assert (guard[..., :3] == 7).all() and (guard[..., 3 + V:] == 7).all()
+    x, t, _ = make(cuda_device, 2, 9, 64, "bf16")
+    big = torch.empty(2, 10, 64, dtype=x.dtype, device=x.device)
+    for out in (x[:, :, :32], x.float(), big[:1, :9].expand(2, 9, 64),
+                torch.empty(2, 64, 9, dtype=x.dtype, device=x.device).transpose(1, 2),
+                x.clone().requires_grad_(True)):
+        with pytest.raises(ValueError):
+            ops.preference_loss_grad(x, t, out=out)
+    big[:, :9] = x
+    with pytest.raises(ValueError, match="shares"):
+        ops.preference_loss_grad(big[:, :9], t, out=big[:, 1:])
+
+
+def test_refusals(cuda_device):
+    x, t, _ = make(cuda_device, 2, 4, 50, "bf16")
+    f = torch.zeros(2, 4, device=x.device)
+    adv = torch.zeros(2, device=x.device)
+    ids = torch.zeros(2, 4, 3, dtype=torch.int64, device=x.device)
+    tl = ids.float()
+    with pytest.raises(TypeError):
+        ops.token_logprobs(x.half(), t)
+    with pytest.raises(TypeError):
+        ops.token_logprobs(x, t.int())
+    with pytest.raises(ValueError):
+        ops.token_logprobs(x, t[:, :3])
+    with pytest.raises(ValueError):
+        ops.token_logprobs(x[0, 0], t[0, 0])
+    with pytest.raises(ValueError):
+        ops.token_logprobs(x[..., :0], t)
+    with pytest.raises(RuntimeError):
+        ops.token_logprobs(x, t.cpu())
+    for tau in (0.0, -1.0, float("nan"), float("inf"), 1e-9):
+        with pytest.raises(_native.LemaError, match="temperature"):
+            ops.token_logprobs(x, t, temperature=tau)
+    with pytest.raises(ValueError):
+        ops.preference_loss(x[:1], t[:1])
+    with pytest.raises(ValueError):
+        ops.preference_loss(x.view(8, 50), t.view(8))
+    with pytest.raises(ValueError, match="detach"):
+        ops.preference_loss(x, t, f.clone().requires_grad_(True))
+    for kw in ({"beta": 0.0}, {"beta": float("nan")}, {"label_smoothing": 0.5},
+               {"label_smoothing": -0.1}):
+        with pytest.raises(_native.LemaError):
+            ops.preference_loss(x, t, **kw)
+    with pytest.raises(ValueError):
+        ops.policy_loss(x, t, f, torch.zeros(4, device=x.device))
+    with pytest.raises(ValueError):
+        ops.policy_loss(x, t, f, adv.double())
+    with pytest.raises(ValueError):
+        ops.policy_loss(x, t, f, adv, reduction="mean")
+    for kw in ({"clip": (-0.1, 0.2)}, {"clip": (0.2, float("inf"))}, {"clip": (1.5, 0.2)},
+               {"kl_coef": -1.0}):
+        with pytest.raises(_native.LemaError):
+            ops.policy_loss(x, t, f, adv, **kw)
+    with pytest.raises(TypeError):
+        ops.distill_loss(x, ids.float(), tl)
+    with pytest.raises(ValueError):
+        ops.distill_loss(x, ids, tl[..., :2])
+    with pytest.raises(TypeError):
+        ops.distill_loss(x, ids, tl, torch.ones(2, 4, device=x.device))
+    with pytest.raises(_native.LemaError):
+        ops.distill_loss(x, ids[..., :0], tl[..., :0])
+    with pytest.raises(_native.LemaError):
+        big = torch.zeros(2, 4, 1025, device=x.device)
+        ops.distill_loss(x, big.long(), big)
+
+
+def test_autograd_use(cuda_device):
+    """Twice through a retained graph, a modified input, no second derivative, an
+    expanded upstream gradient, a loss added to others."""
+    x, t, _ = make(cuda_device, 2, 6, 700, "fp32")
+    xr = x.clone().requires_grad_(True)
+    loss, _ = ops.preference_loss(xr, t)
+    (a,) = torch.autograd.grad(loss, xr, retain_graph=True)
+    (b,) = torch.autograd.grad(loss, xr)
+    assert torch.equal(a, b)
+    lp = ops.token_logprobs(xr, t)
+    (s,) = torch.autograd.grad(lp.sum(), xr, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(s.sum(), xr)
+    y = (x * 1.0).requires_grad_(True)
+    z = y * 1.0
+    lp = ops.token_logprobs(z, t)
+    z.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        lp.sum().backward()
+    h = x.clone().requires_grad_(True)
+    w = torch.randn(700, 700, device=x.device) * 0.02
+    logits = (h @ w).bfloat16()
+    total = ops.policy_loss(logits, t, None, torch.ones(2, device=x.device))[0] \
+        - ops.token_logprobs(logits, t).mean()
+    total.backward()
+    assert torch.isfinite(h.grad).all() and h.grad.abs().sum() > 0
+
+
+def test_same_bits_every_time(cuda_device):
+    x, t, _ = make(cuda_device, 4, 150, 8200, "bf16")
+    tl, ids = torch.topk(x.float(), 32, -1)
+    ids[..., 7] = ids[..., 3]
+    adv = torch.randn(4, device=x.device)
+    for f in (lambda: ops.preference_loss_grad(x, t), lambda: ops.distill_loss_grad(x, ids, tl),
+              lambda: ops.policy_loss_grad(x, t, None, adv, reduction="sequence")):
+        first = f()
+        for _ in range(3):
+            for a, b in zip(first, f()):
+                assert torch.equal(a, b)
+
+
+def test_streams_and_graphs(cuda_device):
+    """On another stream than the default; captured, replayed on new inputs; two graphs
+    captured one after the other and replayed at once (each has its own workspace)."""
+    dev = cuda_device
+    data = [make(dev, 4, 40, 5000, "bf16", seed=s) for s in range(4)]
+    adv = torch.randn(4, device=dev)
+    want = [(ops.preference_loss_grad(x, t), ops.policy_loss_grad(x, t, None, adv))
+            for x, t, _ in data]
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        got = ops.preference_loss_grad(data[1][0], data[1][1])
+    side.synchronize()
+    for a, b in zip(want[1][0], got):
+        assert torch.equal(a, b)
+    graphs = []
+    for i in range(2):
+        x, t = data[i][0].clone(), data[i][1].clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs = (ops.preference_loss_grad(x, t), ops.policy_loss_grad(x, t, None, adv))
+        graphs.append((g, x, t, outs))
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    for round_ in (0, 2):
+        for (g, x, t, _), (nx, nt, _) in zip(graphs, data[round_:round_ + 2]):
+            x.copy_(nx)
+            t.copy_(nt)
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for s, (g, *_) in zip(streams, graphs):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for (_, _, _, outs), w in zip(graphs, want[round_:round_ + 2]):
+            for a, b in zip([v for o in outs for v in o], [v for o in w for v in o]):
+                assert torch.equal(a, b)
+
+
+def test_backward_in_a_graph(cuda_device):
+    """Forward and backward of the autograd form captured together."""
+    x, t, _ = make(cuda_device, 2, 30, 3000, "bf16")
+    want = ops.preference_loss_grad(x, t)
+    xr = x.clone().requires_grad_(True)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        loss, _ = ops.preference_loss(xr, t)
+        (dx,) = torch.autograd.grad(loss, xr)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(loss.detach(), want[0]) and torch.equal(dx, want[2])
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """More than 2^31 logits: the last rows against their own small call."""
+    T, V = 68000, 32000
+    x = torch.zeros(T, V, dtype=torch.bfloat16, device=cuda_device)
+    t = torch.full((T,), IGN, device=cuda_device)
+    tail, tt, _ = make(cuda_device, 1, 6, V, "bf16", ignore=0)
+    x[-6:] = tail[0]
+    t[-6:] = tt[0]
+    adv = torch.ones(T, device=cuda_device)
+    want = ops.policy_loss_grad(tail[0], tt[0], None, adv[:6])
+    loss, lps, _, dx = ops.policy_loss_grad(x, t, None, adv, out=x)
+    assert torch.equal(loss, want[0]) and torch.equal(lps[-6:], want[1])
+    assert torch.equal(dx[-6:], want[3]) and not lps[:-6].any() and not dx[:-6].any()
