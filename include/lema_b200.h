@@ -385,22 +385,13 @@ LEMA_API int lema_policy_loss(const void* x, int32_t x_f32, int64_t n0, int64_t 
  * teacher_ids [n0, n1, K] int64 (ids_i32: int32), teacher_logits [n0, n1, K] bf16
  * (tl_f32 = 0) or fp32, mask [n0, n1] bytes (0: row not counted; NULL: all count).
  * Entries of logit -inf have no weight, whatever their index; a row of them alone
- * contributes 0. An index that repeats adds its weights. stats / coef (may be NULL):
- * the inputs of lema_distill_loss_bwd. */
+ * contributes 0. An index that repeats adds its weights. */
 LEMA_API int lema_distill_loss(const void* x, int32_t x_f32, int64_t n0, int64_t n1, int64_t ld0,
                                int64_t ld1, int64_t V, const void* teacher_ids, int32_t ids_i32,
                                const void* teacher_logits, int32_t tl_f32, int64_t K,
                                const uint8_t* mask, double temperature, double grad_scale,
-                               void* ws, int64_t ws_bytes, float* stats, float* coef, float* loss,
+                               const float* upstream, void* ws, int64_t ws_bytes, float* loss,
                                void* dx, int64_t ldd0, int64_t ldd1, void* stream);
-
-/* dx of lema_distill_loss from its stats and coef. */
-LEMA_API int lema_distill_loss_bwd(const void* x, int32_t x_f32, int64_t n0, int64_t n1,
-                                   int64_t ld0, int64_t ld1, int64_t V, const void* teacher_ids,
-                                   int32_t ids_i32, const void* teacher_logits, int32_t tl_f32,
-                                   int64_t K, const uint8_t* mask, double temperature,
-                                   const float* stats, const float* coef, const float* upstream,
-                                   void* dx, int64_t ldd0, int64_t ldd1, void* stream);
 
 /* ---- K6: grouped W8A8 GEMM (MoE experts) -------------------------------- */
 /* Tokens are pre-sorted by expert: rows [offsets[e], offsets[e+1]) of xq/sx/y

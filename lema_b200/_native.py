@@ -77,10 +77,8 @@ _SIGNATURES: dict[str, list] = {
                                        vp, i64, i64, vp],
     "lema_policy_loss": _LOGITS + [vp, i64, f64, vp, vp, i64, i64, vp, f64, f64, f64, i32, f64,
                                    vp, i64, vp, vp, vp, vp, vp, vp, i64, i64, vp],
-    "lema_distill_loss": _LOGITS + [vp, i32, vp, i32, i64, vp, f64, f64, vp, i64, vp, vp, vp, vp,
+    "lema_distill_loss": _LOGITS + [vp, i32, vp, i32, i64, vp, f64, f64, vp, vp, i64, vp, vp,
                                     i64, i64, vp],
-    "lema_distill_loss_bwd": _LOGITS + [vp, i32, vp, i32, i64, vp, f64, vp, vp, vp, vp, i64, i64,
-                                        vp],
     "lema_ckpt_save": [vp, vp, sz, i32, vp, vp, vp],
     "lema_ckpt_restore": [vp, vp, sz, vp, vp, vp],
     "lema_mm_create": [i64, i64, i32, C.POINTER(vp)],
@@ -164,7 +162,6 @@ KERNELS_PER_CALL = {
     "lema_adamw_requant_rows": 1, "lema_device_error_async": 1, "lema_attn_fwd": 1,
     "lema_attn_bwd": 3, "lema_token_logprobs": 1, "lema_token_logprobs_bwd": 1,
     "lema_preference_loss": 3, "lema_policy_loss": 3, "lema_distill_loss": 3,
-    "lema_distill_loss_bwd": 1,
 }
 # Running count of this library's kernel launches issued by this process.
 kernel_launches = 0
@@ -222,6 +219,7 @@ DEVICE_ERROR_NAMES = {
     0x104: "a split GEMM tile's partial accumulators never arrived",
     0x105: "an attention kernel timed out waiting for a tile, a score buffer or P",
     0x106: "a loss was given a target or teacher index outside the vocabulary",
+    0x107: "a loss kernel timed out waiting for a row or for its cluster",
 }
 
 

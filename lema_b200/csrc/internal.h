@@ -41,6 +41,7 @@ enum DeviceErr : int32_t {
   kDevErrSplitTimeout = 0x104,  // a split tile's partial accumulators never arrived
   kDevErrAttnTimeout = 0x105,   // an attention kernel's wait ran out
   kDevErrIndex = 0x106,         // a loss's target or teacher index lies outside the vocabulary
+  kDevErrLossTimeout = 0x107,   // a loss kernel's wait for a row or its cluster ran out
 };
 
 // While alive, GEMMs issued by this thread run every tile whole (no split-K

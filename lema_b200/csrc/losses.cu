@@ -23,6 +23,7 @@
 #include <cuda_bf16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "internal.h"
@@ -42,11 +43,11 @@ struct RowMap {
   }
 };
 
-// Workspace: head, counted rows of each sequence, partial sums of token_kernel's CTAs, what
-// each row leaves for it.
+// Workspace: head, counted rows of each sequence, the list of rows, partial sums of
+// token_kernel's CTAs, what each row leaves for it.
 struct WsHead {
-  int64_t total;    // rows that count
-  uint32_t ticket;  // CTAs of token_kernel / pair_kernel that are done
+  unsigned long long total, out;  // rows that count, and that do not
+  uint32_t ticket;                // CTAs of token_kernel that are done
 };
 constexpr int64_t kWsHead = 256;
 constexpr int kTokenThreads = 256;
@@ -65,7 +66,7 @@ struct RowArgs {
   int64_t T;
   int32_t V;
   double inv_tau;                // 1 / tau
-  float c;                       // log2(e) / tau
+  float c, c_lo;                 // log2(e) / tau, rounded, and what the rounding left
   const int64_t* targets;        // [T]; null for distill
   int64_t ignore;
   float* logps;                  // [T]
@@ -79,7 +80,8 @@ struct RowArgs {
   float grad_scale;
   int32_t* err;
   WsHead* head;
-  int32_t* seq_count;            // [n0] counted rows of each sequence
+  int32_t* seq_count;            // [n0] counted rows of each sequence (per_sequence only)
+  int32_t* list;                 // [T] the rows that count, then the others
   float* loss;
   float* kl;
   // policy
@@ -116,9 +118,9 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // ---- 16-byte vectors of a row ---------------------------------------------------
-// A row may start at any element. It is read as the aligned 16-byte vectors that hold it: the
-// first and the last may also hold neighbours' elements, which are replaced by -inf (they
-// share a 16-byte granule with the row, so the load stays inside the allocation's pages).
+// A row may start at any element: its aligned 16-byte vectors are moved whole, the elements in
+// front of the first and behind the last (its edges, fewer than a vector each) one by one, by
+// the threads 0 .. kEdges - 1 of whoever holds the row.
 
 template <typename T>
 struct Vec;
@@ -160,33 +162,37 @@ struct Vec<float> {
   }
 };
 
+constexpr int kEdges = 16;  // edge e: element e of the head (e < 8), or e - 8 of the tail
+
 template <typename T>
 struct Span {
-  const uint4* v0;  // the row's first aligned vector
-  int lead;         // elements in front of the row in it
-  int nvec;
-  int V;
-  __device__ __forceinline__ Span(const T* x, int V_) : V(V_) {
-    const uintptr_t p = reinterpret_cast<uintptr_t>(x);
-    v0 = reinterpret_cast<const uint4*>(p & ~uintptr_t{15});
-    lead = static_cast<int>((p & 15u) / sizeof(T));
-    nvec = (lead + V + Vec<T>::kE - 1) / Vec<T>::kE;
+  int head, nvec, tail;  // elements, vectors, elements
+  __device__ __forceinline__ Span(const T* x, int V) {
+    const int to_go = static_cast<int>((16u - (reinterpret_cast<uintptr_t>(x) & 15u)) & 15u);
+    head = min(V, to_go / static_cast<int>(sizeof(T)));
+    nvec = (V - head) / Vec<T>::kE;
+    tail = V - head - nvec * Vec<T>::kE;
   }
-  // Elements of vector v outside the row become -inf.
-  __device__ __forceinline__ void clean(uint4& w, int v) const {
-    if (v == 0 || v == nvec - 1) {
-      T e[Vec<T>::kE];
-      *reinterpret_cast<uint4*>(e) = w;
-      const T neg_inf = static_cast<T>(-INFINITY);
-#pragma unroll
-      for (int j = 0; j < Vec<T>::kE; ++j) {
-        const int i = v * Vec<T>::kE + j - lead;
-        if (i < 0 || i >= V) e[j] = neg_inf;
-      }
-      w = *reinterpret_cast<const uint4*>(e);
-    }
+  __device__ __forceinline__ const uint4* vecs(const T* x) const {
+    return reinterpret_cast<const uint4*>(x + head);
+  }
+  // The element that is edge e, or -1.
+  __device__ __forceinline__ int edge(int e) const {
+    if (e < 8) return e < head ? e : -1;
+    return e - 8 < tail ? head + nvec * Vec<T>::kE + e - 8 : -1;
+  }
+  // Which thread of G holds element i (vectors are dealt round robin).
+  __device__ __forceinline__ int owner(int i, int G) const {
+    if (i < head) return i;
+    const int v = (i - head) / Vec<T>::kE;
+    return v < nvec ? v % G : i - head - nvec * Vec<T>::kE + 8;
   }
 };
+
+template <typename T>
+__device__ __forceinline__ uint4 neg_inf_vec() {
+  return make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
+}
 
 __device__ __forceinline__ uint4 ld16(const uint4* p) {
   uint4 r;
@@ -196,34 +202,41 @@ __device__ __forceinline__ uint4 ld16(const uint4* p) {
   return r;
 }
 
-// exp((x - m) / tau) of a vector's elements, as packed fp32 pairs: the maximum is taken off
-// first, so that rows of the type's lowest value stay finite.
-template <typename T>
-__device__ __forceinline__ void exp_vec(const uint4& w, uint64_t neg_m2, uint64_t c2,
+// 2^((x - m) c), c = log2(e) / tau, for the elements of a vector as packed fp32 pairs. The
+// maximum is taken off first, so that rows of the type's lowest value stay finite.
+//
+// FULL carries c as two fp32. Its rounding alone shifts every log-probability the same way
+// (2e-8 of (x - m) at tau = 1), which a sum over a sequence does not average out: the rewards of
+// 640-token sequences were 5e-6 off with c alone, 1e-6 with both. x - m is then kept above
+// -1e30, where the result is 0 all the same, because -inf times the second part would be NaN.
+struct ExpScale {
+  uint64_t neg_m, c, c_lo;
+  __device__ __forceinline__ ExpScale(float m, float c_, float c_lo_)
+      : neg_m(f2_splat(m == -INFINITY ? 0.f : -m)), c(f2_splat(c_)), c_lo(f2_splat(c_lo_)) {}
+};
+__device__ __forceinline__ float keep_finite(float d) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(d), "f"(-1e30f));
+  return r;
+}
+template <bool FULL>
+__device__ __forceinline__ uint64_t exp_pair(uint64_t x, const ExpScale& k) {
+  uint64_t d = f2_add(x, k.neg_m);
+  float lo, hi;
+  if (FULL) {
+    f2_unpack(d, lo, hi);
+    d = f2_pack(keep_finite(lo), keep_finite(hi));
+    f2_unpack(f2_fma(d, k.c, f2_mul(d, k.c_lo)), lo, hi);
+  } else {
+    f2_unpack(f2_mul(d, k.c), lo, hi);
+  }
+  return f2_pack(ex2(lo), ex2(hi));
+}
+template <typename T, bool FULL>
+__device__ __forceinline__ void exp_vec(const uint4& w, const ExpScale& k,
                                         uint64_t (&e)[Vec<T>::kE / 2]) {
 #pragma unroll
-  for (int i = 0; i < Vec<T>::kE / 2; ++i) {
-    float lo, hi;
-    f2_unpack(f2_mul(f2_add(Vec<T>::pair(w, i), neg_m2), c2), lo, hi);
-    e[i] = f2_pack(ex2(lo), ex2(hi));
-  }
-}
-
-// Writes vector v (elements of a row at `dst`, whose phase within 16 bytes is the input row's
-// when SAME): whole vectors at once, the row's ends element by element.
-template <typename T>
-__device__ __forceinline__ void store_vec(T* dst, const Span<T>& sp, int v, const uint4& w,
-                                          bool same) {
-  const int i0 = v * Vec<T>::kE - sp.lead;
-  if (same && i0 >= 0 && i0 + Vec<T>::kE <= sp.V) {
-    *reinterpret_cast<uint4*>(dst + i0) = w;
-  } else {
-    T e[Vec<T>::kE];
-    *reinterpret_cast<uint4*>(e) = w;
-#pragma unroll
-    for (int j = 0; j < Vec<T>::kE; ++j)
-      if (i0 + j >= 0 && i0 + j < sp.V) dst[i0 + j] = e[j];
-  }
+  for (int i = 0; i < Vec<T>::kE / 2; ++i) e[i] = exp_pair<FULL>(Vec<T>::pair(w, i), k);
 }
 
 template <typename T>
@@ -231,18 +244,12 @@ __device__ __forceinline__ bool same_phase(const T* a, const T* b) {
   return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15u) == 0;
 }
 
-// Adds k to element i of the row (a point mass) if vector v holds it.
+// A vector whose output row starts at another phase within 16 bytes than the input row.
 template <typename T>
-__device__ __forceinline__ void add_mass(uint64_t (&g)[Vec<T>::kE / 2], int at, float k) {
-  // `at`: the element's place in the vector, outside [0, kE) for all but one vector
+__device__ __noinline__ void store_apart(T* dst, uint4 w) {
+  const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
-  for (int i = 0; i < Vec<T>::kE / 2; ++i) {
-    float lo, hi;
-    f2_unpack(g[i], lo, hi);
-    lo += at == 2 * i ? k : 0.f;
-    hi += at == 2 * i + 1 ? k : 0.f;
-    g[i] = f2_pack(lo, hi);
-  }
+  for (int j = 0; j < Vec<T>::kE; ++j) dst[j] = e[j];
 }
 
 // ---- reductions ------------------------------------------------------------------
@@ -269,66 +276,76 @@ __device__ __forceinline__ double block_sum_d(double v, double* red) {
   return r;
 }
 
-// Maximum and sum of a row from each thread's (m, s); every thread gets both. The threads'
-// sums are added in fp64.
-template <int THREADS>
-__device__ __forceinline__ void block_combine(float& m, double& s, float c, float* redf,
+// Barrier of a group of G threads: a warp, or the whole CTA.
+template <int G>
+__device__ __forceinline__ void group_sync() {
+  if (G == 32)
+    __syncwarp();
+  else
+    __syncthreads();
+}
+
+// Maximum and sum of a row from the (m, s) of a group's threads; every thread gets both. The
+// threads' sums are added in fp64.
+template <int G>
+__device__ __forceinline__ void group_combine(float& m, double& s, float c, float* redf,
                                               double* redd) {
   const float mt = m;
+  const int warp = (threadIdx.x % G) >> 5;
   m = warp_max(m);
-  if (THREADS > 32) {
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) redf[threadIdx.x >> 5] = m;
-    __syncthreads();
+  if (G > 32) {
+    group_sync<G>();
+    if ((threadIdx.x & 31) == 0) redf[warp] = m;
+    group_sync<G>();
     m = redf[0];
 #pragma unroll
-    for (int w = 1; w < THREADS / 32; ++w) m = fmaxf(m, redf[w]);
+    for (int w = 1; w < G / 32; ++w) m = fmaxf(m, redf[w]);
   }
   // a thread that saw only -inf adds nothing; a row of -inf alone becomes NaN
   s *= static_cast<double>(ex2((mt - m) * c));
   s = warp_sum(s);
-  if (THREADS > 32) {
-    if ((threadIdx.x & 31) == 0) redd[threadIdx.x >> 5] = s;
-    __syncthreads();
+  if (G > 32) {
+    if ((threadIdx.x & 31) == 0) redd[warp] = s;
+    group_sync<G>();
     s = redd[0];
 #pragma unroll
-    for (int w = 1; w < THREADS / 32; ++w) s += redd[w];
+    for (int w = 1; w < G / 32; ++w) s += redd[w];
   }
 }
 
-// One thread's share of a row's maximum and sum: vectors tid, tid + STEP, ..., in one sweep with
-// a running maximum, U loads in flight.
-template <typename T, int STEP, int U>
-__device__ __forceinline__ void thread_stats(const Span<T>& sp, int tid, float c, float& m,
-                                             double& s) {
+// One thread's share of a row's maximum and sum: its edge and the vectors tid, tid + G, ..., in
+// one sweep with a running maximum, U loads in flight.
+template <typename T, int G, int U, bool FULL>
+__device__ __forceinline__ void thread_stats(const T* x, const Span<T>& sp, int tid, float c,
+                                             float c_lo, float& m, double& s) {
+  const uint4* xv = sp.vecs(x);
   m = -INFINITY;
   float sum = 0.f;
-  const uint64_t c2 = f2_splat(c);
-  for (int base = tid; base < sp.nvec; base += STEP * U) {
+  if (sp.head + sp.tail > 0 && tid < kEdges) {
+    const int i = sp.edge(tid);
+    if (i >= 0) {
+      m = to_f(x[i]);
+      // 1, or NaN for an element without a value; an element of -inf adds nothing
+      sum = m == -INFINITY ? 0.f : m - m + 1.f;
+      if (m != m) m = -INFINITY;
+    }
+  }
+  for (int base = tid; base < sp.nvec; base += G * U) {
     uint4 w[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int v = base + u * STEP;
-      if (v < sp.nvec)
-        w[u] = ld16(sp.v0 + v);
-      else
-        w[u] = make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
-    }
+    for (int u = 0; u < U; ++u)
+      w[u] = base + u * G < sp.nvec ? ld16(xv + base + u * G) : neg_inf_vec<T>();
     float mx = m;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      sp.clean(w[u], base + u * STEP);
-      mx = fmaxf(mx, Vec<T>::max(w[u]));
-    }
-    const float mm = mx == -INFINITY ? 0.f : mx;
-    sum *= ex2((m - mm) * c);
+    for (int u = 0; u < U; ++u) mx = fmaxf(mx, Vec<T>::max(w[u]));
+    sum *= ex2((m - (mx == -INFINITY ? 0.f : mx)) * c);
     m = mx;
-    const uint64_t neg_m2 = f2_splat(-mm);
+    const ExpScale k(m, c, c_lo);
     uint64_t acc = f2_splat(0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       uint64_t e[Vec<T>::kE / 2];
-      exp_vec<T>(w[u], neg_m2, c2, e);
+      exp_vec<T, FULL>(w[u], k, e);
 #pragma unroll
       for (int i = 0; i < Vec<T>::kE / 2; ++i) acc = f2_add(acc, e[i]);
     }
@@ -365,14 +382,24 @@ __device__ __forceinline__ double token_weight(const RowArgs& a, int64_t r) {
   return 1.0 / static_cast<double>(n);
 }
 
+// What the clipped policy loss knows of a token besides its log-probability.
+struct Token {
+  float adv, old, ref;
+};
+__device__ __forceinline__ Token load_token(const RowArgs& a, int64_t r) {
+  const int64_t b = r / a.in.n1, t = r % a.in.n1;
+  return Token{a.adv[b * a.adv_s0 + t * a.adv_s1], a.old_logps ? a.old_logps[r] : 0.f,
+               a.ref_logps ? a.ref_logps[r] : 0.f};
+}
+
 // dL/dlp of one token of the clipped policy loss over its weight, and (LOSS) its loss and KL.
 // F = double for what is returned, float for the gradient's coefficient.
 template <typename F, bool LOSS>
-__device__ __forceinline__ F policy_token(const RowArgs& a, int64_t r, F lp, F* loss, F* kl) {
-  const int64_t b = r / a.in.n1, t = r % a.in.n1;
-  const F A = a.adv[b * a.adv_s0 + t * a.adv_s1];
+__device__ __forceinline__ F policy_token(const RowArgs& a, const Token& tk, F lp, F* loss,
+                                          F* kl) {
+  const F A = tk.adv;
   // on-policy the ratio is 1, and NaN for a log-probability that is not finite
-  const F ratio = exp(lp - (a.old_logps ? static_cast<F>(a.old_logps[r]) : lp));
+  const F ratio = exp(lp - (a.old_logps ? static_cast<F>(tk.old) : lp));
   const F lo = static_cast<F>(1.0 - a.clip_lo), hi = static_cast<F>(1.0 + a.clip_hi);
   const F bent = ratio < lo ? lo : (ratio > hi ? hi : ratio);  // a NaN ratio stays NaN
   const F plain = ratio * A, clipped = bent * A;
@@ -380,7 +407,7 @@ __device__ __forceinline__ F policy_token(const RowArgs& a, int64_t r, F lp, F* 
   F coef = use_plain ? -plain : F(0);
   F d_kl = F(0);
   if (a.ref_logps) {
-    const F d = static_cast<F>(a.ref_logps[r]) - lp;
+    const F d = static_cast<F>(tk.ref) - lp;
     const F e = expm1(d);
     d_kl = e - d;
     coef -= static_cast<F>(a.kl_coef) * e;
@@ -394,220 +421,827 @@ __device__ __forceinline__ F policy_token(const RowArgs& a, int64_t r, F lp, F* 
 
 // ---- kernels ---------------------------------------------------------------------
 
-// Counts the rows that enter the loss: in all, and for each sequence of n1 rows. Clears the
-// ticket.
-__global__ void __launch_bounds__(1024) count_kernel(RowArgs a) {
-  __shared__ double red[32];
-  if (a.seq_count != nullptr && a.per_sequence)
-    for (int64_t b = threadIdx.x; b < a.n0; b += blockDim.x) a.seq_count[b] = 0;
-  if (threadIdx.x == 0) a.head->ticket = 0;
-  __syncthreads();
-  double n = 0;
-  for (int64_t r0 = 0; r0 < a.T; r0 += blockDim.x) {
-    const int64_t r = r0 + threadIdx.x;
-    int64_t target;
-    if (r < a.T && row_counts(a, r, target)) {
-      n += 1;
-      if (a.per_sequence) atomicAdd(&a.seq_count[r / a.in.n1], 1);
+// Lists the rows that enter the loss (list[0 .. total)), then the others from the end
+// backwards, and counts them for each sequence. One CTA, which clears the counters itself, or
+// several over counters cleared before; the order of the list, which the atomics then leave
+// open, moves no result. A thread takes kCountRows rows at once: two barriers for 8192 rows.
+constexpr int kCountThreads = 1024;
+constexpr int kCountRows = 8;
+constexpr int kCountBlock = kCountThreads * kCountRows;
+__global__ void __launch_bounds__(kCountThreads) count_kernel(RowArgs a) {
+  constexpr int kCells = kCountRows * kCountThreads / 32;  // a warp's rows at one offset
+  __shared__ int32_t s_cell[kCells];
+  __shared__ int64_t s_base, s_base_out;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (gridDim.x == 1) {
+    if (a.per_sequence)
+      for (int64_t b = tid; b < a.n0; b += kCountThreads) a.seq_count[b] = 0;
+    if (tid == 0) {
+      a.head->ticket = 0;
+      a.head->total = 0;
+      a.head->out = 0;
     }
+    __syncthreads();
   }
-  const double total = block_sum_d(n, red);
-  if (threadIdx.x == 0) a.head->total = static_cast<int64_t>(total);
+  for (int64_t r0 = blockIdx.x * int64_t{kCountBlock}; r0 < a.T;
+       r0 += gridDim.x * int64_t{kCountBlock}) {
+    bool in[kCountRows];
+#pragma unroll
+    for (int j = 0; j < kCountRows; ++j) {
+      const int64_t r = r0 + j * kCountThreads + tid;
+      int64_t target;
+      in[j] = r < a.T && row_counts(a, r, target);
+    }
+    uint32_t ballot[kCountRows];
+#pragma unroll
+    for (int j = 0; j < kCountRows; ++j) {
+      ballot[j] = __ballot_sync(0xffffffffu, in[j]);
+      if (lane == 0) s_cell[j * 32 + warp] = __popc(ballot[j]);
+      if (a.per_sequence) {
+        const int64_t r = r0 + j * kCountThreads + tid, b = r / a.in.n1;
+        // a warp inside one sequence adds once
+        const bool one = (r - lane) / a.in.n1 == (r - lane + 31) / a.in.n1;
+        if (one ? lane == 0 && ballot[j] != 0 : in[j])
+          atomicAdd(&a.seq_count[b], one ? __popc(ballot[j]) : 1);
+      }
+    }
+    __syncthreads();
+    if (warp == 0) {
+      int n[kCells / 32], sum = 0;
+#pragma unroll
+      for (int j = 0; j < kCells / 32; ++j) {
+        n[j] = s_cell[lane * (kCells / 32) + j];
+        sum += n[j];
+      }
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      int at = incl - sum;
+#pragma unroll
+      for (int j = 0; j < kCells / 32; ++j) {
+        s_cell[lane * (kCells / 32) + j] = at;
+        at += n[j];
+      }
+      if (lane == 31) {
+        const int64_t rows = a.T - r0 < kCountBlock ? a.T - r0 : kCountBlock;
+        s_base = static_cast<int64_t>(
+            atomicAdd(&a.head->total, static_cast<unsigned long long>(incl)));
+        s_base_out = static_cast<int64_t>(
+            atomicAdd(&a.head->out, static_cast<unsigned long long>(rows - incl)));
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kCountRows; ++j) {
+      const int place = j * kCountThreads + tid;
+      const int64_t r = r0 + place;
+      // counted rows of this block in front of r
+      const int rank = s_cell[j * 32 + warp] + __popc(ballot[j] & ((1u << lane) - 1u));
+      if (in[j])
+        a.list[s_base + rank] = static_cast<int32_t>(r);
+      else if (r < a.T)
+        a.list[a.T - 1 - (s_base_out + place - rank)] = static_cast<int32_t>(r);
+    }
+    __syncthreads();
+  }
 }
 
-// A row that does not count.
-template <typename T, int THREADS>
+// A gradient row of zeros.
+template <typename T, int G>
 __device__ __forceinline__ void zero_row(const RowArgs& a, int64_t r, int tid) {
-  if (tid == 0) {
-    if (a.logps) a.logps[r] = 0.f;
-    if (a.stats) a.stats[r] = make_float2(0.f, 0.f);
-    if (a.coef) a.coef[r] = 0.f;
-  }
   if (a.dx == nullptr) return;
   T* dx = static_cast<T*>(a.dx) + a.out.at(r);
   const Span<T> so(dx, a.V);
-  for (int v = tid; v < so.nvec; v += THREADS)
-    store_vec<T>(dx, so, v, make_uint4(0u, 0u, 0u, 0u), true);
+  uint4* dv = reinterpret_cast<uint4*>(dx + so.head);
+  for (int v = tid; v < so.nvec; v += G) dv[v] = make_uint4(0u, 0u, 0u, 0u);
+  if (tid < kEdges && so.edge(tid) >= 0) put(dx + so.edge(tid), 0.f);
 }
 
-// token_logprobs: one CTA a row.
+// token_logprobs: a group of G threads a row, a warp for short rows (one CTA a row leaves most
+// of its threads without a vector there).
 constexpr int kStatThreads = 256;
-template <typename T>
+template <typename T, int G>
 __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
   __shared__ float redf[kStatThreads / 32];
   __shared__ double redd[kStatThreads / 32];
-  const int tid = threadIdx.x;
-  for (int64_t r = blockIdx.x; r < a.T; r += gridDim.x) {
-    int64_t target;
-    if (!row_counts(a, r, target)) {
-      zero_row<T, kStatThreads>(a, r, tid);
-      continue;
-    }
-    const T* x = static_cast<const T*>(a.x) + a.in.at(r);
-    const bool ok = target >= 0 && target < a.V;
-    const float xt = ok ? to_f(x[target]) : 0.f;
-    const Span<T> sp(x, a.V);
-    float m;
-    double s;
-    thread_stats<T, kStatThreads, 4>(sp, tid, a.c, m, s);
-    block_combine<kStatThreads>(m, s, a.c, redf, redd);
+  const int tid = threadIdx.x % G;
+  const int64_t r = blockIdx.x * int64_t{kStatThreads / G} + threadIdx.x / G;
+  if (r >= a.T) return;
+  int64_t target;
+  if (!row_counts(a, r, target)) {
     if (tid == 0) {
-      const double lp = ok ? (static_cast<double>(xt) - m) * a.inv_tau - log(s) : NAN;
-      if (!ok) atomicMax(a.err, static_cast<int32_t>(kDevErrIndex));
-      a.logps[r] = static_cast<float>(lp);
-      if (a.lp64) a.lp64[r] = lp;
-      if (a.stats) a.stats[r] = make_float2(m, static_cast<float>(1.0 / s));
+      a.logps[r] = 0.f;
+      if (a.stats) a.stats[r] = make_float2(0.f, 0.f);
     }
+    return;
+  }
+  const T* x = static_cast<const T*>(a.x) + a.in.at(r);
+  const bool ok = target >= 0 && target < a.V;
+  const float xt = ok ? to_f(x[target]) : 0.f;
+  const Span<T> sp(x, a.V);
+  float m;
+  double s;
+  thread_stats<T, G, 4, true>(x, sp, tid, a.c, a.c_lo, m, s);
+  group_combine<G>(m, s, a.c, redf, redd);
+  if (tid == 0) {
+    const double lp = ok ? (static_cast<double>(xt) - m) * a.inv_tau - log(s) : NAN;
+    if (!ok) atomicMax(a.err, static_cast<int32_t>(kDevErrIndex));
+    a.logps[r] = static_cast<float>(lp);
+    if (a.lp64) a.lp64[r] = lp;
+    if (a.stats) a.stats[r] = make_float2(m, static_cast<float>(1.0 / s));
   }
 }
 
-// The teacher's entries of a row: unnormalised weights, indices (-1: no weight) and the
-// student's logits there. Returns the sum of the weights; *a_sum the row's share of
-// RowStat::a, *any false for a row without an entry, *bad whether an index is outside the
-// vocabulary.
-template <typename T, int THREADS>
-__device__ __forceinline__ double teacher_row(const RowArgs& a, int64_t r, const T* x, float m,
-                                              int tid, float* s_p, int32_t* s_id, float* s_x,
-                                              float* redf, double* redd, double* a_sum, bool* any,
-                                              bool* bad) {
-  float tm = -INFINITY;
-  bool entry = false, wrong = false;
-  for (int k = tid; k < a.K; k += THREADS) {
-    const float t = teacher_logit(a, r * a.K + k);
-    s_p[k] = t;
-    entry |= t != -INFINITY;
-    tm = fmaxf(tm, t);
+// ---- a teacher's entries of one row -----------------------------------------------
+
+// Unnormalised weights p' = exp((t - t_max) / tau), checked indices (-1: no weight) and the
+// student's logits there, of the row's K entries, by one warp. `d_sum`: sum of
+// p' ((t - t_max) - x); `p_sum`: sum of p'; `t_sum`: the same in fp32, 0 for a row without an
+// entry; `bad`: an entry with a weight has its index outside the vocabulary.
+struct TeacherSums {
+  double d_sum, p_sum;
+  float t_sum;
+  bool bad;
+  // sum of p' ((t - t_max) - (x - m)), RowStat::a
+  __device__ __forceinline__ double about(float m) const {
+    return bad ? NAN : d_sum + p_sum * static_cast<double>(m);
   }
-  tm = warp_max(tm);
-  *any = __syncthreads_or(entry);
-  if ((threadIdx.x & 31) == 0) redf[threadIdx.x >> 5] = tm;
-  __syncthreads();
-  tm = redf[0];
+};
+template <typename T>
+__device__ __forceinline__ TeacherSums teacher_weights(const RowArgs& a, int64_t r, const T* x,
+                                                       int lane, float* s_p, float* s_x,
+                                                       int32_t* s_id) {
+  constexpr int kU = 4;
+  const int64_t at = r * a.K;
+  float tm = -INFINITY;
+  for (int k0 = lane; k0 < a.K; k0 += 32 * kU) {
+    float t[kU], xv[kU];
+    int64_t id[kU];
 #pragma unroll
-  for (int w = 1; w < THREADS / 32; ++w) tm = fmaxf(tm, redf[w]);
-  double sum = 0.0, acc = 0.0;
-  for (int k = tid; k < a.K; k += THREADS) {
-    const float t = s_p[k];
-    int32_t keep = -1;
-    float p = 0.f;
-    if (*any && t != -INFINITY) {
-      const double d = static_cast<double>(t) - tm;
-      p = static_cast<float>(exp(d * a.inv_tau));
-      sum += static_cast<double>(p);
-      const int64_t id = teacher_id(a, r * a.K + k);
-      if (id < 0 || id >= a.V) {
-        wrong = true;
-      } else if (p != 0.f) {
-        const float xv = to_f(x[id]);
-        acc += static_cast<double>(p) * (d - (static_cast<double>(xv) - m));
-        keep = static_cast<int32_t>(id);
-        s_x[k] = xv;
+    for (int u = 0; u < kU; ++u) {
+      const int k = k0 + 32 * u;
+      t[u] = k < a.K ? teacher_logit(a, at + k) : -INFINITY;
+      id[u] = k < a.K ? teacher_id(a, at + k) : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const bool use = t[u] != -INFINITY && id[u] >= 0 && id[u] < a.V;
+      xv[u] = use ? to_f(x[id[u]]) : 0.f;
+      if (!use) id[u] = -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kU; ++u) {
+      const int k = k0 + 32 * u;
+      tm = fmaxf(tm, t[u]);
+      if (k < a.K) {
+        s_p[k] = t[u];
+        s_x[k] = xv[u];
+        s_id[k] = static_cast<int32_t>(id[u]);
       }
     }
-    s_id[k] = keep;
-    s_p[k] = p;
   }
-  *bad = __syncthreads_or(wrong);
-  *a_sum = block_sum_d(acc, redd);
-  return block_sum_d(sum, redd);
-}
-
-// Adds the teacher's weights to a row whose k q has been written: entries that repeat an
-// index write the same value, summed in the same order.
-template <typename T, int THREADS>
-__device__ __forceinline__ void teacher_masses(const RowArgs& a, T* dx, int tid, const float* s_p,
-                                               const int32_t* s_id, const float* s_x, float m,
-                                               float inv_s, float inv_t, float k) {
-  for (int j = tid; j < a.K; j += THREADS) {
-    const int32_t id = s_id[j];
-    if (id < 0) continue;
+  tm = warp_max(tm);
+  double sum = 0.0, d_sum = 0.0;
+  bool bad = false;
+  for (int k = lane; k < a.K; k += 32) {  // each lane reads back its own entries
+    const float t = s_p[k];
     float p = 0.f;
-    for (int i = 0; i < a.K; ++i) p += s_id[i] == id ? s_p[i] : 0.f;
-    put(dx + id, k * (ex2((s_x[j] - m) * a.c) * inv_s - p * inv_t));
+    if (t != -INFINITY) {
+      const float d = t - tm;
+      p = expf(static_cast<float>(static_cast<double>(d) * a.inv_tau));
+      sum += static_cast<double>(p);
+      bad |= p != 0.f && s_id[k] < 0;
+      if (p != 0.f)
+        d_sum += static_cast<double>(p) *
+                 (static_cast<double>(t) - static_cast<double>(tm) - static_cast<double>(s_x[k]));
+    }
+    s_p[k] = p;
+    if (p == 0.f) s_id[k] = -1;
+  }
+  bad = __any_sync(0xffffffffu, bad);
+  sum = warp_sum(sum);
+  return TeacherSums{warp_sum(d_sum), sum, static_cast<float>(sum), bad};
+}
+
+// The value of a gradient row at an entry's index: k (q - p), p the sum of the entries that hold
+// this index, in their order, so that entries which repeat it write the same value.
+__device__ __forceinline__ float teacher_value(const RowArgs& a, int32_t id, const float* s_p,
+                                               const int32_t* s_id, float q, float inv_t,
+                                               float k) {
+  float p = 0.f;
+  for (int i = 0; i < a.K; ++i) p += s_id[i] == id ? s_p[i] : 0.f;
+  return k * (q - p * inv_t);
+}
+
+// k of a distilled row: tau over the number of rows, 0 for a row without an entry.
+__device__ __forceinline__ float row_share(const RowArgs& a) {
+  return static_cast<float>(1.0 / (static_cast<double>(a.head->total) * a.inv_tau));
+}
+__device__ __forceinline__ float teacher_coef(const TeacherSums& t, float share) {
+  return t.bad ? NAN : (t.t_sum == 0.f ? 0.f : share);
+}
+
+// k of a token of the policy loss.
+__device__ __forceinline__ float policy_coef(const RowArgs& a, const Token& tk, float xt, float m,
+                                             float s, float w) {
+  const float lp = static_cast<float>((static_cast<double>(xt) - m) * a.inv_tau) - logf(s);
+  return policy_token<float, false>(a, tk, lp, nullptr, nullptr) * w;
+}
+
+__device__ __forceinline__ float grad_factor(const RowArgs& a) {
+  return a.grad_scale * (a.upstream ? *a.upstream : 1.f);
+}
+
+__device__ __forceinline__ void note_bad_index(const RowArgs& a) {
+  atomicMax(a.err, static_cast<int32_t>(kDevErrIndex));
+}
+
+// ---- rows that fit the registers of a warp or of 128 threads ------------------------
+
+// k (1[v = target] - q_v), or for distill k (q_v - p_v), and what the row leaves for
+// token_kernel. G threads hold a row, kE * NV elements each: it is read once, its exponentials
+// stay in registers and are scaled and written once. Loads of many resident groups overlap.
+constexpr int kDirectThreads = 128;
+template <typename T, int OBJ, int G, int NV>
+__global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
+  constexpr int E = Vec<T>::kE, kGroups = kDirectThreads / G;
+  __shared__ float redf[2][kDirectThreads / 32];
+  __shared__ TeacherSums s_t[kGroups];
+  extern __shared__ __align__(16) char smem[];
+  const int tid = threadIdx.x % G, group = threadIdx.x / G, warp = tid >> 5;
+  float* s_p = reinterpret_cast<float*>(smem) + group * 3 * a.K;
+  float* s_x = s_p + a.K;
+  int32_t* s_id = reinterpret_cast<int32_t*>(s_x + a.K);
+  ptx::griddep_wait();
+  const int64_t job = blockIdx.x * int64_t{kGroups} + group;
+  if (job >= a.T) return;
+  const int64_t r = a.list[job];
+  if (job >= static_cast<int64_t>(a.head->total)) {
+    zero_row<T, G>(a, r, tid);
+    return;
+  }
+  const T* x = static_cast<const T*>(a.x) + a.in.at(r);
+  const Span<T> sp(x, a.V);
+  const uint4* xv = sp.vecs(x);
+  uint4 w[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    w[i] = tid + i * G < sp.nvec ? ld16(xv + tid + i * G) : neg_inf_vec<T>();
+  const int edge = tid < kEdges ? sp.edge(tid) : -1;
+  const float xe = edge >= 0 ? to_f(x[edge]) : -INFINITY;
+  const int64_t target = OBJ == kDistill ? -1 : a.targets[r];
+  const bool ok = target >= 0 && target < a.V;
+  const float xt = ok ? to_f(x[target]) : NAN;
+  Token tk{};
+  float weight = 0.f;
+  if (OBJ == kPolicy) {
+    tk = load_token(a, r);
+    weight = static_cast<float>(token_weight(a, r) * a.inv_tau);
+  } else if (warp == 0) {
+    const TeacherSums t = teacher_weights<T>(a, r, x, tid, s_p, s_x, s_id);
+    if (tid == 0) s_t[group] = t;
+  }
+  float m = xe;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) m = fmaxf(m, Vec<T>::max(w[i]));
+  m = warp_max(m);
+  if (G > 32) {
+    if ((threadIdx.x & 31) == 0) redf[0][warp] = m;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < G / 32; ++j) m = fmaxf(m, redf[0][j]);
+  } else {
+    __syncwarp();
+  }
+  const ExpScale ks(m, a.c, a.c_lo);
+  uint64_t e[NV][E / 2];
+  uint64_t acc2 = f2_splat(0.f);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    exp_vec<T, false>(w[i], ks, e[i]);
+#pragma unroll
+    for (int j = 0; j < E / 2; ++j) acc2 = f2_add(acc2, e[i][j]);
+  }
+  float s, hi;
+  f2_unpack(acc2, s, hi);
+  const float ee = xe == -INFINITY ? 0.f : ex2((xe - m) * a.c);
+  s = warp_sum(s + hi + ee);
+  if (G > 32) {
+    if ((threadIdx.x & 31) == 0) redf[1][warp] = s;
+    __syncthreads();
+    s = 0.f;
+#pragma unroll
+    for (int j = 0; j < G / 32; ++j) s += redf[1][j];
+  } else {
+    __syncwarp();
+  }
+  if (m == -INFINITY) s = NAN;
+  const float inv_s = 1.f / s;
+  float k;
+  if (OBJ == kDistill) {
+    const TeacherSums t = s_t[group];
+    k = teacher_coef(t, row_share(a));
+    if (tid == 0) {
+      if (t.bad) note_bad_index(a);
+      a.row[r] = RowStat{m, s, t.t_sum, 0.f, t.about(m)};
+    }
+  } else {
+    k = policy_coef(a, tk, xt, m, s, weight);
+    if (tid == 0) {
+      if (!ok) note_bad_index(a);
+      a.row[r] = RowStat{m, s, xt, 0.f, 0.0};
+    }
+  }
+  if (a.dx == nullptr) return;
+  k *= grad_factor(a);
+  if (k == 0.f) {
+    zero_row<T, G>(a, r, tid);
+    return;
+  }
+  T* dx = static_cast<T*>(a.dx) + a.out.at(r);
+  const float kq = (OBJ == kDistill ? k : -k) * inv_s;
+  const uint64_t kq2 = f2_splat(kq);
+  const bool same = same_phase<T>(x, dx);
+  uint4* dv = reinterpret_cast<uint4*>(dx + sp.head);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = tid + i * G;
+#pragma unroll
+    for (int j = 0; j < E / 2; ++j) e[i][j] = f2_mul(e[i][j], kq2);
+    const uint4 o = Vec<T>::pack(e[i]);
+    if (v < sp.nvec) {
+      if (same)
+        dv[v] = o;
+      else
+        store_apart<T>(dx + sp.head + v * E, o);
+    }
+  }
+  if (edge >= 0) put(dx + edge, ee * kq);
+  if (OBJ == kPolicy) {
+    // the target's value, by the thread that has just written what the others hold there
+    if (ok && tid == sp.owner(static_cast<int>(target), G))
+      put(dx + target, k + ex2((xt - m) * a.c) * kq);
+  } else {
+    group_sync<G>();
+    const float inv_t = 1.f / s_t[group].t_sum;
+    for (int j = tid; j < a.K; j += G)
+      if (s_id[j] >= 0)
+        put(dx + s_id[j], teacher_value(a, s_id[j], s_p, s_id, ex2((s_x[j] - m) * a.c) * inv_s,
+                                        inv_t, k));
   }
 }
 
-// Gradient rows: k (1[v = target] - q_v), or for distill k (q_v - p_v). Rows are swept twice;
-// the second sweep finds them in L2.
+// ---- rows held by one CTA, or by the CTAs of a cluster ------------------------------
+
+// The same for longer rows. A persistent CTA of 512 threads holds a row, or its share of one,
+// in registers (kE * NV elements a thread); while it works, a producer warp already brings the
+// next rows into a ring of shared memory with bulk copies, so that HBM is read and written
+// without a pause, and what else the rows need: their edges, the token's numbers or the
+// teacher's entries. A cluster of cs CTAs shares rows too long for one, or few rows of any
+// length; its CTAs exchange maxima and sums through each other's shared memory.
+constexpr int kRingThreads = 512;
+constexpr int kRingWarps = kRingThreads / 32;
+constexpr int kMaxStages = 4;
+constexpr int kMaxCluster = 8;
+
+// What the producer puts down for a row, so that the consumers' registers hold the row itself.
+struct RowInfo {
+  int64_t row;        // -1: no more
+  char* dx;           // the gradient row, and where this CTA's share of its vectors goes
+  char* dv;
+  int32_t nv;         // vectors in this CTA's share
+  int32_t head, nvec; // the row's Span
+  int32_t same;       // the gradient row has the input row's phase
+  int32_t target;     // -1 outside the vocabulary
+  int32_t owner;      // the thread that holds the target, -1: another CTA's
+  float xt, w;
+  Token tk;
+  TeacherSums t;
+  float edge[kEdges];
+  int32_t edge_at[kEdges];  // -1: none (all of them in CTAs other than the first)
+};
+
+// What a CTA of a cluster knows of a row: its share's maximum and sum.
+struct __align__(8) Share {
+  float m, s;
+};
+
+// Whether element i of a row lies in the share of nv vectors from `start` on; the first CTA's
+// share has the edges.
+template <typename T>
+__device__ __forceinline__ bool in_share(int head, int nvec, int start, int nv, int rank, int i) {
+  const int v = (i - head) / Vec<T>::kE - start;
+  return i < head || i >= head + nvec * Vec<T>::kE ? rank == 0 : v >= 0 && v < nv;
+}
+// The thread that holds element i of its share.
+template <typename T>
+__device__ __forceinline__ int share_owner(const Span<T>& sp, int start, int i) {
+  if (i < sp.head || i >= sp.head + sp.nvec * Vec<T>::kE) return sp.owner(i, 1);
+  return ((i - sp.head) / Vec<T>::kE - start) % kRingThreads;
+}
+
+__device__ __forceinline__ void ring_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+__device__ __forceinline__ bool ring_all(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, 1, 512, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(ok))
+      : "memory");
+  return r != 0;
+}
+
+// Bulk copy into this CTA's shared memory (both addresses and the size multiples of 16 bytes).
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::
+          "r"(ptx::smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(ptx::smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(
+                   ptx::smem_u32(bar)),
+               "r"(bytes)
+               : "memory");
+}
+// 8 bytes into a CTA of the cluster, counted on its barrier.
+__device__ __forceinline__ void store_remote(uint32_t dst, float a, float b, uint32_t bar) {
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(
+          dst),
+      "f"(a), "f"(b), "r"(bar)
+      : "memory");
+}
+
+template <typename T, int OBJ, int NV>
+__global__ void __launch_bounds__(kRingThreads + 32, 1)
+    ring_kernel(RowArgs a, int cs, int per, int stages) {
+  constexpr int E = Vec<T>::kE;
+  extern __shared__ __align__(16) char smem[];
+  uint4* ring = reinterpret_cast<uint4*>(smem);  // [stages][per]
+  float* s_p0 = reinterpret_cast<float*>(ring + static_cast<int64_t>(stages) * per);
+  float* s_x0 = s_p0 + (stages + 1) * a.K;  // each [stages + 1][K]
+  int32_t* s_id0 = reinterpret_cast<int32_t*>(s_x0 + (stages + 1) * a.K);
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], exchanged[2];
+  // one more than the stages: a row's numbers are used until its end, its stage is free before
+  __shared__ RowInfo info[kMaxStages + 1];
+  __shared__ Share share[2][kMaxCluster];
+  __shared__ float red_m[kRingWarps], red_s[kRingWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = cs > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
+  const int64_t first = blockIdx.x / cs, step = gridDim.x / cs;
+  const int start = rank * per;  // this CTA's first vector of a row; rank 0 has the edges too
+  if (tid == 0) {
+    for (int i = 0; i < stages; ++i) {
+      ptx::mbar_init(&full[i], 1);
+      ptx::mbar_init(&empty[i], 1);
+    }
+    ptx::mbar_init(&exchanged[0], 1);
+    ptx::mbar_init(&exchanged[1], 1);
+    ptx::fence_mbar_init();
+  }
+  __syncthreads();
+  if (cs > 1) ptx::cluster_sync();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  ptx::griddep_wait();
+  const int64_t total = static_cast<int64_t>(a.head->total);
+
+  if (warp == kRingWarps) {
+    // ---- producer: 32 rows' numbers at a time, then each row's copy
+    int i = 0, st = 0, slot = 0;
+    uint32_t phase = 0;
+    bool ok = true, more = true;
+    for (int64_t base = first; more && ok; base += 32 * step) {
+      const int64_t job = base + lane * step;
+      const bool live = job < total;
+      int64_t row = -1;
+      int32_t target = -1;
+      Token tk{};
+      float xt = NAN, w = 0.f;
+      if (live) {
+        row = a.list[job];
+        if (OBJ == kPolicy) {
+          const int64_t t = a.targets[row];
+          if (t >= 0 && t < a.V) {
+            target = static_cast<int32_t>(t);
+            xt = to_f((static_cast<const T*>(a.x) + a.in.at(row))[t]);
+          }
+          tk = load_token(a, row);
+          w = static_cast<float>(token_weight(a, row) * a.inv_tau);
+        }
+      }
+      const int n = __popc(__ballot_sync(0xffffffffu, live));
+      more = n == 32;
+      for (int j = 0; j <= n && ok; ++j) {
+        if (j == n && more) break;  // the end goes behind the last row
+        if (i >= stages) ok = ptx::mbar_wait(&empty[st], phase ^ 1u);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) {
+          if (lane == 0) atomicMax(a.err, static_cast<int32_t>(kDevErrLossTimeout));
+          break;
+        }
+        const int src = j & 31;
+        const int64_t r = j < n ? __shfl_sync(0xffffffffu, row, src) : -1;
+        RowInfo* inf = &info[slot];
+        if (r >= 0) {
+          const T* x = static_cast<const T*>(a.x) + a.in.at(r);
+          T* dx = static_cast<T*>(a.dx) + a.out.at(r);
+          const Span<T> sp(x, a.V);
+          const int nv = max(0, min(per, sp.nvec - start));
+          if (lane == 0 && nv > 0) {
+            mbar_expect_tx(&full[st], nv * 16u);
+            bulk_load(ring + static_cast<int64_t>(st) * per, sp.vecs(x) + start, nv * 16u,
+                      &full[st]);
+          }
+          if (lane < kEdges) {
+            const int e = rank == 0 ? sp.edge(lane) : -1;
+            inf->edge_at[lane] = e;
+            inf->edge[lane] = e >= 0 ? to_f(x[e]) : -INFINITY;
+          }
+          if (OBJ == kDistill) {
+            const TeacherSums t = teacher_weights<T>(a, r, x, lane, s_p0 + slot * a.K,
+                                                     s_x0 + slot * a.K, s_id0 + slot * a.K);
+            if (lane == 0) inf->t = t;
+          }
+          if (lane == src) {
+            inf->dx = reinterpret_cast<char*>(dx);
+            inf->dv = reinterpret_cast<char*>(dx + sp.head + static_cast<int64_t>(start) * E);
+            inf->nv = nv;
+            inf->head = sp.head;
+            inf->nvec = sp.nvec;
+            inf->same = same_phase<T>(x, dx);
+            inf->target = target;
+            inf->owner = target >= 0 && in_share<T>(sp.head, sp.nvec, start, nv, rank, target)
+                             ? share_owner<T>(sp, start, target)
+                             : -1;
+            inf->xt = xt;
+            inf->w = w;
+            inf->tk = tk;
+          }
+        }
+        if (lane == src) inf->row = r;
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&full[st]);
+        ++i;
+        slot = slot == stages ? 0 : slot + 1;
+        if (++st == stages) {
+          st = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (!ok) {
+      // copies in flight end before this CTA does
+      for (int j = 0; j < min(i, stages); ++j) {
+        const int back = (i - 1 - j) % stages;
+        ptx::mbar_wait(&full[back], ((i - 1 - j) / stages) & 1);
+      }
+    }
+    __syncwarp();
+  } else {
+    const float factor = grad_factor(a);
+    const float each = OBJ == kDistill ? row_share(a) : 0.f;
+    bool ok = true;
+    int st = 0, slot = 0;
+    uint32_t phase = 0;
+    for (uint32_t i = 0;; ++i) {
+      ok = ptx::mbar_wait(&full[st], phase) && ok;
+      if (!ring_all(ok)) {
+        if (tid == 0) atomicMax(a.err, static_cast<int32_t>(kDevErrLossTimeout));
+        break;
+      }
+      const RowInfo* inf = &info[slot];
+      if (inf->row < 0) break;
+      const int nv = inf->nv;
+      const uint4* buf = ring + static_cast<int64_t>(st) * per;
+      // the row's share into registers, and its maximum
+      const float xe = tid < kEdges ? inf->edge[tid] : -INFINITY;
+      uint4 w[NV];
+      float m = xe;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const int v = tid + j * kRingThreads;
+        w[j] = v < nv ? buf[v] : neg_inf_vec<T>();
+        m = fmaxf(m, Vec<T>::max(w[j]));
+      }
+      m = warp_max(m);
+      if (lane == 0) red_m[warp] = m;
+      ring_sync();
+      if (tid == 0) ptx::mbar_arrive(&empty[st]);
+      m = red_m[0];
+#pragma unroll
+      for (int j = 1; j < kRingWarps; ++j) m = fmaxf(m, red_m[j]);
+      // exponentials, their sum
+      const ExpScale ks(m, a.c, a.c_lo);
+      uint64_t e[NV][E / 2];
+      uint64_t acc2 = f2_splat(0.f);
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        exp_vec<T, false>(w[j], ks, e[j]);
+#pragma unroll
+        for (int l = 0; l < E / 2; ++l) acc2 = f2_add(acc2, e[j][l]);
+      }
+      const float ee = xe == -INFINITY ? 0.f : ex2((xe - m) * a.c);
+      float s, hi;
+      f2_unpack(acc2, s, hi);
+      s = warp_sum(s + hi + ee);
+      if (lane == 0) red_s[warp] = s;
+      ring_sync();
+      s = 0.f;
+#pragma unroll
+      for (int j = 0; j < kRingWarps; ++j) s += red_s[j];
+      float scale = 1.f, m_row = m;
+      if (cs > 1) {
+        const uint32_t b = i & 1;
+        if (tid == 0) ptx::mbar_arrive_expect_tx(&exchanged[b], 8u * cs);
+        if (tid < cs)
+          store_remote(ptx::mapa_shared(ptx::smem_u32(&share[b][rank]), tid), m, s,
+                       ptx::mapa_shared(ptx::smem_u32(&exchanged[b]), tid));
+        ok = ptx::mbar_wait(&exchanged[b], (i >> 1) & 1) && ok;
+        m_row = share[b][0].m;
+        for (int j = 1; j < cs; ++j) m_row = fmaxf(m_row, share[b][j].m);
+        s = 0.f;
+        for (int j = 0; j < cs; ++j) {
+          // a share of -inf alone adds nothing
+          const Share o = share[b][j];
+          s += o.s * (o.m == -INFINITY ? 0.f : ex2((o.m - m_row) * a.c));
+        }
+        scale = m == -INFINITY ? 0.f : ex2((m - m_row) * a.c);
+      }
+      if (m_row == -INFINITY) s = NAN;
+      const float inv_s = 1.f / s;
+      float k;
+      if (OBJ == kDistill) {
+        k = teacher_coef(inf->t, each);
+        if (tid == 0 && rank == 0) {
+          if (inf->t.bad) note_bad_index(a);
+          a.row[inf->row] = RowStat{m_row, s, inf->t.t_sum, 0.f, inf->t.about(m_row)};
+        }
+      } else {
+        k = policy_coef(a, inf->tk, inf->xt, m_row, s, inf->w);
+        if (tid == 0 && rank == 0) {
+          if (inf->target < 0) note_bad_index(a);
+          a.row[inf->row] = RowStat{m_row, s, inf->xt, 0.f, 0.0};
+        }
+      }
+      k *= factor;
+      if (a.dx != nullptr) {
+        const bool zero = k == 0.f;
+        const float kq = zero ? 0.f : (OBJ == kDistill ? k : -k) * inv_s * scale;
+        const uint64_t kq2 = f2_splat(kq);
+        if (inf->same) {
+          uint4* dv = reinterpret_cast<uint4*>(inf->dv);
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            const int v = tid + j * kRingThreads;
+#pragma unroll
+            for (int l = 0; l < E / 2; ++l) e[j][l] = f2_mul(e[j][l], kq2);
+            const uint4 o = Vec<T>::pack(e[j]);
+            if (v < nv) dv[v] = o;
+          }
+        } else {
+          T* de = reinterpret_cast<T*>(inf->dv);
+#pragma unroll
+          for (int j = 0; j < NV; ++j) {
+            const int v = tid + j * kRingThreads;
+#pragma unroll
+            for (int l = 0; l < E / 2; ++l) e[j][l] = f2_mul(e[j][l], kq2);
+            if (v < nv) store_apart<T>(de + v * E, Vec<T>::pack(e[j]));
+          }
+        }
+        T* dx = reinterpret_cast<T*>(inf->dx);
+        if (tid < kEdges && inf->edge_at[tid] >= 0) put(dx + inf->edge_at[tid], ee * kq);
+        if (!zero) {
+          if (OBJ == kPolicy) {
+            // the target's value, by the thread that has just written what the others hold there
+            if (tid == inf->owner)
+              put(dx + inf->target, k - ex2((inf->xt - m_row) * a.c) * inv_s * k);
+          } else {
+            ring_sync();
+            const float* s_p = s_p0 + slot * a.K;
+            const float* s_x = s_x0 + slot * a.K;
+            const int32_t* s_id = s_id0 + slot * a.K;
+            const float inv_t = 1.f / inf->t.t_sum;
+            for (int j = tid; j < a.K; j += kRingThreads)
+              if (s_id[j] >= 0 &&
+                  in_share<T>(inf->head, inf->nvec, start, nv, rank, s_id[j]))
+                put(dx + s_id[j],
+                    teacher_value(a, s_id[j], s_p, s_id, ex2((s_x[j] - m_row) * a.c) * inv_s,
+                                  inv_t, k));
+          }
+        }
+      }
+      slot = slot == stages ? 0 : slot + 1;
+      if (++st == stages) {
+        st = 0;
+        phase ^= 1u;
+      }
+    }
+    for (int64_t job = total + blockIdx.x; job < a.T; job += gridDim.x)
+      zero_row<T, kRingThreads>(a, a.list[job], tid);
+  }
+  if (cs > 1) ptx::cluster_sync();  // no CTA leaves while another may still write to it
+}
+
+// ---- rows too long for a cluster -----------------------------------------------------
+
+// One CTA a row, swept twice; the second sweep finds it in L2.
 constexpr int kRowThreads = 512;
 template <typename T, int OBJ>
-__global__ void __launch_bounds__(kRowThreads) rows_kernel(RowArgs a) {
+__global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
+  constexpr int E = Vec<T>::kE;
+  extern __shared__ __align__(16) char smem[];
+  float* s_p = reinterpret_cast<float*>(smem);
+  float* s_x = s_p + a.K;
+  int32_t* s_id = reinterpret_cast<int32_t*>(s_x + a.K);
   __shared__ float redf[kRowThreads / 32];
   __shared__ double redd[kRowThreads / 32];
-  __shared__ float s_p[OBJ == kDistill ? kMaxTeacher : 1];
-  __shared__ int32_t s_id[OBJ == kDistill ? kMaxTeacher : 1];
-  __shared__ float s_x[OBJ == kDistill ? kMaxTeacher : 1];
+  __shared__ TeacherSums s_t;
   const int tid = threadIdx.x;
-  for (int64_t r = blockIdx.x; r < a.T; r += gridDim.x) {
-    int64_t target = -1;
-    if (!row_counts(a, r, target)) {
+  ptx::griddep_wait();
+  const int64_t total = static_cast<int64_t>(a.head->total);
+  const float factor = grad_factor(a);
+  for (int64_t job = blockIdx.x; job < a.T; job += gridDim.x) {
+    const int64_t r = a.list[job];
+    if (job >= total) {
       zero_row<T, kRowThreads>(a, r, tid);
       continue;
     }
     const T* x = static_cast<const T*>(a.x) + a.in.at(r);
     const Span<T> sp(x, a.V);
-    const bool ok = OBJ == kDistill || (target >= 0 && target < a.V);
-    const float xt = OBJ != kDistill && ok ? to_f(x[target]) : 0.f;
+    const int64_t target = OBJ == kDistill ? -1 : a.targets[r];
+    const bool ok = target >= 0 && target < a.V;
+    const float xt = ok ? to_f(x[target]) : NAN;
+    const int edge = tid < kEdges ? sp.edge(tid) : -1;
+    const float xe = edge >= 0 ? to_f(x[edge]) : 0.f;
+    if (OBJ == kDistill && tid < 32) {
+      const TeacherSums t = teacher_weights<T>(a, r, x, tid, s_p, s_x, s_id);
+      if (tid == 0) s_t = t;
+    }
     float m;
-    double s;
-    thread_stats<T, kRowThreads, 4>(sp, tid, a.c, m, s);
-    block_combine<kRowThreads>(m, s, a.c, redf, redd);
-    const float inv_s = static_cast<float>(1.0 / s);
-    float k, inv_t = 0.f;
+    double sd;
+    thread_stats<T, kRowThreads, 4, false>(x, sp, tid, a.c, a.c_lo, m, sd);
+    group_combine<kRowThreads>(m, sd, a.c, redf, redd);
+    const float s = static_cast<float>(sd), inv_s = 1.f / s;
+    float k;
     if (OBJ == kDistill) {
-      bool any, bad;
-      double acc;
-      const double tsum = teacher_row<T, kRowThreads>(a, r, x, m, tid, s_p, s_id, s_x, redf, redd,
-                                                      &acc, &any, &bad);
-      inv_t = static_cast<float>(1.0 / tsum);
-      const float w = any ? static_cast<float>(token_weight(a, r) / a.inv_tau) : 0.f;
-      k = bad ? NAN : w;
+      k = teacher_coef(s_t, row_share(a));
       if (tid == 0) {
-        if (bad) atomicMax(a.err, static_cast<int32_t>(kDevErrIndex));
-        if (a.coef) a.coef[r] = k;
-        a.row[r] = RowStat{m, static_cast<float>(s), any ? static_cast<float>(tsum) : 0.f, 0.f,
-                           bad ? NAN : acc};
+        if (s_t.bad) note_bad_index(a);
+        a.row[r] = RowStat{m, s, s_t.t_sum, 0.f, s_t.about(m)};
       }
     } else {
-      const float lp = ok ? static_cast<float>((static_cast<double>(xt) - m) * a.inv_tau) -
-                                logf(static_cast<float>(s))
-                          : NAN;
-      k = policy_token<float, false>(a, r, lp, nullptr, nullptr) *
-          static_cast<float>(token_weight(a, r) * a.inv_tau);
+      k = policy_coef(a, load_token(a, r), xt, m, s,
+                      static_cast<float>(token_weight(a, r) * a.inv_tau));
       if (tid == 0) {
-        if (!ok) atomicMax(a.err, static_cast<int32_t>(kDevErrIndex));
-        a.row[r] = RowStat{m, static_cast<float>(s), ok ? xt : NAN, 0.f, 0.0};
+        if (!ok) note_bad_index(a);
+        a.row[r] = RowStat{m, s, xt, 0.f, 0.0};
       }
     }
-    if (tid == 0 && a.stats) a.stats[r] = make_float2(m, inv_s);
-    if (a.dx == nullptr) continue;
-    k *= a.grad_scale;
-    T* dx = static_cast<T*>(a.dx) + a.out.at(r);
-    const bool same = same_phase<T>(x, dx);
-    if (k == 0.f) {
-      const Span<T> so(dx, a.V);
-      for (int v = tid; v < so.nvec; v += kRowThreads)
-        store_vec<T>(dx, so, v, make_uint4(0u, 0u, 0u, 0u), true);
-      __syncthreads();
-      continue;
-    }
-    const uint64_t neg_m2 = f2_splat(-m), c2 = f2_splat(a.c);
-    const uint64_t kq2 = f2_splat(OBJ == kDistill ? k * inv_s : -k * inv_s);
-    const int at = OBJ == kDistill ? -1 : static_cast<int>(target) + sp.lead;
-    for (int v = tid; v < sp.nvec; v += kRowThreads) {
-      const uint4 w = ld16(sp.v0 + v);
-      uint64_t e[Vec<T>::kE / 2];
-      exp_vec<T>(w, neg_m2, c2, e);
+    k *= factor;
+    if (a.dx != nullptr && k == 0.f) {
+      zero_row<T, kRowThreads>(a, r, tid);
+    } else if (a.dx != nullptr) {
+      T* dx = static_cast<T*>(a.dx) + a.out.at(r);
+      const bool same = same_phase<T>(x, dx);
+      const ExpScale ks(m, a.c, a.c_lo);
+      const float kq = (OBJ == kDistill ? k : -k) * inv_s;
+      const uint64_t kq2 = f2_splat(kq);
+      const uint4* xv = sp.vecs(x);
+      uint4* dv = reinterpret_cast<uint4*>(dx + sp.head);
+      for (int v = tid; v < sp.nvec; v += kRowThreads) {
+        uint64_t e[E / 2];
+        exp_vec<T, false>(ld16(xv + v), ks, e);
 #pragma unroll
-      for (int i = 0; i < Vec<T>::kE / 2; ++i) e[i] = f2_mul(e[i], kq2);
-      if (OBJ != kDistill && at / Vec<T>::kE == v) add_mass<T>(e, at - v * Vec<T>::kE, k);
-      store_vec<T>(dx, sp, v, Vec<T>::pack(e), same);
+        for (int i = 0; i < E / 2; ++i) e[i] = f2_mul(e[i], kq2);
+        if (same)
+          dv[v] = Vec<T>::pack(e);
+        else
+          store_apart<T>(dx + sp.head + static_cast<int64_t>(v) * E, Vec<T>::pack(e));
+      }
+      if (edge >= 0) put(dx + edge, ex2((xe - m) * a.c) * kq);
+      if (OBJ == kPolicy) {
+        if (ok && tid == sp.owner(static_cast<int>(target), kRowThreads))
+          put(dx + target, k + ex2((xt - m) * a.c) * kq);
+      } else {
+        __syncthreads();
+        const float inv_t = 1.f / s_t.t_sum;
+        for (int j = tid; j < a.K; j += kRowThreads)
+          if (s_id[j] >= 0)
+            put(dx + s_id[j], teacher_value(a, s_id[j], s_p, s_id,
+                                            ex2((s_x[j] - m) * a.c) * inv_s, inv_t, k));
+      }
     }
     __syncthreads();
-    if (OBJ == kDistill) {
-      teacher_masses<T, kRowThreads>(a, dx, tid, s_p, s_id, s_x, m, inv_s, inv_t, k);
-      __syncthreads();
-    }
   }
 }
 
@@ -617,6 +1251,7 @@ template <int OBJ>
 __global__ void __launch_bounds__(kTokenThreads) token_kernel(RowArgs a) {
   __shared__ double red[kTokenThreads / 32];
   __shared__ bool s_last;
+  ptx::griddep_wait();
   const int64_t r = blockIdx.x * static_cast<int64_t>(kTokenThreads) + threadIdx.x;
   double loss = 0.0, kl = 0.0;
   int64_t target;
@@ -632,11 +1267,16 @@ __global__ void __launch_bounds__(kTokenThreads) token_kernel(RowArgs a) {
     } else {
       const double lp = (static_cast<double>(st.x) - st.m) * a.inv_tau - log_s;
       a.logps[r] = static_cast<float>(lp);
-      const double coef = policy_token<double, true>(a, r, lp, &loss, &kl);
+      const double coef = policy_token<double, true>(a, load_token(a, r), lp, &loss, &kl);
       if (a.coef) a.coef[r] = static_cast<float>(w * coef);
+      if (a.stats) a.stats[r] = make_float2(st.m, 1.f / st.s);
       loss *= w;
       kl *= w;
     }
+  } else if (OBJ == kPolicy && r < a.T) {
+    a.logps[r] = 0.f;
+    if (a.coef) a.coef[r] = 0.f;
+    if (a.stats) a.stats[r] = make_float2(0.f, 0.f);
   }
   loss = block_sum_d(loss, red);
   kl = block_sum_d(kl, red);
@@ -706,99 +1346,67 @@ __global__ void __launch_bounds__(256) pair_sum_kernel(const double2* part, int6
   if (threadIdx.x == 0) *loss = static_cast<float>(l);
 }
 
-// Gradient rows from saved statistics: k (1[v = target] - q_v). A CTA takes kBwdVecs vectors
-// of one row; nothing is reduced, so rows of any length keep every SM busy.
+// Gradient rows from saved statistics: k (1[v = target] - q_v). A group of G threads takes
+// G * kBwdU vectors of one row; nothing is reduced, so rows of any length keep every SM busy.
 constexpr int kBwdThreads = 256;
 constexpr int kBwdU = 4;
-constexpr int kBwdVecs = kBwdThreads * kBwdU;
-template <typename T>
+template <typename T, int G>
 __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, int chunks) {
-  const int tid = threadIdx.x;
-  const int64_t units = a.T * chunks;
-  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
-    const int64_t r = unit / chunks;
-    const int v0 = static_cast<int>(unit - r * chunks) * kBwdVecs;
-    const T* x = static_cast<const T*>(a.x) + a.in.at(r);
-    T* dx = static_cast<T*>(a.dx) + a.out.at(r);
-    const Span<T> sp(x, a.V);
-    const int64_t target = a.targets[r];
-    const float k = target == a.ignore
-                        ? 0.f
-                        : a.g[r] * a.grad_scale * (a.upstream ? *a.upstream : 1.f) *
-                              static_cast<float>(a.inv_tau);
-    const bool same = same_phase<T>(x, dx);
-    if (k == 0.f) {
-      // zeros need no input: whole vectors of the output's own phase
-      const Span<T> so(dx, a.V);
+  constexpr int E = Vec<T>::kE;
+  const int tid = threadIdx.x % G;
+  const int64_t unit = blockIdx.x * int64_t{kBwdThreads / G} + threadIdx.x / G;
+  const int64_t r = unit / chunks;
+  if (r >= a.T) return;
+  const int chunk = static_cast<int>(unit - r * chunks);
+  const int v0 = chunk * (G * kBwdU) + tid;
+  const T* x = static_cast<const T*>(a.x) + a.in.at(r);
+  T* dx = static_cast<T*>(a.dx) + a.out.at(r);
+  const int64_t target = a.targets[r];
+  const float k =
+      target == a.ignore ? 0.f : a.g[r] * grad_factor(a) * static_cast<float>(a.inv_tau);
+  if (k == 0.f) {
+    // zeros need no input: whole vectors of the output's own phase
+    const Span<T> so(dx, a.V);
+    uint4* dv = reinterpret_cast<uint4*>(dx + so.head);
 #pragma unroll
-      for (int u = 0; u < kBwdU; ++u) {
-        const int v = v0 + tid + u * kBwdThreads;
-        if (v < so.nvec) store_vec<T>(dx, so, v, make_uint4(0u, 0u, 0u, 0u), true);
-      }
-      continue;
-    }
-    uint4 w[kBwdU];
-#pragma unroll
-    for (int u = 0; u < kBwdU; ++u) {
-      const int v = v0 + tid + u * kBwdThreads;
-      if (v < sp.nvec) w[u] = ld16(sp.v0 + v);
-    }
-    const float2 st = a.stats[r];
-    const uint64_t neg_m2 = f2_splat(-st.x), c2 = f2_splat(a.c), kq2 = f2_splat(-k * st.y);
-    const int64_t at = target + sp.lead;
-#pragma unroll
-    for (int u = 0; u < kBwdU; ++u) {
-      const int v = v0 + tid + u * kBwdThreads;
-      if (v >= sp.nvec) continue;
-      uint64_t e[Vec<T>::kE / 2];
-      exp_vec<T>(w[u], neg_m2, c2, e);
-#pragma unroll
-      for (int i = 0; i < Vec<T>::kE / 2; ++i) e[i] = f2_mul(e[i], kq2);
-      if (at / Vec<T>::kE == v) add_mass<T>(e, static_cast<int>(at - v * Vec<T>::kE), k);
-      store_vec<T>(dx, sp, v, Vec<T>::pack(e), same);
-    }
+    for (int u = 0; u < kBwdU; ++u)
+      if (v0 + u * G < so.nvec) dv[v0 + u * G] = make_uint4(0u, 0u, 0u, 0u);
+    if (chunk == 0 && tid < kEdges && so.edge(tid) >= 0) put(dx + so.edge(tid), 0.f);
+    return;
   }
-}
-
-// distill's gradient rows from saved statistics.
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(RowArgs a) {
-  __shared__ float redf[kRowThreads / 32];
-  __shared__ double redd[kRowThreads / 32];
-  __shared__ float s_p[kMaxTeacher];
-  __shared__ int32_t s_id[kMaxTeacher];
-  __shared__ float s_x[kMaxTeacher];
-  const int tid = threadIdx.x;
-  const float up = a.upstream ? *a.upstream : 1.f;
-  for (int64_t r = blockIdx.x; r < a.T; r += gridDim.x) {
-    int64_t target;
-    const float k = row_counts(a, r, target) ? a.g[r] * up : 0.f;
-    if (k == 0.f) {
-      zero_row<T, kRowThreads>(a, r, tid);
-      continue;
-    }
-    const T* x = static_cast<const T*>(a.x) + a.in.at(r);
-    T* dx = static_cast<T*>(a.dx) + a.out.at(r);
-    const Span<T> sp(x, a.V);
-    const bool same = same_phase<T>(x, dx);
-    const float2 st = a.stats[r];
-    bool any, bad;
-    double acc;
-    const double tsum = teacher_row<T, kRowThreads>(a, r, x, st.x, tid, s_p, s_id, s_x, redf, redd,
-                                                    &acc, &any, &bad);
-    const uint64_t neg_m2 = f2_splat(-st.x), c2 = f2_splat(a.c), kq2 = f2_splat(k * st.y);
-    for (int v = tid; v < sp.nvec; v += kRowThreads) {
-      const uint4 w = ld16(sp.v0 + v);
-      uint64_t e[Vec<T>::kE / 2];
-      exp_vec<T>(w, neg_m2, c2, e);
+  const Span<T> sp(x, a.V);
+  const uint4* xv = sp.vecs(x);
+  uint4 w[kBwdU];
 #pragma unroll
-      for (int i = 0; i < Vec<T>::kE / 2; ++i) e[i] = f2_mul(e[i], kq2);
-      store_vec<T>(dx, sp, v, Vec<T>::pack(e), same);
-    }
-    __syncthreads();
-    teacher_masses<T, kRowThreads>(a, dx, tid, s_p, s_id, s_x, st.x, st.y,
-                                   static_cast<float>(1.0 / tsum), k);
-    __syncthreads();
+  for (int u = 0; u < kBwdU; ++u)
+    if (v0 + u * G < sp.nvec) w[u] = ld16(xv + v0 + u * G);
+  const float2 st = a.stats[r];
+  const ExpScale ks(st.x, a.c, a.c_lo);
+  const float kq = -k * st.y;
+  const uint64_t kq2 = f2_splat(kq);
+  const bool same = same_phase<T>(x, dx);
+  uint4* dv = reinterpret_cast<uint4*>(dx + sp.head);
+  // the target's value, by the thread that has just written what the others hold there
+  const bool ok = target >= 0 && target < a.V;
+  const int tv = ok ? static_cast<int>(target) - sp.head : -1;  // its place behind the head
+  const float xt = ok ? to_f(x[target]) : 0.f;
+#pragma unroll
+  for (int u = 0; u < kBwdU; ++u) {
+    const int v = v0 + u * G;
+    if (v >= sp.nvec) continue;
+    uint64_t e[E / 2];
+    exp_vec<T, false>(w[u], ks, e);
+#pragma unroll
+    for (int i = 0; i < E / 2; ++i) e[i] = f2_mul(e[i], kq2);
+    if (same)
+      dv[v] = Vec<T>::pack(e);
+    else
+      store_apart<T>(dx + sp.head + static_cast<int64_t>(v) * E, Vec<T>::pack(e));
+    if (tv >= 0 && tv / E == v) put(dx + target, k + ex2((xt - st.x) * a.c) * kq);
+  }
+  if (chunk == 0 && tid < kEdges && sp.edge(tid) >= 0) {
+    const int i = sp.edge(tid);
+    put(dx + i, ex2((to_f(x[i]) - st.x) * a.c) * kq + (i == target ? k : 0.f));
   }
 }
 
@@ -830,7 +1438,9 @@ int make_rows(RowArgs& a, const void* x, int64_t n0, int64_t n1, int64_t ld0, in
   a.T = n0 * n1;
   a.V = static_cast<int32_t>(V);
   a.inv_tau = 1.0 / temperature;
-  a.c = static_cast<float>(1.4426950408889634 / temperature);
+  const double c = 1.4426950408889634 / temperature;
+  a.c = static_cast<float>(c);
+  a.c_lo = static_cast<float>(c - static_cast<double>(a.c));
   a.grad_scale = 1.f;
   return LEMA_OK;
 }
@@ -857,7 +1467,7 @@ int64_t token_ctas(int64_t T) { return (T + kTokenThreads - 1) / kTokenThreads; 
 int64_t parts(int64_t n0, int64_t T) { return std::max(token_ctas(T), n0) + 1; }
 
 int64_t ws_bytes_for(int64_t n0, int64_t T) {
-  return kWsHead + round256(n0 * 4) + round256(parts(n0, T) * 16) +
+  return kWsHead + round256(n0 * 4) + round256(T * 4) + round256(parts(n0, T) * 16) +
          T * static_cast<int64_t>(sizeof(RowStat));
 }
 
@@ -870,6 +1480,8 @@ int set_ws(RowArgs& a, void* ws, int64_t ws_bytes) {
   p += kWsHead;
   a.seq_count = reinterpret_cast<int32_t*>(p);
   p += round256(a.n0 * 4);
+  a.list = reinterpret_cast<int32_t*>(p);
+  p += round256(a.T * 4);
   a.part = reinterpret_cast<double2*>(p);
   p += round256(parts(a.n0, a.T) * 16);
   a.row = reinterpret_cast<RowStat*>(p);
@@ -877,49 +1489,191 @@ int set_ws(RowArgs& a, void* ws, int64_t ws_bytes) {
   return LEMA_OK;
 }
 
-unsigned rows_grid(const RowArgs& a) {
-  return static_cast<unsigned>(std::min<int64_t>(a.T, 1 << 20));
+// Whole vectors that a row holds, at most.
+int max_vecs(const RowArgs& a, int x_f32) { return a.V / (x_f32 ? 4 : 8); }
+
+// A launch that may begin while the kernel before it on the stream still runs (every kernel
+// launched so waits for that one before it touches what it wrote), in clusters of cs CTAs.
+template <typename... P, typename... A>
+int launch_after(void (*kern)(P...), int64_t grid, int threads, int smem, int cs, cudaStream_t s,
+                 A... args) {
+  if (grid > INT32_MAX) return set_error(LEMA_ERR_UNSUPPORTED, "too many rows");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cs);
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cs > 1 ? 2 : 1;
+  LEMA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+  return LEMA_OK;
+}
+
+// A warp a row while four vectors a lane hold it.
+bool warp_rows(int nvec) { return nvec <= 128; }
+
+template <typename T>
+int launch_logprobs_t(const RowArgs& a, int nvec, cudaStream_t s) {
+  if (warp_rows(nvec)) {
+    const int64_t per = kStatThreads / 32;
+    logprobs_kernel<T, 32><<<static_cast<unsigned>((a.T + per - 1) / per), kStatThreads, 0, s>>>(a);
+  } else {
+    logprobs_kernel<T, kStatThreads><<<static_cast<unsigned>(a.T), kStatThreads, 0, s>>>(a);
+  }
+  LEMA_CUDA_TRY(cudaGetLastError());
+  return LEMA_OK;
 }
 
 int launch_logprobs(const RowArgs& a, int x_f32, cudaStream_t s) {
-  if (x_f32)
-    logprobs_kernel<float><<<rows_grid(a), kStatThreads, 0, s>>>(a);
+  const int nvec = max_vecs(a, x_f32);
+  return x_f32 ? launch_logprobs_t<float>(a, nvec, s)
+               : launch_logprobs_t<__nv_bfloat16>(a, nvec, s);
+}
+
+template <typename T>
+int launch_logprobs_bwd_t(const RowArgs& a, int nvec, cudaStream_t s) {
+  const int g = warp_rows(nvec) ? 32 : kBwdThreads;
+  const int chunks = std::max(1, (nvec + g * kBwdU - 1) / (g * kBwdU));
+  const int64_t per = kBwdThreads / g, grid = (a.T * chunks + per - 1) / per;
+  if (grid > INT32_MAX) return set_error(LEMA_ERR_UNSUPPORTED, "too many rows");
+  if (g == 32)
+    logprobs_bwd_kernel<T, 32><<<static_cast<unsigned>(grid), kBwdThreads, 0, s>>>(a, chunks);
   else
-    logprobs_kernel<__nv_bfloat16><<<rows_grid(a), kStatThreads, 0, s>>>(a);
+    logprobs_bwd_kernel<T, kBwdThreads>
+        <<<static_cast<unsigned>(grid), kBwdThreads, 0, s>>>(a, chunks);
   LEMA_CUDA_TRY(cudaGetLastError());
   return LEMA_OK;
 }
 
 int launch_logprobs_bwd(const RowArgs& a, int x_f32, cudaStream_t s) {
-  const int e = x_f32 ? 4 : 8;
-  // a misaligned row spans up to one vector more
-  const int chunks = static_cast<int>(((a.V + e - 1) / e + 1 + kBwdVecs - 1) / kBwdVecs);
-  const int64_t grid = std::min<int64_t>(a.T * chunks, INT32_MAX);
-  if (x_f32)
-    logprobs_bwd_kernel<float><<<static_cast<unsigned>(grid), kBwdThreads, 0, s>>>(a, chunks);
-  else
-    logprobs_bwd_kernel<__nv_bfloat16><<<static_cast<unsigned>(grid), kBwdThreads, 0, s>>>(a,
-                                                                                        chunks);
-  LEMA_CUDA_TRY(cudaGetLastError());
+  const int nvec = max_vecs(a, x_f32);
+  return x_f32 ? launch_logprobs_bwd_t<float>(a, nvec, s)
+               : launch_logprobs_bwd_t<__nv_bfloat16>(a, nvec, s);
+}
+
+constexpr int kRingSmem = 216 * 1024;
+
+template <typename Kern>
+int allow_smem(Kern kern, int bytes, std::atomic<uint64_t>& done) {
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64) return set_error(LEMA_ERR_CUDA, "bad device");
+  if (!(done.load() >> dev & 1)) {
+    LEMA_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done |= uint64_t{1} << dev;
+  }
   return LEMA_OK;
 }
 
-// Counts, the rows' statistics and gradients, the tokens' terms.
+// Clusters of cs CTAs that are resident at once.
+template <typename Kern>
+int resident_clusters(Kern kern, int cs, int smem, int* out) {
+  static std::atomic<int> cache[64][4];  // by device and log2(cs); 1 CTA an SM either way
+  const int dev = current_device(), slot = cs == 2 ? 1 : (cs == 4 ? 2 : 3);
+  int n = cache[dev][slot].load();
+  if (n == 0) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(cs));
+    cfg.blockDim = dim3(kRingThreads + 32);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(cs);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    LEMA_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+    if (n < 1) return set_error(LEMA_ERR_CUDA, "no cluster fits this device");
+    cache[dev][slot].store(n);
+  }
+  *out = n;
+  return LEMA_OK;
+}
+
+template <typename T, int OBJ, int NV>
+int launch_ring(const RowArgs& a, int cs, int per, cudaStream_t s) {
+  const int stage = per * 16;
+  int stages = 0, smem = 0;
+  for (int n = kMaxStages; n >= 1 && stages == 0; --n) {
+    smem = n * stage + (n + 1) * a.K * 12;
+    if (smem <= kRingSmem) stages = n;
+  }
+  auto kern = ring_kernel<T, OBJ, NV>;
+  static std::atomic<uint64_t> done{0};
+  int rc = allow_smem(kern, kRingSmem, done);
+  if (rc) return rc;
+  int clusters = device_sm_count();
+  if (cs > 1 && (rc = resident_clusters(kern, cs, smem, &clusters))) return rc;
+  const int64_t n = std::min<int64_t>(a.T, clusters);
+  return launch_after(kern, n * cs, kRingThreads + 32, smem, cs, s, a, cs, per, stages);
+}
+
+template <typename T, int OBJ, int G, int NV>
+int launch_direct(const RowArgs& a, int64_t grid, int smem, cudaStream_t s) {
+  auto kern = direct_kernel<T, OBJ, G, NV>;
+  static std::atomic<uint64_t> done{0};
+  if (OBJ == kDistill) {  // four warps with 1024 entries each take more than the default 48 KB
+    const int rc = allow_smem(kern, kDirectThreads / G * kMaxTeacher * 12, done);
+    if (rc) return rc;
+  }
+  return launch_after(kern, grid, kDirectThreads, smem, 1, s, a);
+}
+
+// How a row is held, by the vectors it spans. kNv vectors are the 64 elements that a thread
+// keeps as fp32.
+template <typename T, int OBJ>
+int launch_rows(const RowArgs& a, int nvec, cudaStream_t s) {
+  constexpr int kNv = 64 / Vec<T>::kE;
+  const int teacher = a.K * 12;
+  if (nvec <= 128 * kNv) {
+    const bool warps = nvec <= 32 * kNv;
+    const int64_t per = warps ? kDirectThreads / 32 : 1, grid = (a.T + per - 1) / per;
+    const int smem = static_cast<int>(per) * teacher;
+    if (nvec <= 8 * kNv) return launch_direct<T, OBJ, 32, kNv / 4>(a, grid, smem, s);
+    if (nvec <= 16 * kNv) return launch_direct<T, OBJ, 32, kNv / 2>(a, grid, smem, s);
+    if (warps) return launch_direct<T, OBJ, 32, kNv>(a, grid, smem, s);
+    if (nvec <= 64 * kNv) return launch_direct<T, OBJ, 128, kNv / 2>(a, grid, smem, s);
+    return launch_direct<T, OBJ, 128, kNv>(a, grid, smem, s);
+  }
+  int cs = 1;
+  while (cs < kMaxCluster && nvec > cs * kRingThreads * kNv) cs *= 2;
+  if (nvec > cs * kRingThreads * kNv)
+    return launch_after(stream_kernel<T, OBJ>, std::min<int64_t>(a.T, 2 * device_sm_count()),
+                        kRowThreads, teacher, 1, s, a);
+  // few rows: spread each while SMs would be idle and every thread still has a vector
+  while (cs < kMaxCluster && a.T * cs * 2 <= device_sm_count() &&
+         nvec >= cs * 2 * kRingThreads)
+    cs *= 2;
+  const int share = (nvec + cs - 1) / cs;
+  if (share <= kRingThreads * kNv / 4) return launch_ring<T, OBJ, kNv / 4>(a, cs, share, s);
+  if (share <= kRingThreads * kNv / 2) return launch_ring<T, OBJ, kNv / 2>(a, cs, share, s);
+  return launch_ring<T, OBJ, kNv>(a, cs, share, s);
+}
+
+// The list of rows, their statistics and gradients, the tokens' terms.
 template <int OBJ>
 int launch_loss(const RowArgs& a, int x_f32, cudaStream_t s) {
-  count_kernel<<<1, 1024, 0, s>>>(a);
+  // one CTA lists 8192 rows in about the time that clearing the counters first would take
+  int64_t ctas = 1;
+  if (a.T > kCountBlock) {
+    ctas = std::min<int64_t>((a.T + kCountBlock - 1) / kCountBlock, device_sm_count());
+    LEMA_CUDA_TRY(cudaMemsetAsync(a.head, 0, kWsHead + (a.per_sequence ? a.n0 * 4 : 0), s));
+  }
+  count_kernel<<<static_cast<unsigned>(ctas), kCountThreads, 0, s>>>(a);
   LEMA_CUDA_TRY(cudaGetLastError());
   if (a.T > 0) {
-    if (x_f32)
-      rows_kernel<float, OBJ><<<rows_grid(a), kRowThreads, 0, s>>>(a);
-    else
-      rows_kernel<__nv_bfloat16, OBJ><<<rows_grid(a), kRowThreads, 0, s>>>(a);
-    LEMA_CUDA_TRY(cudaGetLastError());
+    const int nvec = max_vecs(a, x_f32);
+    const int rc = x_f32 ? launch_rows<float, OBJ>(a, nvec, s)
+                         : launch_rows<__nv_bfloat16, OBJ>(a, nvec, s);
+    if (rc) return rc;
   }
-  token_kernel<OBJ><<<static_cast<unsigned>(std::max<int64_t>(1, token_ctas(a.T))), kTokenThreads,
-                      0, s>>>(a);
-  LEMA_CUDA_TRY(cudaGetLastError());
-  return LEMA_OK;
+  return launch_after(token_kernel<OBJ>, std::max<int64_t>(1, token_ctas(a.T)), kTokenThreads, 0,
+                      1, s, a);
 }
 
 // Statistics are read and written as pairs.
@@ -1060,69 +1814,31 @@ extern "C" int lema_policy_loss(const void* x, int32_t x_f32, int64_t n0, int64_
   return launch_loss<kPolicy>(a, x_f32, static_cast<cudaStream_t>(stream));
 }
 
-namespace lema {
-namespace {
-int set_teacher(RowArgs& a, const void* ids, int32_t ids_i32, const void* logits, int32_t tl_f32,
-                int64_t K, const uint8_t* mask) {
-  if (K < 1 || K > kMaxTeacher)
-    return set_error(LEMA_ERR_UNSUPPORTED, "between 1 and 1024 teacher entries a row");
-  if (a.T > 0 && (!ids || !logits)) return bad("null teacher indices or logits");
-  a.teacher_ids = ids;
-  a.ids_i32 = ids_i32;
-  a.teacher_logits = logits;
-  a.tl_f32 = tl_f32;
-  a.K = static_cast<int32_t>(K);
-  a.mask = mask;
-  return LEMA_OK;
-}
-}  // namespace
-}  // namespace lema
-
 extern "C" int lema_distill_loss(const void* x, int32_t x_f32, int64_t n0, int64_t n1,
                                  int64_t ld0, int64_t ld1, int64_t V, const void* teacher_ids,
                                  int32_t ids_i32, const void* teacher_logits, int32_t tl_f32,
                                  int64_t K, const uint8_t* mask, double temperature,
-                                 double grad_scale, void* ws, int64_t ws_bytes, float* stats,
-                                 float* coef, float* loss, void* dx, int64_t ldd0, int64_t ldd1,
-                                 void* stream) {
+                                 double grad_scale, const float* upstream, void* ws,
+                                 int64_t ws_bytes, float* loss, void* dx, int64_t ldd0,
+                                 int64_t ldd1, void* stream) {
   clear_error();
   RowArgs a;
   int rc = make_rows(a, x, n0, n1, ld0, ld1, V, temperature);
   if (rc) return rc;
   if (!loss) return bad("null loss");
-  if ((rc = set_teacher(a, teacher_ids, ids_i32, teacher_logits, tl_f32, K, mask)) ||
-      (rc = set_ws(a, ws, ws_bytes)) || (rc = set_out(a, dx, ldd0, ldd1)) || (rc = need_err(a)))
+  if (K < 1 || K > kMaxTeacher)
+    return set_error(LEMA_ERR_UNSUPPORTED, "between 1 and 1024 teacher entries a row");
+  if (a.T > 0 && (!teacher_ids || !teacher_logits)) return bad("null teacher indices or logits");
+  if ((rc = set_ws(a, ws, ws_bytes)) || (rc = set_out(a, dx, ldd0, ldd1)) || (rc = need_err(a)))
     return rc;
-  if ((rc = set_stats(a, stats))) return rc;
-  a.coef = coef;
+  a.teacher_ids = teacher_ids;
+  a.ids_i32 = ids_i32;
+  a.teacher_logits = teacher_logits;
+  a.tl_f32 = tl_f32;
+  a.K = static_cast<int32_t>(K);
+  a.mask = mask;
   a.grad_scale = static_cast<float>(grad_scale);
+  a.upstream = upstream;
   a.loss = loss;
   return launch_loss<kDistill>(a, x_f32, static_cast<cudaStream_t>(stream));
-}
-
-extern "C" int lema_distill_loss_bwd(const void* x, int32_t x_f32, int64_t n0, int64_t n1,
-                                     int64_t ld0, int64_t ld1, int64_t V,
-                                     const void* teacher_ids, int32_t ids_i32,
-                                     const void* teacher_logits, int32_t tl_f32, int64_t K,
-                                     const uint8_t* mask, double temperature, const float* stats,
-                                     const float* coef, const float* upstream, void* dx,
-                                     int64_t ldd0, int64_t ldd1, void* stream) {
-  clear_error();
-  RowArgs a;
-  int rc = make_rows(a, x, n0, n1, ld0, ld1, V, temperature);
-  if (rc) return rc;
-  if ((rc = set_teacher(a, teacher_ids, ids_i32, teacher_logits, tl_f32, K, mask))) return rc;
-  if (a.T == 0) return LEMA_OK;
-  if (!stats || !coef || !dx) return bad("null pointer");
-  if ((rc = set_out(a, dx, ldd0, ldd1))) return rc;
-  if ((rc = set_stats(a, stats))) return rc;
-  a.g = coef;
-  a.upstream = upstream;
-  auto s = static_cast<cudaStream_t>(stream);
-  if (x_f32)
-    distill_bwd_kernel<float><<<rows_grid(a), kRowThreads, 0, s>>>(a);
-  else
-    distill_bwd_kernel<__nv_bfloat16><<<rows_grid(a), kRowThreads, 0, s>>>(a);
-  LEMA_CUDA_TRY(cudaGetLastError());
-  return LEMA_OK;
 }

@@ -1179,45 +1179,36 @@ def _teacher(x: _Logits, ids: torch.Tensor, logits: torch.Tensor, mask):
     return ids.contiguous(), logits.contiguous(), mask
 
 
-def _distill(logits, teacher_ids, teacher_logits, mask, temperature, grad_scale, out, want_dx,
-             want_saved):
+def _distill(logits, ids, tl, mask, temperature, grad_scale, upstream, out, want_dx):
+    """One call on checked teacher tensors: (loss, dlogits or None)."""
     x = _Logits(logits)
-    ids, tl, mask = _teacher(x, teacher_ids, teacher_logits, mask)
     ws, n = x.workspace()
-    T = x.n0 * x.n1
-    # the loss, then the statistics (pairs: 8-byte aligned) and the coefficients
-    f = torch.empty(2 + (3 * T if want_saved else 0), dtype=torch.float32, device=x.dev)
-    stats, coef = (f[2:2 + 2 * T], f[2 + 2 * T:]) if want_saved else (None, None)
+    loss = torch.empty((), dtype=torch.float32, device=x.dev)
     dx = view = None
     if want_dx:
         dx, view = x.grad_out(logits, out)
     x.call("lema_distill_loss", ids.data_ptr(), int(ids.dtype == torch.int32), tl.data_ptr(),
            int(tl.dtype == torch.float32), ids.shape[-1], _ptr(mask), float(temperature),
-           float(grad_scale), ws.data_ptr(), n, _ptr(stats), _ptr(coef), f.data_ptr(), _ptr(view),
+           float(grad_scale), _ptr(upstream), ws.data_ptr(), n, loss.data_ptr(), _ptr(view),
            view.stride(0) if want_dx else 0, view.stride(1) if want_dx else 0)
-    return ids, tl, mask, f[0], stats, coef, dx
+    return loss, dx
 
 
 class _DistillFn(torch.autograd.Function):
+    """The backward runs the fused pass: rows are held on chip while their statistics are
+    taken, so it moves no more bytes than one from saved statistics."""
+
     @staticmethod
-    def forward(ctx, logits, teacher_ids, teacher_logits, mask, temperature):
-        ids, tl, mask, loss, stats, coef, _ = _distill(logits, teacher_ids, teacher_logits, mask,
-                                                       temperature, 1.0, None, False, True)
-        ctx.save_for_backward(logits, ids, tl, mask, stats, coef)
-        ctx.temperature = float(temperature)
-        return loss
+    def forward(ctx, logits, ids, tl, mask, temperature):
+        ctx.save_for_backward(logits, ids, tl, mask)
+        ctx.temperature = temperature
+        return _distill(logits, ids, tl, mask, temperature, 1.0, None, None, False)[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        logits, ids, tl, mask, stats, coef = ctx.saved_tensors
-        x = _Logits(logits)
-        dx, view = x.grad_out(logits, None)
-        up = dloss.float()
-        x.call("lema_distill_loss_bwd", ids.data_ptr(), int(ids.dtype == torch.int32),
-               tl.data_ptr(), int(tl.dtype == torch.float32), ids.shape[-1], _ptr(mask),
-               ctx.temperature, stats.data_ptr(), coef.data_ptr(), up.data_ptr(),
-               view.data_ptr(), view.stride(0), view.stride(1))
+        logits, ids, tl, mask = ctx.saved_tensors
+        dx = _distill(logits, ids, tl, mask, ctx.temperature, 1.0, dloss.float(), None, True)[1]
         return dx, None, None, None, None
 
 
@@ -1230,11 +1221,10 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     int64; teacher_logits [..., K] bf16 or fp32 (-inf: no entry, whatever its
     index; an index that repeats adds its weights); mask [...] bool, False rows
     are not read. Differentiable in the logits."""
+    ids, tl, mask = _teacher(_Logits(logits), teacher_ids, teacher_logits, mask)
     if logits.requires_grad and torch.is_grad_enabled():
-        return _DistillFn.apply(logits, teacher_ids, teacher_logits, mask, temperature)
-    _, _, _, loss, *_ = _distill(logits, teacher_ids, teacher_logits, mask, temperature, 1.0, None,
-                                 False, False)
-    return loss
+        return _DistillFn.apply(logits, ids, tl, mask, temperature)
+    return _distill(logits, ids, tl, mask, temperature, 1.0, None, None, False)[0]
 
 
 def distill_loss_grad(logits: torch.Tensor, teacher_ids: torch.Tensor,
@@ -1244,6 +1234,5 @@ def distill_loss_grad(logits: torch.Tensor, teacher_ids: torch.Tensor,
     """``distill_loss`` and its gradient in one pass over the logits: (loss, dlogits).
     dlogits = grad_scale * dloss/dlogits, written into ``out`` when given (which may
     be ``logits`` itself)."""
-    *_, loss, _, _, dx = _distill(logits, teacher_ids, teacher_logits, mask, temperature,
-                                  grad_scale, out, True, False)
-    return loss, dx
+    ids, tl, mask = _teacher(_Logits(logits), teacher_ids, teacher_logits, mask)
+    return _distill(logits, ids, tl, mask, temperature, grad_scale, None, out, True)

@@ -49,7 +49,7 @@ def policy(ws=FAKE, n=1 << 20, clip=(0.2, 0.2), kl=0.0, adv=FAKE, out=(None, 0, 
 
 def distill(K=3, ids=FAKE, ws=FAKE, n=1 << 20, out=(None, 0, 0)):
     return N.lib().lema_distill_loss(FAKE, 0, 2, 3, 300, 100, 100, ids, 0, FAKE, 1, K, None, 1.0,
-                                     1.0, ws, n, None, None, FAKE, *out, None)
+                                     1.0, None, ws, n, FAKE, *out, None)
 
 
 def test_losses_refuse():
