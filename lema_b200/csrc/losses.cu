@@ -102,6 +102,7 @@ struct RowArgs {
   // backward from saved statistics
   const float* g;                // [T] gradient of each row's log-probability (or row weight)
   const float* upstream;         // scalar, may be null
+  int32_t zeros_done;            // the rows of zeros are written
 };
 
 enum Objective { kLogp = 0, kPolicy = 1, kDistill = 2 };
@@ -202,46 +203,90 @@ __device__ __forceinline__ uint4 ld16(const uint4* p) {
   return r;
 }
 
-// 2^((x - m) c), c = log2(e) / tau, for the elements of a vector as packed fp32 pairs. The
-// maximum is taken off first, so that rows of the type's lowest value stay finite.
-//
-// FULL carries c as two fp32. Its rounding alone shifts every log-probability the same way
-// (2e-8 of (x - m) at tau = 1), which a sum over a sequence does not average out: the rewards of
-// 640-token sequences were 5e-6 off with c alone, 1e-6 with both. x - m is then kept above
-// -1e30, where the result is 0 all the same, because -inf times the second part would be NaN.
+// 2^((x - m) c), c = log2(e) / tau, for the elements of a vector as packed fp32 pairs, with one
+// multiply-add each: x c - fl(m c). The rounding of m c is the same factor in every exponential of
+// the row, at most 2^-13 from 1; `fix` takes it out. Rows with |m c| above 2048 (a row of the
+// type's lowest value, for one) are shifted by their maximum first, see shift_vec.
 struct ExpScale {
-  uint64_t neg_m, c, c_lo;
-  __device__ __forceinline__ ExpScale(float m, float c_, float c_lo_)
-      : neg_m(f2_splat(m == -INFINITY ? 0.f : -m)), c(f2_splat(c_)), c_lo(f2_splat(c_lo_)) {}
-};
-__device__ __forceinline__ float keep_finite(float d) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(d), "f"(-1e30f));
-  return r;
-}
-template <bool FULL>
-__device__ __forceinline__ uint64_t exp_pair(uint64_t x, const ExpScale& k) {
-  uint64_t d = f2_add(x, k.neg_m);
-  float lo, hi;
-  if (FULL) {
-    f2_unpack(d, lo, hi);
-    d = f2_pack(keep_finite(lo), keep_finite(hi));
-    f2_unpack(f2_fma(d, k.c, f2_mul(d, k.c_lo)), lo, hi);
-  } else {
-    f2_unpack(f2_mul(d, k.c), lo, hi);
+  uint64_t c, mc;
+  float fix;  // sum of exp((x - m) / tau) = fix * sum of what exp_vec gives
+  __device__ __forceinline__ ExpScale(float m, float c_) : c(f2_splat(c_)) {
+    m = m == -INFINITY ? 0.f : m;
+    const float p = m * c_;
+    mc = f2_splat(-p);
+    fix = 1.f - 0.69314718f * fmaf(m, c_, -p);  // 2^(fl(m c) - m c)
   }
+};
+__device__ __forceinline__ bool far_max(float m, float c) {
+  return fabsf(m * c) > 2048.f && m != -INFINITY;
+}
+__device__ __forceinline__ uint64_t exp_pair(uint64_t x, const ExpScale& k) {
+  float lo, hi;
+  f2_unpack(f2_fma(x, k.c, k.mc), lo, hi);
   return f2_pack(ex2(lo), ex2(hi));
 }
-template <typename T, bool FULL>
+template <typename T>
 __device__ __forceinline__ void exp_vec(const uint4& w, const ExpScale& k,
                                         uint64_t (&e)[Vec<T>::kE / 2]) {
 #pragma unroll
-  for (int i = 0; i < Vec<T>::kE / 2; ++i) e[i] = exp_pair<FULL>(Vec<T>::pair(w, i), k);
+  for (int i = 0; i < Vec<T>::kE / 2; ++i) e[i] = exp_pair(Vec<T>::pair(w, i), k);
+}
+// x - m in place of x, rounded to T. With |m c| above 2048 the elements whose exponential is not 0
+// lie within 6 percent of m, where the difference is a small multiple of their last place: exact.
+template <typename T>
+__device__ __forceinline__ void shift_vec(uint4& w, float m) {
+  uint64_t d[Vec<T>::kE / 2];
+#pragma unroll
+  for (int i = 0; i < Vec<T>::kE / 2; ++i) d[i] = f2_add(Vec<T>::pair(w, i), f2_splat(-m));
+  w = Vec<T>::pack(d);
+}
+
+// The same exponentials without the bias of ex2.approx (5e-8 of each on average, the same way in
+// every row: a preference reward sums hundreds of log-probabilities and keeps little of them,
+// and was 5e-6 off with it): 2^n p(f), n + f = (x - m) c with c in two parts, p a polynomial of
+// degree 6 with p(0) = 1, fitted to 2^f on [-1/2, 1/2] by minimax (relative error 2e-9 before
+// its fp32 roundings, whose mean is 1e-9). Exponents below -125 are taken as -125: 2^-125 next
+// to the maximum's 1 is lost in any sum. Costs six multiply-adds in place of a trip through
+// the special-function unit.
+__device__ __forceinline__ uint64_t exp_pair_exact(uint64_t x, uint64_t neg_m, const ExpScale& k,
+                                                   uint64_t c_lo, float d_min) {
+  const uint64_t magic = f2_splat(12582912.f), minus = f2_splat(-12582912.f);  // 1.5 * 2^23
+  float lo, hi;
+  f2_unpack(f2_add(x, neg_m), lo, hi);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(d_min));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(d_min));
+  const uint64_t d = f2_pack(lo, hi);
+  const uint64_t t = f2_fma(d, k.c, magic);
+  const uint64_t n = f2_add(t, minus);
+  uint64_t f = f2_fma(d, k.c, f2_fma(n, f2_splat(-1.f), f2_splat(0.f)));
+  f = f2_fma(d, c_lo, f);
+  uint64_t p = f2_splat(1.5353361959569156e-4f);
+  p = f2_fma(p, f, f2_splat(1.3398875016719103e-3f));
+  p = f2_fma(p, f, f2_splat(9.61843691766262e-3f));
+  p = f2_fma(p, f, f2_splat(5.5503323674201965e-2f));
+  p = f2_fma(p, f, f2_splat(2.4022647738456726e-1f));
+  p = f2_fma(p, f, f2_splat(6.931471824645996e-1f));
+  p = f2_fma(p, f, f2_splat(1.f));
+  // 2^n from the low bits of t; a NaN stays one in the product
+  float tl, th;
+  f2_unpack(t, tl, th);
+  return f2_mul(p, f2_pack(__uint_as_float((__float_as_uint(tl) << 23) + 0x3f800000u),
+                           __uint_as_float((__float_as_uint(th) << 23) + 0x3f800000u)));
 }
 
 template <typename T>
 __device__ __forceinline__ bool same_phase(const T* a, const T* b) {
   return ((reinterpret_cast<uintptr_t>(a) ^ reinterpret_cast<uintptr_t>(b)) & 15u) == 0;
+}
+
+// A predicated store: no branch among a row's stores.
+__device__ __forceinline__ void st16_if(uint4* p, const uint4& v, bool yes) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %5, 0;\n\t"
+      "@p st.global.v4.u32 [%0], {%1, %2, %3, %4};\n\t}\n" ::"l"(p),
+      "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w), "r"(static_cast<uint32_t>(yes))
+      : "memory");
 }
 
 // A vector whose output row starts at another phase within 16 bytes than the input row.
@@ -314,11 +359,12 @@ __device__ __forceinline__ void group_combine(float& m, double& s, float c, floa
 }
 
 // One thread's share of a row's maximum and sum: its edge and the vectors tid, tid + G, ..., in
-// one sweep with a running maximum, U loads in flight.
-template <typename T, int G, int U, bool FULL>
+// one sweep with a running maximum, U loads in flight. EXACT: by exp_pair_exact.
+template <typename T, int G, int U, bool EXACT>
 __device__ __forceinline__ void thread_stats(const T* x, const Span<T>& sp, int tid, float c,
                                              float c_lo, float& m, double& s) {
   const uint4* xv = sp.vecs(x);
+  const float d_min = -125.f / c;
   m = -INFINITY;
   float sum = 0.f;
   if (sp.head + sp.tail > 0 && tid < kEdges) {
@@ -340,18 +386,26 @@ __device__ __forceinline__ void thread_stats(const T* x, const Span<T>& sp, int 
     for (int u = 0; u < U; ++u) mx = fmaxf(mx, Vec<T>::max(w[u]));
     sum *= ex2((m - (mx == -INFINITY ? 0.f : mx)) * c);
     m = mx;
-    const ExpScale k(m, c, c_lo);
+    float at = m;
+    if (!EXACT && far_max(m, c)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) shift_vec<T>(w[u], m);
+      at = 0.f;
+    }
+    const ExpScale k(at, c);
+    const uint64_t neg_m = f2_splat(m == -INFINITY ? 0.f : -m), c_lo2 = f2_splat(c_lo);
     uint64_t acc = f2_splat(0.f);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      uint64_t e[Vec<T>::kE / 2];
-      exp_vec<T, FULL>(w[u], k, e);
 #pragma unroll
-      for (int i = 0; i < Vec<T>::kE / 2; ++i) acc = f2_add(acc, e[i]);
+      for (int i = 0; i < Vec<T>::kE / 2; ++i) {
+        const uint64_t p = Vec<T>::pair(w[u], i);
+        acc = f2_add(acc, EXACT ? exp_pair_exact(p, neg_m, k, c_lo2, d_min) : exp_pair(p, k));
+      }
     }
     float lo, hi;
     f2_unpack(acc, lo, hi);
-    sum += lo + hi;
+    sum += EXACT ? lo + hi : (lo + hi) * k.fix;
   }
   s = static_cast<double>(sum);
 }
@@ -524,7 +578,7 @@ __device__ __forceinline__ void zero_row(const RowArgs& a, int64_t r, int tid) {
 // token_logprobs: a group of G threads a row, a warp for short rows (one CTA a row leaves most
 // of its threads without a vector there).
 constexpr int kStatThreads = 256;
-template <typename T, int G>
+template <typename T, int G, bool EXACT>
 __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
   __shared__ float redf[kStatThreads / 32];
   __shared__ double redd[kStatThreads / 32];
@@ -537,6 +591,7 @@ __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
       a.logps[r] = 0.f;
       if (a.stats) a.stats[r] = make_float2(0.f, 0.f);
     }
+    zero_row<T, G>(a, r, tid);  // among reads: HBM takes writes alone at half the rate of both
     return;
   }
   const T* x = static_cast<const T*>(a.x) + a.in.at(r);
@@ -545,7 +600,7 @@ __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
   const Span<T> sp(x, a.V);
   float m;
   double s;
-  thread_stats<T, G, 4, true>(x, sp, tid, a.c, a.c_lo, m, s);
+  thread_stats<T, G, 4, EXACT>(x, sp, tid, a.c, a.c_lo, m, s);
   group_combine<G>(m, s, a.c, redf, redd);
   if (tid == 0) {
     const double lp = ok ? (static_cast<double>(xt) - m) * a.inv_tau - log(s) : NAN;
@@ -648,7 +703,7 @@ __device__ __forceinline__ float teacher_coef(const TeacherSums& t, float share)
 // k of a token of the policy loss.
 __device__ __forceinline__ float policy_coef(const RowArgs& a, const Token& tk, float xt, float m,
                                              float s, float w) {
-  const float lp = static_cast<float>((static_cast<double>(xt) - m) * a.inv_tau) - logf(s);
+  const float lp = (xt - m) * static_cast<float>(a.inv_tau) - logf(s);
   return policy_token<float, false>(a, tk, lp, nullptr, nullptr) * w;
 }
 
@@ -677,10 +732,10 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   float* s_x = s_p + a.K;
   int32_t* s_id = reinterpret_cast<int32_t*>(s_x + a.K);
   ptx::griddep_wait();
-  const int64_t job = blockIdx.x * int64_t{kGroups} + group;
-  if (job >= a.T) return;
-  const int64_t r = a.list[job];
-  if (job >= static_cast<int64_t>(a.head->total)) {
+  const int64_t r = blockIdx.x * int64_t{kGroups} + group;
+  if (r >= a.T) return;
+  int64_t target = -1;
+  if (!row_counts(a, r, target)) {
     zero_row<T, G>(a, r, tid);
     return;
   }
@@ -693,7 +748,6 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
     w[i] = tid + i * G < sp.nvec ? ld16(xv + tid + i * G) : neg_inf_vec<T>();
   const int edge = tid < kEdges ? sp.edge(tid) : -1;
   const float xe = edge >= 0 ? to_f(x[edge]) : -INFINITY;
-  const int64_t target = OBJ == kDistill ? -1 : a.targets[r];
   const bool ok = target >= 0 && target < a.V;
   const float xt = ok ? to_f(x[target]) : NAN;
   Token tk{};
@@ -717,19 +771,24 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   } else {
     __syncwarp();
   }
-  const ExpScale ks(m, a.c, a.c_lo);
+  const bool far = far_max(m, a.c);
+  if (far) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) shift_vec<T>(w[i], m);
+  }
+  const ExpScale ks(far ? 0.f : m, a.c);
   uint64_t e[NV][E / 2];
   uint64_t acc2 = f2_splat(0.f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    exp_vec<T, false>(w[i], ks, e[i]);
+    exp_vec<T>(w[i], ks, e[i]);
 #pragma unroll
     for (int j = 0; j < E / 2; ++j) acc2 = f2_add(acc2, e[i][j]);
   }
   float s, hi;
   f2_unpack(acc2, s, hi);
   const float ee = xe == -INFINITY ? 0.f : ex2((xe - m) * a.c);
-  s = warp_sum(s + hi + ee);
+  s = warp_sum((s + hi) * ks.fix + ee);
   if (G > 32) {
     if ((threadIdx.x & 31) == 0) redf[1][warp] = s;
     __syncthreads();
@@ -764,7 +823,7 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   }
   T* dx = static_cast<T*>(a.dx) + a.out.at(r);
   const float kq = (OBJ == kDistill ? k : -k) * inv_s;
-  const uint64_t kq2 = f2_splat(kq);
+  const uint64_t kq2 = f2_splat(kq * ks.fix);
   const bool same = same_phase<T>(x, dx);
   uint4* dv = reinterpret_cast<uint4*>(dx + sp.head);
 #pragma unroll
@@ -797,15 +856,24 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
 
 // ---- rows held by one CTA, or by the CTAs of a cluster ------------------------------
 
-// The same for longer rows. A persistent CTA of 512 threads holds a row, or its share of one,
-// in registers (kE * NV elements a thread); while it works, a producer warp already brings the
-// next rows into a ring of shared memory with bulk copies, so that HBM is read and written
-// without a pause, and what else the rows need: their edges, the token's numbers or the
-// teacher's entries. A cluster of cs CTAs shares rows too long for one, or few rows of any
-// length; its CTAs exchange maxima and sums through each other's shared memory.
-constexpr int kRingThreads = 512;
-constexpr int kRingWarps = kRingThreads / 32;
-constexpr int kMaxStages = 4;
+// The same for longer rows. A persistent CTA, two of them an SM, holds a row or its share of one
+// in the registers of 224 threads. Its eighth warp, the producer, brings the next rows in through
+// a ring of shared memory with bulk copies, so that HBM is read and written without a pause, and
+// with them what else the rows need: their edges, the token's numbers or the teacher's entries. A
+// chunk of the ring is free as soon as it is in registers. Rows are held as they are, not as
+// exponentials, which are taken twice (for the sum and for the gradient): half the registers,
+// hence two CTAs an SM, one of which works while the other waits for its reductions.
+//
+// A cluster of cs CTAs shares rows too long for one, or few rows of any length; its CTAs exchange
+// maxima and sums through each other's shared memory.
+constexpr int kRingWarps = 7;
+constexpr int kRingThreads = kRingWarps * 32;
+constexpr int kRingVecs = 18;                            // a thread's vectors, at most
+constexpr int kChunkVecs = 3;                            // of them in a chunk
+constexpr int kChunk = kChunkVecs * kRingThreads;        // vectors
+constexpr int kRingCap = kRingVecs * kRingThreads;       // vectors of a share, at most
+constexpr int kMaxStages = 9;
+constexpr int kZeroBytes = 8192;                         // source of the rows of zeros
 constexpr int kMaxCluster = 8;
 
 // What the producer puts down for a row, so that the consumers' registers hold the row itself.
@@ -844,16 +912,18 @@ __device__ __forceinline__ int share_owner(const Span<T>& sp, int start, int i) 
   return ((i - sp.head) / Vec<T>::kE - start) % kRingThreads;
 }
 
-__device__ __forceinline__ void ring_sync() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
+__device__ __forceinline__ void ring_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(kRingThreads) : "memory");
+}
 __device__ __forceinline__ bool ring_all(bool ok) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.u32 p, %1, 0;\n\t"
-      "bar.red.and.pred q, 1, 512, p;\n\t"
+      "bar.red.and.pred q, 1, %2, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}\n"
       : "=r"(r)
-      : "r"(static_cast<uint32_t>(ok))
+      : "r"(static_cast<uint32_t>(ok)), "n"(kRingThreads)
       : "memory");
   return r != 0;
 }
@@ -866,6 +936,11 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
           "r"(ptx::smem_u32(dst)),
       "l"(src), "r"(bytes), "r"(ptx::smem_u32(bar))
       : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(ptx::smem_u32(src)), "r"(bytes)
+               : "memory");
 }
 __device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(
@@ -882,178 +957,247 @@ __device__ __forceinline__ void store_remote(uint32_t dst, float a, float b, uin
       : "memory");
 }
 
-template <typename T, int OBJ, int NV>
-__global__ void __launch_bounds__(kRingThreads + 32, 1)
+template <typename T, int OBJ>
+__global__ void __launch_bounds__(kRingThreads + 32, 2)
     ring_kernel(RowArgs a, int cs, int per, int stages) {
   constexpr int E = Vec<T>::kE;
   extern __shared__ __align__(16) char smem[];
-  uint4* ring = reinterpret_cast<uint4*>(smem);  // [stages][per]
-  float* s_p0 = reinterpret_cast<float*>(ring + static_cast<int64_t>(stages) * per);
+  uint4* zeros = reinterpret_cast<uint4*>(smem);
+  uint4* ring = zeros + kZeroBytes / 16;  // [stages][kChunk]
+  float* s_p0 = reinterpret_cast<float*>(ring + stages * kChunk);
   float* s_x0 = s_p0 + (stages + 1) * a.K;  // each [stages + 1][K]
   int32_t* s_id0 = reinterpret_cast<int32_t*>(s_x0 + (stages + 1) * a.K);
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], exchanged[2];
-  // one more than the stages: a row's numbers are used until its end, its stage is free before
+  // A row's numbers come with its first chunk and are used until its end. The producer is at
+  // most `stages` rows ahead of a row whose first chunk every warp has read, and a warp reads
+  // that after it is done with the row before: one slot more than stages.
   __shared__ RowInfo info[kMaxStages + 1];
   __shared__ Share share[2][kMaxCluster];
-  __shared__ float red_m[kRingWarps], red_s[kRingWarps];
+  __shared__ float red_m[8], red_s[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = cs > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
-  const int64_t first = blockIdx.x / cs, step = gridDim.x / cs;
   const int start = rank * per;  // this CTA's first vector of a row; rank 0 has the edges too
   if (tid == 0) {
     for (int i = 0; i < stages; ++i) {
       ptx::mbar_init(&full[i], 1);
-      ptx::mbar_init(&empty[i], 1);
+      ptx::mbar_init(&empty[i], kRingWarps);
     }
     ptx::mbar_init(&exchanged[0], 1);
     ptx::mbar_init(&exchanged[1], 1);
     ptx::fence_mbar_init();
   }
+  for (int i = tid; i < kZeroBytes / 16; i += kRingThreads + 32) zeros[i] = make_uint4(0, 0, 0, 0);
+  ptx::fence_proxy_async_smem();  // bulk copies read them
   __syncthreads();
   if (cs > 1) ptx::cluster_sync();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   ptx::griddep_wait();
   const int64_t total = static_cast<int64_t>(a.head->total);
+  const int64_t first = blockIdx.x / cs, step = gridDim.x / cs;
 
   if (warp == kRingWarps) {
-    // ---- producer: 32 rows' numbers at a time, then each row's copy
-    int i = 0, st = 0, slot = 0;
+    // ---- producer: 32 rows' numbers at a time, then each row's copies
+    int i = 0, st = 0, slot = 0;  // chunks so far, the next one's stage, the next row's slot
     uint32_t phase = 0;
     bool ok = true, more = true;
+    // The rows of zeros, dealt to every CTA, are written between the others by bulk copies from
+    // shared memory: HBM takes writes alone at 3.9 TB/s, reads and writes together at 6.5.
+    const int64_t rest = a.T - total;
+    const int n_zero = a.dx != nullptr && rest > blockIdx.x
+                           ? static_cast<int>((rest - blockIdx.x + gridDim.x - 1) / gridDim.x)
+                           : 0;
+    const int n_row = total > first ? static_cast<int>((total - first + step - 1) / step) : 0;
+    int z = 0, done = 0;
+    const int32_t* z_list = a.list + total + blockIdx.x;
+    int32_t z_row = n_zero > 0 ? z_list[0] : 0;
+    const auto zero_rows = [&](int until) {
+      for (; z < until; ++z) {
+        T* dx = static_cast<T*>(a.dx) + a.out.at(z_row);
+        if (z + 1 < n_zero) z_row = z_list[(z + 1) * static_cast<int64_t>(gridDim.x)];
+        const Span<T> so(dx, a.V);
+        if (lane < kEdges && so.edge(lane) >= 0) put(dx + so.edge(lane), 0.f);
+        char* to = reinterpret_cast<char*>(dx + so.head);
+        const int bytes = so.nvec * 16;
+        for (int at = lane * kZeroBytes; at < bytes; at += 32 * kZeroBytes)
+          bulk_store(to + at, zeros, min(kZeroBytes, bytes - at));
+        ptx::bulk_commit_group();
+      }
+    };
     for (int64_t base = first; more && ok; base += 32 * step) {
       const int64_t job = base + lane * step;
       const bool live = job < total;
-      int64_t row = -1;
+      int64_t row = -1, x_at = 0, dx_at = 0;
       int32_t target = -1;
       Token tk{};
       float xt = NAN, w = 0.f;
       if (live) {
         row = a.list[job];
+        x_at = a.in.at(row);
+        dx_at = a.out.at(row);
         if (OBJ == kPolicy) {
           const int64_t t = a.targets[row];
           if (t >= 0 && t < a.V) {
             target = static_cast<int32_t>(t);
-            xt = to_f((static_cast<const T*>(a.x) + a.in.at(row))[t]);
+            xt = to_f((static_cast<const T*>(a.x) + x_at)[t]);
           }
           tk = load_token(a, row);
           w = static_cast<float>(token_weight(a, row) * a.inv_tau);
+        } else {
+          w = row_share(a);
         }
       }
       const int n = __popc(__ballot_sync(0xffffffffu, live));
       more = n == 32;
       for (int j = 0; j <= n && ok; ++j) {
         if (j == n && more) break;  // the end goes behind the last row
-        if (i >= stages) ok = ptx::mbar_wait(&empty[st], phase ^ 1u);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {
-          if (lane == 0) atomicMax(a.err, static_cast<int32_t>(kDevErrLossTimeout));
-          break;
-        }
         const int src = j & 31;
-        const int64_t r = j < n ? __shfl_sync(0xffffffffu, row, src) : -1;
+        const T* x = static_cast<const T*>(a.x) + __shfl_sync(0xffffffffu, x_at, src);
+        T* dx = static_cast<T*>(a.dx) + __shfl_sync(0xffffffffu, dx_at, src);
+        const int64_t r = __shfl_sync(0xffffffffu, row, src);
+        const Span<T> sp(x, a.V);
+        const int nv = j < n ? max(0, min(per, sp.nvec - start)) : 0;
+        const uint4* from = sp.vecs(x) + start;
         RowInfo* inf = &info[slot];
-        if (r >= 0) {
-          const T* x = static_cast<const T*>(a.x) + a.in.at(r);
-          T* dx = static_cast<T*>(a.dx) + a.out.at(r);
-          const Span<T> sp(x, a.V);
-          const int nv = max(0, min(per, sp.nvec - start));
-          if (lane == 0 && nv > 0) {
-            mbar_expect_tx(&full[st], nv * 16u);
-            bulk_load(ring + static_cast<int64_t>(st) * per, sp.vecs(x) + start, nv * 16u,
-                      &full[st]);
+        // at least one chunk, which brings the numbers
+        int c = 0;
+        do {
+          if (i >= stages) ok = ptx::mbar_wait(&empty[st], phase ^ 1u);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int m = min(kChunk, nv - c);
+          if (lane == 0 && m > 0) {
+            mbar_expect_tx(&full[st], m * 16u);
+            bulk_load(ring + st * kChunk, from + c, m * 16u, &full[st]);
           }
-          if (lane < kEdges) {
-            const int e = rank == 0 ? sp.edge(lane) : -1;
-            inf->edge_at[lane] = e;
-            inf->edge[lane] = e >= 0 ? to_f(x[e]) : -INFINITY;
+          if (c == 0) {
+            if (j < n) {
+              if (lane < kEdges) {
+                const int e = rank == 0 ? sp.edge(lane) : -1;
+                inf->edge_at[lane] = e;
+                inf->edge[lane] = e >= 0 ? to_f(x[e]) : -INFINITY;
+              }
+              if (OBJ == kDistill) {
+                const TeacherSums t = teacher_weights<T>(a, r, x, lane, s_p0 + slot * a.K,
+                                                         s_x0 + slot * a.K, s_id0 + slot * a.K);
+                if (lane == 0) inf->t = t;
+              }
+            }
+            if (lane == src) {
+              inf->row = j < n ? r : -1;
+              inf->dx = reinterpret_cast<char*>(dx);
+              inf->dv = reinterpret_cast<char*>(dx + sp.head + static_cast<int64_t>(start) * E);
+              inf->nv = nv;
+              inf->head = sp.head;
+              inf->nvec = sp.nvec;
+              inf->same = same_phase<T>(x, dx);
+              inf->target = target;
+              inf->owner =
+                  target >= 0 && in_share<T>(sp.head, sp.nvec, start, nv, rank, target)
+                      ? share_owner<T>(sp, start, target)
+                      : -1;
+              inf->xt = xt;
+              inf->w = w;
+              inf->tk = tk;
+            }
+            __syncwarp();
           }
-          if (OBJ == kDistill) {
-            const TeacherSums t = teacher_weights<T>(a, r, x, lane, s_p0 + slot * a.K,
-                                                     s_x0 + slot * a.K, s_id0 + slot * a.K);
-            if (lane == 0) inf->t = t;
+          if (lane == 0) ptx::mbar_arrive(&full[st]);
+          ++i;
+          if (++st == stages) {
+            st = 0;
+            phase ^= 1u;
           }
-          if (lane == src) {
-            inf->dx = reinterpret_cast<char*>(dx);
-            inf->dv = reinterpret_cast<char*>(dx + sp.head + static_cast<int64_t>(start) * E);
-            inf->nv = nv;
-            inf->head = sp.head;
-            inf->nvec = sp.nvec;
-            inf->same = same_phase<T>(x, dx);
-            inf->target = target;
-            inf->owner = target >= 0 && in_share<T>(sp.head, sp.nvec, start, nv, rank, target)
-                             ? share_owner<T>(sp, start, target)
-                             : -1;
-            inf->xt = xt;
-            inf->w = w;
-            inf->tk = tk;
-          }
-        }
-        if (lane == src) inf->row = r;
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&full[st]);
-        ++i;
+          c += kChunk;
+        } while (c < nv);
         slot = slot == stages ? 0 : slot + 1;
-        if (++st == stages) {
-          st = 0;
-          phase ^= 1u;
-        }
+        ++done;
+        if (n_zero > 0 && j < n)
+          zero_rows(static_cast<int>(static_cast<int64_t>(n_zero) * done / n_row));
       }
     }
+    zero_rows(n_zero);
+    ptx::bulk_wait_group_all();
     if (!ok) {
+      if (lane == 0) atomicMax(a.err, static_cast<int32_t>(kDevErrLossTimeout));
       // copies in flight end before this CTA does
-      for (int j = 0; j < min(i, stages); ++j) {
-        const int back = (i - 1 - j) % stages;
-        ptx::mbar_wait(&full[back], ((i - 1 - j) / stages) & 1);
-      }
+      for (int j = 0; j < min(i, stages); ++j)
+        ptx::mbar_wait(&full[(i - 1 - j) % stages], ((i - 1 - j) / stages) & 1);
     }
     __syncwarp();
   } else {
     const float factor = grad_factor(a);
-    const float each = OBJ == kDistill ? row_share(a) : 0.f;
     bool ok = true;
     int st = 0, slot = 0;
     uint32_t phase = 0;
     for (uint32_t i = 0;; ++i) {
+      const RowInfo* inf = &info[slot];
+      // the row's share into registers, and its maximum
+      uint4 w[kRingVecs];
       ok = ptx::mbar_wait(&full[st], phase) && ok;
+      const int nv = inf->nv;
+      const float xe = tid < kEdges ? inf->edge[tid] : -INFINITY;
+      float m = xe;
+#pragma unroll
+      for (int c = 0; c < kRingVecs / kChunkVecs; ++c) {
+        if (c == 0 || c * kChunk < nv) {
+          if (c > 0) ok = ptx::mbar_wait(&full[st], phase) && ok;
+          const uint4* buf = ring + st * kChunk + tid;
+#pragma unroll
+          for (int j = 0; j < kChunkVecs; ++j) w[c * kChunkVecs + j] = buf[j * kRingThreads];
+          if (nv < (c + 1) * kChunk) {  // what the chunk does not fill is old
+#pragma unroll
+            for (int j = 0; j < kChunkVecs; ++j)
+              if (c * kChunk + j * kRingThreads + tid >= nv)
+                w[c * kChunkVecs + j] = neg_inf_vec<T>();
+          }
+#pragma unroll
+          for (int j = 0; j < kChunkVecs; ++j) m = fmaxf(m, Vec<T>::max(w[c * kChunkVecs + j]));
+          __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(&empty[st]);
+          if (++st == stages) {
+            st = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      m = warp_max(m);
+      if (lane == 0) red_m[warp] = m;
+      // one barrier for the maximum and for every thread's waits: all leave here, or none
       if (!ring_all(ok)) {
         if (tid == 0) atomicMax(a.err, static_cast<int32_t>(kDevErrLossTimeout));
         break;
       }
-      const RowInfo* inf = &info[slot];
       if (inf->row < 0) break;
-      const int nv = inf->nv;
-      const uint4* buf = ring + static_cast<int64_t>(st) * per;
-      // the row's share into registers, and its maximum
-      const float xe = tid < kEdges ? inf->edge[tid] : -INFINITY;
-      uint4 w[NV];
-      float m = xe;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int v = tid + j * kRingThreads;
-        w[j] = v < nv ? buf[v] : neg_inf_vec<T>();
-        m = fmaxf(m, Vec<T>::max(w[j]));
-      }
-      m = warp_max(m);
-      if (lane == 0) red_m[warp] = m;
-      ring_sync();
-      if (tid == 0) ptx::mbar_arrive(&empty[st]);
       m = red_m[0];
 #pragma unroll
       for (int j = 1; j < kRingWarps; ++j) m = fmaxf(m, red_m[j]);
-      // exponentials, their sum
-      const ExpScale ks(m, a.c, a.c_lo);
-      uint64_t e[NV][E / 2];
-      uint64_t acc2 = f2_splat(0.f);
+      const bool far = far_max(m, a.c);
+      if (far) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        exp_vec<T, false>(w[j], ks, e[j]);
-#pragma unroll
-        for (int l = 0; l < E / 2; ++l) acc2 = f2_add(acc2, e[j][l]);
+        for (int j = 0; j < kRingVecs; ++j) shift_vec<T>(w[j], m);
       }
+      const ExpScale ks(far ? 0.f : m, a.c);
+      uint64_t acc[E / 2];
+#pragma unroll
+      for (int l = 0; l < E / 2; ++l) acc[l] = f2_splat(0.f);
+#pragma unroll
+      for (int c = 0; c < kRingVecs / kChunkVecs; ++c) {
+        if (c * kChunk < nv) {
+#pragma unroll
+          for (int j = 0; j < kChunkVecs; ++j) {
+            uint64_t e[E / 2];
+            exp_vec<T>(w[c * kChunkVecs + j], ks, e);
+#pragma unroll
+            for (int l = 0; l < E / 2; ++l) acc[l] = f2_add(acc[l], e[l]);
+          }
+        }
+      }
+      uint64_t acc2 = f2_add(acc[0], acc[1]);
+      if (E == 8) acc2 = f2_add(acc2, f2_add(acc[E / 2 - 2], acc[E / 2 - 1]));
       const float ee = xe == -INFINITY ? 0.f : ex2((xe - m) * a.c);
       float s, hi;
       f2_unpack(acc2, s, hi);
-      s = warp_sum(s + hi + ee);
+      s = warp_sum((s + hi) * ks.fix + ee);
       if (lane == 0) red_s[warp] = s;
       ring_sync();
       s = 0.f;
@@ -1081,7 +1225,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1)
       const float inv_s = 1.f / s;
       float k;
       if (OBJ == kDistill) {
-        k = teacher_coef(inf->t, each);
+        k = teacher_coef(inf->t, inf->w);
         if (tid == 0 && rank == 0) {
           if (inf->t.bad) note_bad_index(a);
           a.row[inf->row] = RowStat{m_row, s, inf->t.t_sum, 0.f, inf->t.about(m_row)};
@@ -1095,27 +1239,35 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1)
       }
       k *= factor;
       if (a.dx != nullptr) {
-        const bool zero = k == 0.f;
+        const bool zero = k == 0.f, same = inf->same;
         const float kq = zero ? 0.f : (OBJ == kDistill ? k : -k) * inv_s * scale;
-        const uint64_t kq2 = f2_splat(kq);
-        if (inf->same) {
-          uint4* dv = reinterpret_cast<uint4*>(inf->dv);
+        const uint64_t kq2 = f2_splat(kq * ks.fix);
+        uint4* dv = reinterpret_cast<uint4*>(inf->dv) + tid;
 #pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            const int v = tid + j * kRingThreads;
+        for (int c = 0; c < kRingVecs / kChunkVecs; ++c) {
+          if (c * kChunk < nv) {
+            uint4 o[kChunkVecs];
 #pragma unroll
-            for (int l = 0; l < E / 2; ++l) e[j][l] = f2_mul(e[j][l], kq2);
-            const uint4 o = Vec<T>::pack(e[j]);
-            if (v < nv) dv[v] = o;
-          }
-        } else {
-          T* de = reinterpret_cast<T*>(inf->dv);
+            for (int j = 0; j < kChunkVecs; ++j) {
+              uint64_t e[E / 2];
+              exp_vec<T>(w[c * kChunkVecs + j], ks, e);
 #pragma unroll
-          for (int j = 0; j < NV; ++j) {
-            const int v = tid + j * kRingThreads;
+              for (int l = 0; l < E / 2; ++l) e[l] = f2_mul(e[l], kq2);
+              o[j] = Vec<T>::pack(e);
+            }
+            if (same) {
 #pragma unroll
-            for (int l = 0; l < E / 2; ++l) e[j][l] = f2_mul(e[j][l], kq2);
-            if (v < nv) store_apart<T>(de + v * E, Vec<T>::pack(e[j]));
+              for (int j = 0; j < kChunkVecs; ++j) {
+                const int v = c * kChunk + j * kRingThreads;
+                st16_if(dv + v, o[j], v + tid < nv);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < kChunkVecs; ++j) {
+                const int v = c * kChunk + j * kRingThreads;
+                if (v + tid < nv) store_apart<T>(reinterpret_cast<T*>(dv + v), o[j]);
+              }
+            }
           }
         }
         T* dx = reinterpret_cast<T*>(inf->dx);
@@ -1141,13 +1293,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 1)
         }
       }
       slot = slot == stages ? 0 : slot + 1;
-      if (++st == stages) {
-        st = 0;
-        phase ^= 1u;
-      }
     }
-    for (int64_t job = total + blockIdx.x; job < a.T; job += gridDim.x)
-      zero_row<T, kRingThreads>(a, a.list[job], tid);
   }
   if (cs > 1) ptx::cluster_sync();  // no CTA leaves while another may still write to it
 }
@@ -1168,17 +1314,15 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
   __shared__ TeacherSums s_t;
   const int tid = threadIdx.x;
   ptx::griddep_wait();
-  const int64_t total = static_cast<int64_t>(a.head->total);
   const float factor = grad_factor(a);
-  for (int64_t job = blockIdx.x; job < a.T; job += gridDim.x) {
-    const int64_t r = a.list[job];
-    if (job >= total) {
+  for (int64_t r = blockIdx.x; r < a.T; r += gridDim.x) {
+    int64_t target = -1;
+    if (!row_counts(a, r, target)) {
       zero_row<T, kRowThreads>(a, r, tid);
       continue;
     }
     const T* x = static_cast<const T*>(a.x) + a.in.at(r);
     const Span<T> sp(x, a.V);
-    const int64_t target = OBJ == kDistill ? -1 : a.targets[r];
     const bool ok = target >= 0 && target < a.V;
     const float xt = ok ? to_f(x[target]) : NAN;
     const int edge = tid < kEdges ? sp.edge(tid) : -1;
@@ -1213,14 +1357,17 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
     } else if (a.dx != nullptr) {
       T* dx = static_cast<T*>(a.dx) + a.out.at(r);
       const bool same = same_phase<T>(x, dx);
-      const ExpScale ks(m, a.c, a.c_lo);
+      const bool far = far_max(m, a.c);
+      const ExpScale ks(far ? 0.f : m, a.c);
       const float kq = (OBJ == kDistill ? k : -k) * inv_s;
-      const uint64_t kq2 = f2_splat(kq);
+      const uint64_t kq2 = f2_splat(kq * ks.fix);
       const uint4* xv = sp.vecs(x);
       uint4* dv = reinterpret_cast<uint4*>(dx + sp.head);
       for (int v = tid; v < sp.nvec; v += kRowThreads) {
         uint64_t e[E / 2];
-        exp_vec<T, false>(ld16(xv + v), ks, e);
+        uint4 w = ld16(xv + v);
+        if (far) shift_vec<T>(w, m);
+        exp_vec<T>(w, ks, e);
 #pragma unroll
         for (int i = 0; i < E / 2; ++i) e[i] = f2_mul(e[i], kq2);
         if (same)
@@ -1362,6 +1509,7 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
   const T* x = static_cast<const T*>(a.x) + a.in.at(r);
   T* dx = static_cast<T*>(a.dx) + a.out.at(r);
   const int64_t target = a.targets[r];
+  if (a.zeros_done && target == a.ignore) return;
   const float k =
       target == a.ignore ? 0.f : a.g[r] * grad_factor(a) * static_cast<float>(a.inv_tau);
   if (k == 0.f) {
@@ -1381,9 +1529,10 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
   for (int u = 0; u < kBwdU; ++u)
     if (v0 + u * G < sp.nvec) w[u] = ld16(xv + v0 + u * G);
   const float2 st = a.stats[r];
-  const ExpScale ks(st.x, a.c, a.c_lo);
+  const bool far = far_max(st.x, a.c);
+  const ExpScale ks(far ? 0.f : st.x, a.c);
   const float kq = -k * st.y;
-  const uint64_t kq2 = f2_splat(kq);
+  const uint64_t kq2 = f2_splat(kq * ks.fix);
   const bool same = same_phase<T>(x, dx);
   uint4* dv = reinterpret_cast<uint4*>(dx + sp.head);
   // the target's value, by the thread that has just written what the others hold there
@@ -1395,7 +1544,8 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
     const int v = v0 + u * G;
     if (v >= sp.nvec) continue;
     uint64_t e[E / 2];
-    exp_vec<T, false>(w[u], ks, e);
+    if (far) shift_vec<T>(w[u], st.x);
+    exp_vec<T>(w[u], ks, e);
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) e[i] = f2_mul(e[i], kq2);
     if (same)
@@ -1518,22 +1668,25 @@ int launch_after(void (*kern)(P...), int64_t grid, int threads, int smem, int cs
 // A warp a row while four vectors a lane hold it.
 bool warp_rows(int nvec) { return nvec <= 128; }
 
-template <typename T>
+template <typename T, bool EXACT>
 int launch_logprobs_t(const RowArgs& a, int nvec, cudaStream_t s) {
   if (warp_rows(nvec)) {
     const int64_t per = kStatThreads / 32;
-    logprobs_kernel<T, 32><<<static_cast<unsigned>((a.T + per - 1) / per), kStatThreads, 0, s>>>(a);
+    logprobs_kernel<T, 32, EXACT>
+        <<<static_cast<unsigned>((a.T + per - 1) / per), kStatThreads, 0, s>>>(a);
   } else {
-    logprobs_kernel<T, kStatThreads><<<static_cast<unsigned>(a.T), kStatThreads, 0, s>>>(a);
+    logprobs_kernel<T, kStatThreads, EXACT>
+        <<<static_cast<unsigned>(a.T), kStatThreads, 0, s>>>(a);
   }
   LEMA_CUDA_TRY(cudaGetLastError());
   return LEMA_OK;
 }
 
+template <bool EXACT>
 int launch_logprobs(const RowArgs& a, int x_f32, cudaStream_t s) {
   const int nvec = max_vecs(a, x_f32);
-  return x_f32 ? launch_logprobs_t<float>(a, nvec, s)
-               : launch_logprobs_t<__nv_bfloat16>(a, nvec, s);
+  return x_f32 ? launch_logprobs_t<float, EXACT>(a, nvec, s)
+               : launch_logprobs_t<__nv_bfloat16, EXACT>(a, nvec, s);
 }
 
 template <typename T>
@@ -1557,7 +1710,7 @@ int launch_logprobs_bwd(const RowArgs& a, int x_f32, cudaStream_t s) {
                : launch_logprobs_bwd_t<__nv_bfloat16>(a, nvec, s);
 }
 
-constexpr int kRingSmem = 216 * 1024;
+constexpr int kRingSmem = 108 * 1024;  // two CTAs an SM
 
 template <typename Kern>
 int allow_smem(Kern kern, int bytes, std::atomic<uint64_t>& done) {
@@ -1573,7 +1726,7 @@ int allow_smem(Kern kern, int bytes, std::atomic<uint64_t>& done) {
 // Clusters of cs CTAs that are resident at once.
 template <typename Kern>
 int resident_clusters(Kern kern, int cs, int smem, int* out) {
-  static std::atomic<int> cache[64][4];  // by device and log2(cs); 1 CTA an SM either way
+  static std::atomic<int> cache[64][4];  // by device and log2(cs); 2 CTAs an SM either way
   const int dev = current_device(), slot = cs == 2 ? 1 : (cs == 4 ? 2 : 3);
   int n = cache[dev][slot].load();
   if (n == 0) {
@@ -1595,19 +1748,18 @@ int resident_clusters(Kern kern, int cs, int smem, int* out) {
   return LEMA_OK;
 }
 
-template <typename T, int OBJ, int NV>
+template <typename T, int OBJ>
 int launch_ring(const RowArgs& a, int cs, int per, cudaStream_t s) {
-  const int stage = per * 16;
-  int stages = 0, smem = 0;
-  for (int n = kMaxStages; n >= 1 && stages == 0; --n) {
-    smem = n * stage + (n + 1) * a.K * 12;
-    if (smem <= kRingSmem) stages = n;
-  }
-  auto kern = ring_kernel<T, OBJ, NV>;
+  auto kern = ring_kernel<T, OBJ>;
   static std::atomic<uint64_t> done{0};
   int rc = allow_smem(kern, kRingSmem, done);
   if (rc) return rc;
-  int clusters = device_sm_count();
+  int stages = kMaxStages, smem = 0;
+  for (;; --stages) {
+    smem = kZeroBytes + stages * kChunk * 16 + (stages + 1) * a.K * 12;
+    if (smem <= kRingSmem) break;
+  }
+  int clusters = 2 * device_sm_count();
   if (cs > 1 && (rc = resident_clusters(kern, cs, smem, &clusters))) return rc;
   const int64_t n = std::min<int64_t>(a.T, clusters);
   return launch_after(kern, n * cs, kRingThreads + 32, smem, cs, s, a, cs, per, stages);
@@ -1641,18 +1793,15 @@ int launch_rows(const RowArgs& a, int nvec, cudaStream_t s) {
     return launch_direct<T, OBJ, 128, kNv>(a, grid, smem, s);
   }
   int cs = 1;
-  while (cs < kMaxCluster && nvec > cs * kRingThreads * kNv) cs *= 2;
-  if (nvec > cs * kRingThreads * kNv)
+  while (cs < kMaxCluster && nvec > cs * kRingCap) cs *= 2;
+  if (nvec > cs * kRingCap)
     return launch_after(stream_kernel<T, OBJ>, std::min<int64_t>(a.T, 2 * device_sm_count()),
                         kRowThreads, teacher, 1, s, a);
   // few rows: spread each while SMs would be idle and every thread still has a vector
   while (cs < kMaxCluster && a.T * cs * 2 <= device_sm_count() &&
          nvec >= cs * 2 * kRingThreads)
     cs *= 2;
-  const int share = (nvec + cs - 1) / cs;
-  if (share <= kRingThreads * kNv / 4) return launch_ring<T, OBJ, kNv / 4>(a, cs, share, s);
-  if (share <= kRingThreads * kNv / 2) return launch_ring<T, OBJ, kNv / 2>(a, cs, share, s);
-  return launch_ring<T, OBJ, kNv>(a, cs, share, s);
+  return launch_ring<T, OBJ>(a, cs, (nvec + cs - 1) / cs, s);
 }
 
 // The list of rows, their statistics and gradients, the tokens' terms.
@@ -1713,7 +1862,7 @@ extern "C" int lema_token_logprobs(const void* x, int32_t x_f32, int64_t n0, int
   a.ignore = ignore_index;
   a.logps = logps;
   if ((rc = set_stats(a, stats))) return rc;
-  return launch_logprobs(a, x_f32, static_cast<cudaStream_t>(stream));
+  return launch_logprobs<false>(a, x_f32, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int lema_token_logprobs_bwd(const void* x, int32_t x_f32, int64_t n0, int64_t n1,
@@ -1763,7 +1912,7 @@ extern "C" int lema_preference_loss(const void* x, int32_t x_f32, int64_t n0, in
   if ((rc = set_stats(a, stats))) return rc;
   a.coef = coef;
   auto s = static_cast<cudaStream_t>(stream);
-  if (a.T > 0 && (rc = launch_logprobs(a, x_f32, s))) return rc;
+  if (a.T > 0 && (rc = launch_logprobs<true>(a, x_f32, s))) return rc;
   pair_kernel<<<static_cast<unsigned>(n0 / 2), 256, 0, s>>>(a, n0 / 2, beta, label_smoothing,
                                                             rewards);
   LEMA_CUDA_TRY(cudaGetLastError());
@@ -1771,6 +1920,7 @@ extern "C" int lema_preference_loss(const void* x, int32_t x_f32, int64_t n0, in
   LEMA_CUDA_TRY(cudaGetLastError());
   if (dx == nullptr || a.T == 0) return LEMA_OK;
   a.g = coef;
+  a.zeros_done = 1;
   a.grad_scale = static_cast<float>(grad_scale);
   return launch_logprobs_bwd(a, x_f32, s);
 }
