@@ -65,8 +65,8 @@ struct RowArgs {
   RowMap in;
   int64_t T;
   int32_t V;
-  double inv_tau;                // 1 / tau
-  float c, c_lo;                 // log2(e) / tau, rounded, and what the rounding left
+  double inv_tau, c_full;        // 1 / tau, log2(e) / tau
+  float c, c_lo;                 // log2(e) / tau, rounded down, and what the rounding left
   const int64_t* targets;        // [T]; null for distill
   int64_t ignore;
   float* logps;                  // [T]
@@ -118,6 +118,13 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// The larger of two, NaN if either is.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // ---- 16-byte vectors of a row ---------------------------------------------------
 // A row may start at any element: its aligned 16-byte vectors are moved whole, the elements in
 // front of the first and behind the last (its edges, fewer than a vector each) one by one, by
@@ -137,6 +144,12 @@ struct Vec<__nv_bfloat16> {
     const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
     return fmaxf(__low2float(m), __high2float(m));
   }
+  static __device__ __forceinline__ float max_nan(const uint4& v) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+    const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+    const float a = __low2float(m), b = __high2float(m);
+    return max_or_nan(a, b);
+  }
   static __device__ __forceinline__ uint4 pack(const uint64_t (&p)[4]) {
     return make_uint4(bf16x2_from_f2(p[0]), bf16x2_from_f2(p[1]), bf16x2_from_f2(p[2]),
                       bf16x2_from_f2(p[3]));
@@ -153,6 +166,10 @@ struct Vec<float> {
   static __device__ __forceinline__ float max(const uint4& v) {
     return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
                  fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+  }
+  static __device__ __forceinline__ float max_nan(const uint4& v) {
+    return max_or_nan(max_or_nan(__uint_as_float(v.x), __uint_as_float(v.y)),
+                            max_or_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
   static __device__ __forceinline__ uint4 pack(const uint64_t (&p)[2]) {
     float a, b, c, d;
@@ -214,9 +231,17 @@ struct ExpScale {
     m = m == -INFINITY ? 0.f : m;
     const float p = m * c_;
     mc = f2_splat(-p);
-    fix = 1.f - 0.69314718f * fmaf(m, c_, -p);  // 2^(fl(m c) - m c)
+    fix = 1.f - 0.69314718f * fmaf(m, c_, -p);  // 2^(p - m c)
   }
 };
+// The whole number nearest to m c (0 for a maximum without one).
+__device__ __forceinline__ float whole_max(float m, float c) {
+  return m == -INFINITY ? 0.f : rintf(m * c);
+}
+// 2^n for whole n <= 0.
+__device__ __forceinline__ float exp2_whole(float n) {
+  return n < -126.f ? 0.f : __uint_as_float(static_cast<uint32_t>(static_cast<int>(n) + 127) << 23);
+}
 __device__ __forceinline__ bool far_max(float m, float c) {
   return fabsf(m * c) > 2048.f && m != -INFINITY;
 }
@@ -241,37 +266,48 @@ __device__ __forceinline__ void shift_vec(uint4& w, float m) {
   w = Vec<T>::pack(d);
 }
 
-// The same exponentials without the bias of ex2.approx (5e-8 of each on average, the same way in
-// every row: a preference reward sums hundreds of log-probabilities and keeps little of them,
-// and was 5e-6 off with it): 2^n p(f), n + f = (x - m) c with c in two parts, p a polynomial of
-// degree 6 with p(0) = 1, fitted to 2^f on [-1/2, 1/2] by minimax (relative error 2e-9 before
-// its fp32 roundings, whose mean is 1e-9). Exponents below -125 are taken as -125: 2^-125 next
-// to the maximum's 1 is lost in any sum. Costs six multiply-adds in place of a trip through
-// the special-function unit.
-__device__ __forceinline__ uint64_t exp_pair_exact(uint64_t x, uint64_t neg_m, const ExpScale& k,
-                                                   uint64_t c_lo, float d_min) {
-  const uint64_t magic = f2_splat(12582912.f), minus = f2_splat(-12582912.f);  // 1.5 * 2^23
-  float lo, hi;
-  f2_unpack(f2_add(x, neg_m), lo, hi);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(d_min));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(d_min));
-  const uint64_t d = f2_pack(lo, hi);
-  const uint64_t t = f2_fma(d, k.c, magic);
-  const uint64_t n = f2_add(t, minus);
-  uint64_t f = f2_fma(d, k.c, f2_fma(n, f2_splat(-1.f), f2_splat(0.f)));
-  f = f2_fma(d, c_lo, f);
-  uint64_t p = f2_splat(1.5353361959569156e-4f);
-  p = f2_fma(p, f, f2_splat(1.3398875016719103e-3f));
-  p = f2_fma(p, f, f2_splat(9.61843691766262e-3f));
-  p = f2_fma(p, f, f2_splat(5.5503323674201965e-2f));
-  p = f2_fma(p, f, f2_splat(2.4022647738456726e-1f));
-  p = f2_fma(p, f, f2_splat(6.931471824645996e-1f));
-  p = f2_fma(p, f, f2_splat(1.f));
-  // 2^n from the low bits of t; a NaN stays one in the product
-  float tl, th;
-  f2_unpack(t, tl, th);
-  return f2_mul(p, f2_pack(__uint_as_float((__float_as_uint(tl) << 23) + 0x3f800000u),
-                           __uint_as_float((__float_as_uint(th) << 23) + 0x3f800000u)));
+// The same about a whole n, sums about different n meeting exactly, for log-probabilities that are
+// added up: a preference reward sums hundreds of them and keeps little, so what shifts them all
+// the same way shows (it was 2e-5 off with exp_vec). That is c's own rounding, 1e-8 of x - m,
+// added back here with a second multiply-add; and ex2.approx, which is 5e-8 low on average but 1e-8
+// on [-1/2, 1/2], where its argument is brought here. Elements are kept above n - 120, which
+// is nothing beside the maximum. NaNs are looked for apart.
+struct WholeScale {
+  uint64_t c, c_lo, up, down;  // 1.5 * 2^23 - n, added and taken off: rounds to a whole number
+  __device__ __forceinline__ WholeScale(float n, float c_, float c_lo_)
+      : c(f2_splat(c_)), c_lo(f2_splat(c_lo_)), up(f2_splat(12582912.f - n)),
+        down(f2_splat(n - 12582912.f)) {}
+};
+__device__ __forceinline__ uint64_t exp_pair_whole(uint64_t x, const WholeScale& k) {
+  const uint64_t t = f2_fma(x, k.c, k.up);
+  const uint64_t minus_u = f2_fma(f2_add(t, k.down), f2_splat(-1.f), f2_splat(0.f));
+  float f0, f1, t0, t1;
+  f2_unpack(f2_fma(x, k.c_lo, f2_fma(x, k.c, minus_u)), f0, f1);
+  f2_unpack(t, t0, t1);
+  // times 2^(u - n): the low bits of t, into the exponent
+  return f2_pack(__uint_as_float(__float_as_uint(ex2(f0)) + (__float_as_uint(t0) << 23)),
+                 __uint_as_float(__float_as_uint(ex2(f1)) + (__float_as_uint(t1) << 23)));
+}
+__device__ __forceinline__ void keep_above(uint4& w, float low, __nv_bfloat16) {
+  const __nv_bfloat162 l = __float2bfloat162_rn(low);
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __hmax2(h[i], l);
+}
+__device__ __forceinline__ void keep_above(uint4& w, float low, float) {
+  float* f = reinterpret_cast<float*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f[i] = fmaxf(f[i], low);
+}
+
+// The logarithm of what exp_pair_whole gives for the target over what it should give: the sum of
+// a row's exponentials is off alike on average, so adding this to the target's log-probability
+// leaves what does not add up over a sequence.
+__device__ __forceinline__ double ex2_error(float x, const RowArgs& a) {
+  const double e = static_cast<double>(x) * a.c_full;
+  const float f = static_cast<float>(e - rint(e));
+  if (!(fabsf(f) <= 0.5f)) return 0.0;
+  return log(static_cast<double>(ex2(f))) - 0.6931471805599453 * static_cast<double>(f);
 }
 
 template <typename T>
@@ -330,10 +366,11 @@ __device__ __forceinline__ void group_sync() {
     __syncthreads();
 }
 
-// Maximum and sum of a row from the (m, s) of a group's threads; every thread gets both. The
-// threads' sums are added in fp64.
-template <int G>
-__device__ __forceinline__ void group_combine(float& m, double& s, float c, float* redf,
+// Maximum of a row and sum of exp((x - m) / tau) from the (m, s) of a group's threads; every
+// thread gets both. WHOLE: their sums are about whole_max of their own maxima (about the maximum
+// itself when far_max). Sums meet in fp64.
+template <int G, bool WHOLE>
+__device__ __forceinline__ void group_combine(float& m, double& s, const RowArgs& a, float* redf,
                                               double* redd) {
   const float mt = m;
   const int warp = (threadIdx.x % G) >> 5;
@@ -346,8 +383,11 @@ __device__ __forceinline__ void group_combine(float& m, double& s, float c, floa
 #pragma unroll
     for (int w = 1; w < G / 32; ++w) m = fmaxf(m, redf[w]);
   }
-  // a thread that saw only -inf adds nothing; a row of -inf alone becomes NaN
-  s *= static_cast<double>(ex2((mt - m) * c));
+  // a thread that saw only -inf adds nothing
+  const bool far = !WHOLE || far_max(m, a.c);
+  const float n = whole_max(m, a.c);
+  const float f = far || far_max(mt, a.c) ? ex2((mt - m) * a.c) : exp2_whole(whole_max(mt, a.c) - n);
+  s *= mt == -INFINITY ? 0.0 : static_cast<double>(f);
   s = warp_sum(s);
   if (G > 32) {
     if ((threadIdx.x & 31) == 0) redd[warp] = s;
@@ -356,25 +396,26 @@ __device__ __forceinline__ void group_combine(float& m, double& s, float c, floa
 #pragma unroll
     for (int w = 1; w < G / 32; ++w) s += redd[w];
   }
+  // from about n to about m; a row of -inf alone is NaN
+  if (!far) s *= exp2(static_cast<double>(n) - static_cast<double>(m) * a.c_full);
+  if (m == -INFINITY) s = NAN;
 }
 
 // One thread's share of a row's maximum and sum: its edge and the vectors tid, tid + G, ..., in
-// one sweep with a running maximum, U loads in flight. EXACT: by exp_pair_exact.
-template <typename T, int G, int U, bool EXACT>
+// one sweep with a running maximum, U loads in flight.
+template <typename T, int G, int U, bool WHOLE>
 __device__ __forceinline__ void thread_stats(const T* x, const Span<T>& sp, int tid, float c,
                                              float c_lo, float& m, double& s) {
   const uint4* xv = sp.vecs(x);
-  const float d_min = -125.f / c;
   m = -INFINITY;
   float sum = 0.f;
   if (sp.head + sp.tail > 0 && tid < kEdges) {
     const int i = sp.edge(tid);
-    if (i >= 0) {
-      m = to_f(x[i]);
-      // 1, or NaN for an element without a value; an element of -inf adds nothing
-      sum = m == -INFINITY ? 0.f : m - m + 1.f;
-      if (m != m) m = -INFINITY;
-    }
+    const float xe = i >= 0 ? to_f(x[i]) : -INFINITY;
+    if (xe != xe || xe == INFINITY) sum = NAN;
+    if (fabsf(xe) < INFINITY)
+      sum = WHOLE && !far_max(xe, c) ? ex2(fmaf(xe, c, -whole_max(xe, c)) + xe * c_lo) : 1.f;
+    if (xe == xe) m = xe;
   }
   for (int base = tid; base < sp.nvec; base += G * U) {
     uint4 w[U];
@@ -382,30 +423,43 @@ __device__ __forceinline__ void thread_stats(const T* x, const Span<T>& sp, int 
     for (int u = 0; u < U; ++u)
       w[u] = base + u * G < sp.nvec ? ld16(xv + base + u * G) : neg_inf_vec<T>();
     float mx = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u) mx = fmaxf(mx, Vec<T>::max(w[u]));
-    sum *= ex2((m - (mx == -INFINITY ? 0.f : mx)) * c);
-    m = mx;
-    float at = m;
-    if (!EXACT && far_max(m, c)) {
-#pragma unroll
-      for (int u = 0; u < U; ++u) shift_vec<T>(w[u], m);
-      at = 0.f;
-    }
-    const ExpScale k(at, c);
-    const uint64_t neg_m = f2_splat(m == -INFINITY ? 0.f : -m), c_lo2 = f2_splat(c_lo);
-    uint64_t acc = f2_splat(0.f);
+    bool nan = false;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      const float v = WHOLE ? Vec<T>::max_nan(w[u]) : Vec<T>::max(w[u]);
+      if (WHOLE) nan |= v != v;
+      mx = fmaxf(mx, v);
+    }
+    if (WHOLE && (nan || mx == INFINITY)) {
+      sum = NAN;  // and stays so
+      mx = m;
+    }
+    const bool far = far_max(mx, c);
+    const float n = far ? 0.f : whole_max(mx, c);
+    if (m != -INFINITY)  // the sum so far, about the new maximum
+      sum *= !WHOLE || far || far_max(m, c) ? ex2((m - mx) * c)
+                                            : exp2_whole(whole_max(m, c) - n);
+    m = mx;
+    if (far) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) shift_vec<T>(w[u], m);
+    }
+    const ExpScale k(far ? 0.f : m, c);
+    const WholeScale kw(n, c, c_lo);
+    const float low = (n - 120.f) / c;
+    uint64_t acc[2] = {f2_splat(0.f), f2_splat(0.f)};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (WHOLE) keep_above(w[u], low, T());
 #pragma unroll
       for (int i = 0; i < Vec<T>::kE / 2; ++i) {
         const uint64_t p = Vec<T>::pair(w[u], i);
-        acc = f2_add(acc, EXACT ? exp_pair_exact(p, neg_m, k, c_lo2, d_min) : exp_pair(p, k));
+        acc[i & 1] = f2_add(acc[i & 1], WHOLE ? exp_pair_whole(p, kw) : exp_pair(p, k));
       }
     }
     float lo, hi;
-    f2_unpack(acc, lo, hi);
-    sum += EXACT ? lo + hi : (lo + hi) * k.fix;
+    f2_unpack(f2_add(acc[0], acc[1]), lo, hi);
+    sum += WHOLE ? lo + hi : (lo + hi) * k.fix;
   }
   s = static_cast<double>(sum);
 }
@@ -578,7 +632,7 @@ __device__ __forceinline__ void zero_row(const RowArgs& a, int64_t r, int tid) {
 // token_logprobs: a group of G threads a row, a warp for short rows (one CTA a row leaves most
 // of its threads without a vector there).
 constexpr int kStatThreads = 256;
-template <typename T, int G, bool EXACT>
+template <typename T, int G, bool WHOLE>
 __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
   __shared__ float redf[kStatThreads / 32];
   __shared__ double redd[kStatThreads / 32];
@@ -600,10 +654,12 @@ __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
   const Span<T> sp(x, a.V);
   float m;
   double s;
-  thread_stats<T, G, 4, EXACT>(x, sp, tid, a.c, a.c_lo, m, s);
-  group_combine<G>(m, s, a.c, redf, redd);
+  thread_stats<T, G, 4, WHOLE>(x, sp, tid, a.c, a.c_lo, m, s);
+  group_combine<G, WHOLE>(m, s, a, redf, redd);
   if (tid == 0) {
-    const double lp = ok ? (static_cast<double>(xt) - m) * a.inv_tau - log(s) : NAN;
+    const double lp =
+        ok ? (static_cast<double>(xt) - m) * a.inv_tau + (WHOLE ? ex2_error(xt, a) : 0.0) - log(s)
+           : NAN;
     if (!ok) atomicMax(a.err, static_cast<int32_t>(kDevErrIndex));
     a.logps[r] = static_cast<float>(lp);
     if (a.lp64) a.lp64[r] = lp;
@@ -1334,7 +1390,7 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
     float m;
     double sd;
     thread_stats<T, kRowThreads, 4, false>(x, sp, tid, a.c, a.c_lo, m, sd);
-    group_combine<kRowThreads>(m, sd, a.c, redf, redd);
+    group_combine<kRowThreads, false>(m, sd, a, redf, redd);
     const float s = static_cast<float>(sd), inv_s = 1.f / s;
     float k;
     if (OBJ == kDistill) {
@@ -1589,8 +1645,10 @@ int make_rows(RowArgs& a, const void* x, int64_t n0, int64_t n1, int64_t ld0, in
   a.V = static_cast<int32_t>(V);
   a.inv_tau = 1.0 / temperature;
   const double c = 1.4426950408889634 / temperature;
+  a.c_full = c;
   a.c = static_cast<float>(c);
-  a.c_lo = static_cast<float>(c - static_cast<double>(a.c));
+  if (static_cast<double>(a.c) >= c) a.c = std::nextafterf(a.c, 0.f);
+  a.c_lo = static_cast<float>(c - static_cast<double>(a.c));  // > 0
   a.grad_scale = 1.f;
   return LEMA_OK;
 }
@@ -1668,25 +1726,25 @@ int launch_after(void (*kern)(P...), int64_t grid, int threads, int smem, int cs
 // A warp a row while four vectors a lane hold it.
 bool warp_rows(int nvec) { return nvec <= 128; }
 
-template <typename T, bool EXACT>
+template <typename T, bool WHOLE>
 int launch_logprobs_t(const RowArgs& a, int nvec, cudaStream_t s) {
   if (warp_rows(nvec)) {
     const int64_t per = kStatThreads / 32;
-    logprobs_kernel<T, 32, EXACT>
+    logprobs_kernel<T, 32, WHOLE>
         <<<static_cast<unsigned>((a.T + per - 1) / per), kStatThreads, 0, s>>>(a);
   } else {
-    logprobs_kernel<T, kStatThreads, EXACT>
+    logprobs_kernel<T, kStatThreads, WHOLE>
         <<<static_cast<unsigned>(a.T), kStatThreads, 0, s>>>(a);
   }
   LEMA_CUDA_TRY(cudaGetLastError());
   return LEMA_OK;
 }
 
-template <bool EXACT>
+template <bool WHOLE>
 int launch_logprobs(const RowArgs& a, int x_f32, cudaStream_t s) {
   const int nvec = max_vecs(a, x_f32);
-  return x_f32 ? launch_logprobs_t<float, EXACT>(a, nvec, s)
-               : launch_logprobs_t<__nv_bfloat16, EXACT>(a, nvec, s);
+  return x_f32 ? launch_logprobs_t<float, WHOLE>(a, nvec, s)
+               : launch_logprobs_t<__nv_bfloat16, WHOLE>(a, nvec, s);
 }
 
 template <typename T>
