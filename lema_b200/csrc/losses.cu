@@ -1891,7 +1891,11 @@ int set_stats(RowArgs& a, const float* stats) {
 }
 
 int need_err(RowArgs& a) {
-  a.err = gemm_error_word();
+  static std::atomic<int32_t*> word[64];  // one a device
+  const int dev = current_device();
+  if (dev < 0 || dev >= 64) return set_error(LEMA_ERR_CUDA, "bad device");
+  a.err = word[dev].load();
+  if (a.err == nullptr) word[dev].store(a.err = gemm_error_word());
   return a.err ? LEMA_OK : set_error(LEMA_ERR_CUDA, "cannot resolve device error word");
 }
 

@@ -26,6 +26,7 @@ on the current torch stream of the tensors' device.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -844,32 +845,34 @@ class _Logits:
     checks every loss makes. Copies only when the last stride is not 1 or the
     leading dimensions cannot be seen as [sequences, rows]."""
 
-    __slots__ = ("t", "dev", "lead", "n0", "n1", "ld0", "ld1", "V", "args")
+    __slots__ = ("t", "dev", "lead", "n0", "n1", "V", "args")
 
     def __init__(self, logits: torch.Tensor):
         if not logits.is_cuda:
             _require_cuda(logits)
-        if logits.dtype not in (torch.bfloat16, torch.float32):
-            raise TypeError(f"logits must be bf16 or fp32, got {logits.dtype}")
-        if logits.dim() < 2:
-            raise ValueError(f"logits must be [..., V], got shape {tuple(logits.shape)}")
-        self.lead = logits.shape[:-1]
-        self.V = logits.shape[-1]
-        if self.V < 1:
-            raise ValueError("logits need at least one vocabulary entry")
+        dtype = logits.dtype
+        if dtype is not torch.bfloat16 and dtype is not torch.float32:
+            raise TypeError(f"logits must be bf16 or fp32, got {dtype}")
+        shape = logits.shape
+        V = shape[-1] if len(shape) > 1 else 0
+        if V < 1:
+            raise ValueError(f"logits must be [..., V] with V >= 1, got shape {tuple(shape)}")
+        self.lead = shape[:-1]
+        self.V = V
         self.dev = logits.device
         t = logits
-        if t.dim() > 3:
-            t = t.reshape(-1, t.shape[-2], self.V)
-        elif t.dim() == 2:
+        if len(shape) == 2:
             t = t[None]
-        if t.stride(2) != 1 and self.V > 1:
+        elif len(shape) > 3:
+            t = t.reshape(-1, shape[-2], V)
+        st = t.stride()
+        if st[2] != 1 and V > 1:
             t = t.contiguous()
+            st = t.stride()
         self.t = t
         self.n0, self.n1 = t.shape[0], t.shape[1]
-        self.ld0, self.ld1 = t.stride(0), t.stride(1)
-        self.args = (t.data_ptr(), int(t.dtype == torch.float32), self.n0, self.n1, self.ld0,
-                     self.ld1, self.V)
+        self.args = (t.data_ptr(), 1 if dtype is torch.float32 else 0, self.n0, self.n1, st[0],
+                     st[1], V)
 
     def per_row(self, t: torch.Tensor | None, name: str, dtype: torch.dtype):
         """A contiguous [rows] companion of the logits, on their device."""
@@ -877,7 +880,7 @@ class _Logits:
             return None
         if t.device != self.dev:
             raise RuntimeError(f"{name} on {t.device}, logits on {self.dev}")
-        if t.dtype != dtype:
+        if t.dtype is not dtype:
             raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
         if t.shape != self.lead:
             raise ValueError(f"{name} must have shape {tuple(self.lead)}, got {tuple(t.shape)}")
@@ -886,43 +889,58 @@ class _Logits:
         return t.contiguous()
 
     def grad_out(self, logits: torch.Tensor, out: torch.Tensor | None):
-        """(gradient tensor, its [sequences, rows, V] view)."""
+        """(gradient tensor, its pointer, its two row strides)."""
         if out is None:
             out = torch.empty(logits.shape, dtype=logits.dtype, device=self.dev)
-        else:
-            if out.shape != logits.shape or out.dtype != logits.dtype or out.device != self.dev:
-                raise ValueError("out must have the logits' shape, type and device")
-            if out.requires_grad:
-                raise ValueError("out must not require grad: detach it")
-            same = (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride())
-            if out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr() \
-                    and out.numel() and not same:
-                raise ValueError("out shares the logits' storage without being the logits")
-            if not _rows_disjoint(out):
-                raise ValueError("out needs a unit last stride and rows that do not overlap")
-            if same and self.t.data_ptr() != logits.data_ptr():
-                raise ValueError("out: these logits have to be copied, so out cannot be they")
-            torch.autograd.graph.increment_version(out)
+            return out, (out.data_ptr(), self.n1 * self.V, self.V)
+        if out.shape != logits.shape or out.dtype != logits.dtype or out.device != self.dev:
+            raise ValueError("out must have the logits' shape, type and device")
+        if out.requires_grad:
+            raise ValueError("out must not require grad: detach it")
+        same = (out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride())
+        if out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr() \
+                and out.numel() and not same:
+            raise ValueError("out shares the logits' storage without being the logits")
+        if not _rows_disjoint(out):
+            raise ValueError("out needs a unit last stride and rows that do not overlap")
+        if same and self.t.data_ptr() != logits.data_ptr():
+            raise ValueError("out: these logits have to be copied, so out cannot be they")
+        torch.autograd.graph.increment_version(out)
         view = out
         if out.dim() > 3:
             view = out.view(-1, out.shape[-2], self.V)
         elif out.dim() == 2:
             view = out[None]
-        return out, view
+        return out, (view.data_ptr(), view.stride(0), view.stride(1))
 
     def workspace(self):
-        n = N.lib().lema_loss_workspace_bytes(self.n0, self.n1)
-        if n < 0:
-            raise ValueError("more than 2^31 - 1 rows of logits")
+        n = _loss_workspace_bytes(self.n0, self.n1)
         return torch.empty(n, dtype=torch.uint8, device=self.dev), n
 
     def call(self, name: str, *args) -> None:
         """One entry point on the logits' device and its current stream."""
-        if torch.cuda.current_device() != self.dev.index:
-            with torch.cuda.device(self.dev):
-                N.call(name, *self.args, *args, _stream(self.dev))
+        index = self.dev.index
+        if torch.cuda.current_device() != index:
+            with torch.cuda.device(index):
+                N.call(name, *self.args, *args, _raw_stream(index))
         else:
-            N.call(name, *self.args, *args, _stream(self.dev))
+            N.call(name, *self.args, *args, _raw_stream(index))
+
+
+_NO_GRAD = (None, 0, 0)
+
+
+@functools.lru_cache(maxsize=256)
+def _loss_workspace_bytes(n0: int, n1: int) -> int:
+    n = N.lib().lema_loss_workspace_bytes(n0, n1)
+    if n < 0:
+        raise ValueError("more than 2^31 - 1 rows of logits")
+    return n
+
+
+# The current stream's handle without a Stream object around it, where torch offers that.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _rows_disjoint(t: torch.Tensor) -> bool:
@@ -944,13 +962,23 @@ def _targets(x: _Logits, targets: torch.Tensor) -> torch.Tensor:
     return x.per_row(targets, "targets", torch.int64)
 
 
-def _logprobs_bwd(x: _Logits, logits, targets, ignore_index, temperature, stats, dlogps,
-                  upstream=None) -> torch.Tensor:
-    dx, view = x.grad_out(logits, None)
+def _logprobs_bwd(logits, targets, ignore_index, temperature, stats, dlogps, upstream=None):
+    x = _Logits(logits)
+    dx, where = x.grad_out(logits, None)
     x.call("lema_token_logprobs_bwd", targets.data_ptr(), ignore_index, temperature,
-           stats.data_ptr(), dlogps.data_ptr(), _ptr(upstream), view.data_ptr(), view.stride(0),
-           view.stride(1))
+           stats.data_ptr(), dlogps.data_ptr(), _ptr(upstream), *where)
     return dx
+
+
+def _first_order(backward):
+    """An autograd backward that has no derivative of its own. Only a graph that is to be
+    differentiated again pays for saying so."""
+    once = torch.autograd.function.once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def run(ctx, *grads):
+        return once(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return run
 
 
 def _logprobs_fwd(logits, targets, temperature, ignore_index, want_stats):
@@ -973,11 +1001,11 @@ class _TokenLogprobsFn(torch.autograd.Function):
         return logps
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dlogps):
         logits, targets, stats = ctx.saved_tensors
         temperature, ignore_index = ctx.meta
-        return _logprobs_bwd(_Logits(logits), logits, targets, ignore_index, temperature, stats,
+        return _logprobs_bwd(logits, targets, ignore_index, temperature, stats,
                              dlogps.contiguous()), None, None, None
 
 
@@ -1001,37 +1029,37 @@ def _preference(logits, targets, ref_logps, beta, label_smoothing, ignore_index,
     targets = _targets(x, targets)
     ref = x.per_row(ref_logps, "ref_logps", torch.float32)
     ws, n = x.workspace()
-    f = torch.empty(2 + 4 * x.n0 * x.n1 + x.n0, dtype=torch.float32, device=x.dev)
     T = x.n0 * x.n1
-    stats, logps, coef = f[:2 * T], f[2 * T:3 * T], f[3 * T:4 * T]
-    rewards, loss = f[4 * T:4 * T + x.n0], f[4 * T + x.n0]
-    dx = view = None
-    if want_dx:
-        dx, view = x.grad_out(logits, out)
+    # statistics (pairs, 8-byte aligned), log-probabilities, coefficients
+    saved = torch.empty(4 * T, dtype=torch.float32, device=x.dev)
+    rewards = torch.empty(x.n0, dtype=torch.float32, device=x.dev)
+    loss = torch.empty((), dtype=torch.float32, device=x.dev)
+    dx, where = x.grad_out(logits, out) if want_dx else (None, _NO_GRAD)
+    at = saved.data_ptr()
     x.call("lema_preference_loss", targets.data_ptr(), int(ignore_index), _ptr(ref), float(beta),
-           float(label_smoothing), float(grad_scale), ws.data_ptr(), n, logps.data_ptr(),
-           stats.data_ptr(), coef.data_ptr(), loss.data_ptr(), rewards.data_ptr(), _ptr(view),
-           view.stride(0) if want_dx else 0, view.stride(1) if want_dx else 0)
+           float(label_smoothing), float(grad_scale), ws.data_ptr(), n, at + 8 * T, at,
+           at + 12 * T, loss.data_ptr(), rewards.data_ptr(), *where)
     if want_dx and T:
         N.kernel_launches += 1  # the gradient rows
-    return x, targets, loss, rewards, stats, coef, dx
+    return targets, loss, rewards, saved, dx
 
 
 class _PreferenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, ref_logps, beta, label_smoothing, ignore_index):
-        _, targets, loss, rewards, stats, coef, _ = _preference(
+        targets, loss, rewards, saved, _ = _preference(
             logits, targets, ref_logps, beta, label_smoothing, ignore_index, 1.0, None, False)
-        ctx.save_for_backward(logits, targets, stats, coef)
+        ctx.save_for_backward(logits, targets, saved)
         ctx.ignore_index = ignore_index
         ctx.mark_non_differentiable(rewards)
         return loss, rewards
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dloss, _drewards):
-        logits, targets, stats, coef = ctx.saved_tensors
-        return (_logprobs_bwd(_Logits(logits), logits, targets, ctx.ignore_index, 1.0, stats, coef,
+        logits, targets, saved = ctx.saved_tensors
+        return (_logprobs_bwd(logits, targets, ctx.ignore_index, 1.0, saved,
+                              saved[3 * targets.numel():],
                               dloss.float()), None, None, None, None, None)
 
 
@@ -1049,9 +1077,8 @@ def preference_loss(logits: torch.Tensor, targets: torch.Tensor,
     (no gradient). Differentiable in the logits."""
     if logits.requires_grad and torch.is_grad_enabled():
         return _PreferenceFn.apply(logits, targets, ref_logps, beta, label_smoothing, ignore_index)
-    _, _, loss, rewards, *_ = _preference(logits, targets, ref_logps, beta, label_smoothing,
-                                          ignore_index, 1.0, None, False)
-    return loss, rewards
+    return _preference(logits, targets, ref_logps, beta, label_smoothing, ignore_index, 1.0, None,
+                       False)[1:3]
 
 
 def preference_loss_grad(logits: torch.Tensor, targets: torch.Tensor,
@@ -1061,8 +1088,8 @@ def preference_loss_grad(logits: torch.Tensor, targets: torch.Tensor,
     """``preference_loss`` and its gradient in one call: (loss, rewards, dlogits).
     dlogits = grad_scale * dloss/dlogits, written into ``out`` when given (which
     may be ``logits`` itself)."""
-    _, _, loss, rewards, _, _, dx = _preference(logits, targets, ref_logps, beta, label_smoothing,
-                                                ignore_index, grad_scale, out, True)
+    _, loss, rewards, _, dx = _preference(logits, targets, ref_logps, beta, label_smoothing,
+                                          ignore_index, grad_scale, out, True)
     return loss, rewards, dx
 
 
@@ -1087,41 +1114,41 @@ def _policy(logits, targets, old_logps, advantages, ref_logps, clip, kl_coef, te
     else:
         raise ValueError(f"advantages must have shape {tuple(x.lead)}, or one per sequence")
     ws, n = x.workspace()
-    T = x.n0 * x.n1
     logps = torch.empty(x.lead, dtype=torch.float32, device=x.dev)
-    f = torch.empty(2 + (3 * T if want_saved else 0), dtype=torch.float32, device=x.dev)
-    loss, kl = f[0], f[1]
-    stats, coef = (f[2:2 + 2 * T], f[2 + 2 * T:]) if want_saved else (None, None)
-    dx = view = None
-    if want_dx:
-        dx, view = x.grad_out(logits, out)
+    loss = torch.empty((), dtype=torch.float32, device=x.dev)
+    kl = torch.empty((), dtype=torch.float32, device=x.dev)
+    # statistics (pairs, 8-byte aligned), coefficients
+    T = x.n0 * x.n1
+    saved = torch.empty(3 * T, dtype=torch.float32, device=x.dev) if want_saved else None
+    at = saved.data_ptr() if want_saved else None
+    dx, where = x.grad_out(logits, out) if want_dx else (None, _NO_GRAD)
     x.call("lema_policy_loss", targets.data_ptr(), int(ignore_index), float(temperature),
            _ptr(old), adv.data_ptr(), s0, s1, _ptr(ref), float(clip_lo), float(clip_hi),
            float(kl_coef), int(reduction == "sequence"), float(grad_scale), ws.data_ptr(), n,
-           logps.data_ptr(), _ptr(stats), _ptr(coef), loss.data_ptr(), kl.data_ptr(), _ptr(view),
-           view.stride(0) if want_dx else 0, view.stride(1) if want_dx else 0)
-    return targets, loss, logps, kl, stats, coef, dx
+           logps.data_ptr(), at, at + 8 * T if want_saved else None, loss.data_ptr(),
+           kl.data_ptr(), *where)
+    return targets, loss, logps, kl, saved, dx
 
 
 class _PolicyFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, targets, old_logps, advantages, ref_logps, clip, kl_coef, temperature,
                 reduction, ignore_index):
-        targets, loss, logps, kl, stats, coef, _ = _policy(
+        targets, loss, logps, kl, saved, _ = _policy(
             logits, targets, old_logps, advantages, ref_logps, clip, kl_coef, temperature,
             reduction, ignore_index, 1.0, None, False, True)
-        ctx.save_for_backward(logits, targets, stats, coef)
+        ctx.save_for_backward(logits, targets, saved)
         ctx.meta = (ignore_index, float(temperature))
         ctx.mark_non_differentiable(logps, kl)
         return loss, logps, kl
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dloss, _dlogps, _dkl):
-        logits, targets, stats, coef = ctx.saved_tensors
+        logits, targets, saved = ctx.saved_tensors
         ignore_index, temperature = ctx.meta
-        dx = _logprobs_bwd(_Logits(logits), logits, targets, ignore_index, temperature, stats,
-                           coef, dloss.float())
+        dx = _logprobs_bwd(logits, targets, ignore_index, temperature, saved,
+                           saved[2 * targets.numel():], dloss.float())
         return (dx,) + (None,) * 9
 
 
@@ -1143,10 +1170,8 @@ def policy_loss(logits: torch.Tensor, targets: torch.Tensor, old_logps: torch.Te
     if logits.requires_grad and torch.is_grad_enabled():
         return _PolicyFn.apply(logits, targets, old_logps, advantages, ref_logps, clip, kl_coef,
                                temperature, reduction, ignore_index)
-    _, loss, logps, kl, *_ = _policy(logits, targets, old_logps, advantages, ref_logps, clip,
-                                     kl_coef, temperature, reduction, ignore_index, 1.0, None,
-                                     False, False)
-    return loss, logps, kl
+    return _policy(logits, targets, old_logps, advantages, ref_logps, clip, kl_coef, temperature,
+                   reduction, ignore_index, 1.0, None, False, False)[1:4]
 
 
 def policy_loss_grad(logits: torch.Tensor, targets: torch.Tensor, old_logps: torch.Tensor | None,
@@ -1158,9 +1183,9 @@ def policy_loss_grad(logits: torch.Tensor, targets: torch.Tensor, old_logps: tor
     """``policy_loss`` and its gradient in one pass over the logits: (loss, logps,
     kl, dlogits). dlogits = grad_scale * dloss/dlogits, written into ``out`` when
     given (which may be ``logits`` itself)."""
-    _, loss, logps, kl, _, _, dx = _policy(logits, targets, old_logps, advantages, ref_logps, clip,
-                                           kl_coef, temperature, reduction, ignore_index,
-                                           grad_scale, out, True, False)
+    _, loss, logps, kl, _, dx = _policy(logits, targets, old_logps, advantages, ref_logps, clip,
+                                        kl_coef, temperature, reduction, ignore_index,
+                                        grad_scale, out, True, False)
     return loss, logps, kl, dx
 
 
@@ -1179,18 +1204,14 @@ def _teacher(x: _Logits, ids: torch.Tensor, logits: torch.Tensor, mask):
     return ids.contiguous(), logits.contiguous(), mask
 
 
-def _distill(logits, ids, tl, mask, temperature, grad_scale, upstream, out, want_dx):
+def _distill(x, logits, ids, tl, mask, temperature, grad_scale, upstream, out, want_dx):
     """One call on checked teacher tensors: (loss, dlogits or None)."""
-    x = _Logits(logits)
     ws, n = x.workspace()
     loss = torch.empty((), dtype=torch.float32, device=x.dev)
-    dx = view = None
-    if want_dx:
-        dx, view = x.grad_out(logits, out)
-    x.call("lema_distill_loss", ids.data_ptr(), int(ids.dtype == torch.int32), tl.data_ptr(),
-           int(tl.dtype == torch.float32), ids.shape[-1], _ptr(mask), float(temperature),
-           float(grad_scale), _ptr(upstream), ws.data_ptr(), n, loss.data_ptr(), _ptr(view),
-           view.stride(0) if want_dx else 0, view.stride(1) if want_dx else 0)
+    dx, where = x.grad_out(logits, out) if want_dx else (None, _NO_GRAD)
+    x.call("lema_distill_loss", ids.data_ptr(), int(ids.dtype is torch.int32), tl.data_ptr(),
+           int(tl.dtype is torch.float32), ids.shape[-1], _ptr(mask), float(temperature),
+           float(grad_scale), _ptr(upstream), ws.data_ptr(), n, loss.data_ptr(), *where)
     return loss, dx
 
 
@@ -1202,13 +1223,15 @@ class _DistillFn(torch.autograd.Function):
     def forward(ctx, logits, ids, tl, mask, temperature):
         ctx.save_for_backward(logits, ids, tl, mask)
         ctx.temperature = temperature
-        return _distill(logits, ids, tl, mask, temperature, 1.0, None, None, False)[0]
+        return _distill(_Logits(logits), logits, ids, tl, mask, temperature, 1.0, None, None,
+                        False)[0]
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_first_order
     def backward(ctx, dloss):
         logits, ids, tl, mask = ctx.saved_tensors
-        dx = _distill(logits, ids, tl, mask, ctx.temperature, 1.0, dloss.float(), None, True)[1]
+        dx = _distill(_Logits(logits), logits, ids, tl, mask, ctx.temperature, 1.0, dloss.float(),
+                      None, True)[1]
         return dx, None, None, None, None
 
 
@@ -1221,10 +1244,11 @@ def distill_loss(logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits
     int64; teacher_logits [..., K] bf16 or fp32 (-inf: no entry, whatever its
     index; an index that repeats adds its weights); mask [...] bool, False rows
     are not read. Differentiable in the logits."""
-    ids, tl, mask = _teacher(_Logits(logits), teacher_ids, teacher_logits, mask)
+    x = _Logits(logits)
+    ids, tl, mask = _teacher(x, teacher_ids, teacher_logits, mask)
     if logits.requires_grad and torch.is_grad_enabled():
         return _DistillFn.apply(logits, ids, tl, mask, temperature)
-    return _distill(logits, ids, tl, mask, temperature, 1.0, None, None, False)[0]
+    return _distill(x, logits, ids, tl, mask, temperature, 1.0, None, None, False)[0]
 
 
 def distill_loss_grad(logits: torch.Tensor, teacher_ids: torch.Tensor,
@@ -1234,5 +1258,6 @@ def distill_loss_grad(logits: torch.Tensor, teacher_ids: torch.Tensor,
     """``distill_loss`` and its gradient in one pass over the logits: (loss, dlogits).
     dlogits = grad_scale * dloss/dlogits, written into ``out`` when given (which may
     be ``logits`` itself)."""
-    ids, tl, mask = _teacher(_Logits(logits), teacher_ids, teacher_logits, mask)
-    return _distill(logits, ids, tl, mask, temperature, grad_scale, None, out, True)
+    x = _Logits(logits)
+    ids, tl, mask = _teacher(x, teacher_ids, teacher_logits, mask)
+    return _distill(x, logits, ids, tl, mask, temperature, grad_scale, None, out, True)
