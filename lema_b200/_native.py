@@ -161,7 +161,7 @@ KERNELS_PER_CALL = {
     "lema_rope": 1, "lema_rope_qkv": 1, "lema_swiglu_quant": 1, "lema_swiglu_bwd": 1,
     "lema_adamw_requant_rows": 1, "lema_device_error_async": 1, "lema_attn_fwd": 1,
     "lema_attn_bwd": 3, "lema_token_logprobs": 1, "lema_token_logprobs_bwd": 1,
-    "lema_preference_loss": 3, "lema_policy_loss": 3, "lema_distill_loss": 3,
+    "lema_preference_loss": 2, "lema_policy_loss": 3, "lema_distill_loss": 3,
 }
 # Running count of this library's kernel launches issued by this process.
 kernel_launches = 0

@@ -46,8 +46,8 @@ struct RowMap {
 // Workspace: head, counted rows of each sequence, the list of rows, partial sums of
 // token_kernel's CTAs, what each row leaves for it.
 struct WsHead {
-  unsigned long long total, out;  // rows that count, and that do not
-  uint32_t ticket;                // CTAs of token_kernel that are done
+  int64_t total;    // rows that count
+  uint32_t ticket;  // CTAs of token_kernel or pair_kernel that are done
 };
 constexpr int64_t kWsHead = 256;
 constexpr int kTokenThreads = 256;
@@ -66,7 +66,7 @@ struct RowArgs {
   int64_t T;
   int32_t V;
   double inv_tau, c_full;        // 1 / tau, log2(e) / tau
-  float c, c_lo;                 // log2(e) / tau, rounded down, and what the rounding left
+  float c, c_lo;                 // log2(e) / tau, rounded, and what the rounding left
   const int64_t* targets;        // [T]; null for distill
   int64_t ignore;
   float* logps;                  // [T]
@@ -529,93 +529,126 @@ __device__ __forceinline__ F policy_token(const RowArgs& a, const Token& tk, F l
 
 // ---- kernels ---------------------------------------------------------------------
 
-// Lists the rows that enter the loss (list[0 .. total)), then the others from the end
-// backwards, and counts them for each sequence. One CTA, which clears the counters itself, or
-// several over counters cleared before; the order of the list, which the atomics then leave
-// open, moves no result. A thread takes kCountRows rows at once: two barriers for 8192 rows.
+// Lists the rows that enter the loss in their order (list[0 .. total)), then the others from the
+// end backwards, counts them for each sequence, and clears the ticket. A CTA lists kCountBlock
+// rows, after it has counted those in front of them by itself: the list's order, and with it
+// the order of every sum, is always the same. (seq_count is cleared before when there are
+// several CTAs.)
 constexpr int kCountThreads = 1024;
 constexpr int kCountRows = 8;
 constexpr int kCountBlock = kCountThreads * kCountRows;
 __global__ void __launch_bounds__(kCountThreads) count_kernel(RowArgs a) {
   constexpr int kCells = kCountRows * kCountThreads / 32;  // a warp's rows at one offset
   __shared__ int32_t s_cell[kCells];
-  __shared__ int64_t s_base, s_base_out;
+  __shared__ int32_t s_before;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (gridDim.x == 1) {
-    if (a.per_sequence)
-      for (int64_t b = tid; b < a.n0; b += kCountThreads) a.seq_count[b] = 0;
-    if (tid == 0) {
-      a.head->ticket = 0;
-      a.head->total = 0;
-      a.head->out = 0;
-    }
-    __syncthreads();
+  const int64_t r0 = blockIdx.x * int64_t{kCountBlock};
+  bool in[kCountRows];
+#pragma unroll
+  for (int j = 0; j < kCountRows; ++j) {
+    const int64_t r = r0 + j * kCountThreads + tid;
+    int64_t target;
+    in[j] = r < a.T && row_counts(a, r, target);
   }
-  for (int64_t r0 = blockIdx.x * int64_t{kCountBlock}; r0 < a.T;
-       r0 += gridDim.x * int64_t{kCountBlock}) {
-    bool in[kCountRows];
-#pragma unroll
-    for (int j = 0; j < kCountRows; ++j) {
-      const int64_t r = r0 + j * kCountThreads + tid;
-      int64_t target;
-      in[j] = r < a.T && row_counts(a, r, target);
-    }
-    uint32_t ballot[kCountRows];
-#pragma unroll
-    for (int j = 0; j < kCountRows; ++j) {
-      ballot[j] = __ballot_sync(0xffffffffu, in[j]);
-      if (lane == 0) s_cell[j * 32 + warp] = __popc(ballot[j]);
-      if (a.per_sequence) {
-        const int64_t r = r0 + j * kCountThreads + tid, b = r / a.in.n1;
-        // a warp inside one sequence adds once
-        const bool one = (r - lane) / a.in.n1 == (r - lane + 31) / a.in.n1;
-        if (one ? lane == 0 && ballot[j] != 0 : in[j])
-          atomicAdd(&a.seq_count[b], one ? __popc(ballot[j]) : 1);
-      }
-    }
-    __syncthreads();
-    if (warp == 0) {
-      int n[kCells / 32], sum = 0;
-#pragma unroll
-      for (int j = 0; j < kCells / 32; ++j) {
-        n[j] = s_cell[lane * (kCells / 32) + j];
-        sum += n[j];
-      }
-      int incl = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += up;
-      }
-      int at = incl - sum;
-#pragma unroll
-      for (int j = 0; j < kCells / 32; ++j) {
-        s_cell[lane * (kCells / 32) + j] = at;
-        at += n[j];
-      }
-      if (lane == 31) {
-        const int64_t rows = a.T - r0 < kCountBlock ? a.T - r0 : kCountBlock;
-        s_base = static_cast<int64_t>(
-            atomicAdd(&a.head->total, static_cast<unsigned long long>(incl)));
-        s_base_out = static_cast<int64_t>(
-            atomicAdd(&a.head->out, static_cast<unsigned long long>(rows - incl)));
-      }
-    }
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kCountRows; ++j) {
-      const int place = j * kCountThreads + tid;
-      const int64_t r = r0 + place;
-      // counted rows of this block in front of r
-      const int rank = s_cell[j * 32 + warp] + __popc(ballot[j] & ((1u << lane) - 1u));
-      if (in[j])
-        a.list[s_base + rank] = static_cast<int32_t>(r);
-      else if (r < a.T)
-        a.list[a.T - 1 - (s_base_out + place - rank)] = static_cast<int32_t>(r);
-    }
-    __syncthreads();
+  if (tid == 0) {
+    s_before = 0;
+    if (blockIdx.x == 0) a.head->ticket = 0;
   }
+  if (a.per_sequence && gridDim.x == 1)
+    for (int64_t b = tid; b < a.n0; b += kCountThreads) a.seq_count[b] = 0;
+  __syncthreads();
+  if (r0 > 0) {
+    int n = 0;
+    for (int64_t q0 = 0; q0 < r0; q0 += kCountBlock) {
+      bool was[kCountRows];
+#pragma unroll
+      for (int j = 0; j < kCountRows; ++j) {
+        int64_t target;
+        was[j] = row_counts(a, q0 + j * kCountThreads + tid, target);
+      }
+#pragma unroll
+      for (int j = 0; j < kCountRows; ++j) n += was[j];
+    }
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane == 0) atomicAdd(&s_before, n);
+  }
+  uint32_t ballot[kCountRows];
+#pragma unroll
+  for (int j = 0; j < kCountRows; ++j) {
+    ballot[j] = __ballot_sync(0xffffffffu, in[j]);
+    if (lane == 0) s_cell[j * 32 + warp] = __popc(ballot[j]);
+    if (a.per_sequence) {
+      const int64_t r = r0 + j * kCountThreads + tid, b = r / a.in.n1;
+      // a warp inside one sequence adds once
+      const bool one = (r - lane) / a.in.n1 == (r - lane + 31) / a.in.n1;
+      if (one ? lane == 0 && ballot[j] != 0 : in[j])
+        atomicAdd(&a.seq_count[b], one ? __popc(ballot[j]) : 1);
+    }
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int n[kCells / 32], sum = 0;
+#pragma unroll
+    for (int j = 0; j < kCells / 32; ++j) {
+      n[j] = s_cell[lane * (kCells / 32) + j];
+      sum += n[j];
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    int at = s_before + incl - sum;
+#pragma unroll
+    for (int j = 0; j < kCells / 32; ++j) {
+      s_cell[lane * (kCells / 32) + j] = at;
+      at += n[j];
+    }
+    if (lane == 31 && blockIdx.x == gridDim.x - 1) a.head->total = at;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kCountRows; ++j) {
+    const int64_t r = r0 + j * kCountThreads + tid;
+    // counted rows in front of r
+    const int64_t rank = s_cell[j * 32 + warp] + __popc(ballot[j] & ((1u << lane) - 1u));
+    if (in[j])
+      a.list[rank] = static_cast<int32_t>(r);
+    else if (r < a.T)
+      a.list[a.T - 1 - (r - rank)] = static_cast<int32_t>(r);
+  }
+}
+
+// What a row that does not count leaves in the policy loss's outputs.
+__device__ __forceinline__ void zero_outputs(const RowArgs& a, int64_t r) {
+  if (a.logps) a.logps[r] = 0.f;
+  if (a.coef) a.coef[r] = 0.f;
+  if (a.stats) a.stats[r] = make_float2(0.f, 0.f);
+}
+
+// One token's terms in fp64, from what its row left: its share of the loss and of the KL, its
+// log-probability, and what the backward needs.
+template <int OBJ>
+__device__ __forceinline__ double2 token_terms(const RowArgs& a, int64_t r) {
+  const RowStat st = a.row[r];
+  const double log_s = log(static_cast<double>(st.s));
+  if (OBJ == kDistill) {
+    // sum_k p_k (log p_k - log q_k), p_k = p'_k / t
+    const double t = st.x;
+    if (t == 0.0) return make_double2(0.0, 0.0);
+    return make_double2((st.a / t * a.inv_tau - log(t) + log_s) /
+                            (static_cast<double>(a.head->total) * a.inv_tau * a.inv_tau),
+                        0.0);
+  }
+  const double w = token_weight(a, r), lp = (static_cast<double>(st.x) - st.m) * a.inv_tau - log_s;
+  double loss, kl;
+  const double coef = policy_token<double, true>(a, load_token(a, r), lp, &loss, &kl);
+  a.logps[r] = static_cast<float>(lp);
+  if (a.coef) a.coef[r] = static_cast<float>(w * coef);
+  if (a.stats) a.stats[r] = make_float2(st.m, 1.f / st.s);
+  return make_double2(w * loss, w * kl);
 }
 
 // A gradient row of zeros.
@@ -639,6 +672,7 @@ __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
   const int tid = threadIdx.x % G;
   const int64_t r = blockIdx.x * int64_t{kStatThreads / G} + threadIdx.x / G;
   if (r >= a.T) return;
+  if (r == 0 && tid == 0 && a.head) a.head->ticket = 0;  // pair_kernel's
   int64_t target;
   if (!row_counts(a, r, target)) {
     if (tid == 0) {
@@ -1030,6 +1064,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
   __shared__ RowInfo info[kMaxStages + 1];
   __shared__ Share share[2][kMaxCluster];
   __shared__ float red_m[8], red_s[8];
+  __shared__ double2 red_t[8];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = cs > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
   const int start = rank * per;  // this CTA's first vector of a row; rank 0 has the edges too
@@ -1059,7 +1094,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
     // The rows of zeros, dealt to every CTA, are written between the others by bulk copies from
     // shared memory: HBM takes writes alone at 3.9 TB/s, reads and writes together at 6.5.
     const int64_t rest = a.T - total;
-    const int n_zero = a.dx != nullptr && rest > blockIdx.x
+    const int n_zero = rest > blockIdx.x
                            ? static_cast<int>((rest - blockIdx.x + gridDim.x - 1) / gridDim.x)
                            : 0;
     const int n_row = total > first ? static_cast<int>((total - first + step - 1) / step) : 0;
@@ -1069,7 +1104,9 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
     const auto zero_rows = [&](int until) {
       for (; z < until; ++z) {
         T* dx = static_cast<T*>(a.dx) + a.out.at(z_row);
+        if (OBJ == kPolicy && lane == 0) zero_outputs(a, z_row);
         if (z + 1 < n_zero) z_row = z_list[(z + 1) * static_cast<int64_t>(gridDim.x)];
+        if (a.dx == nullptr) continue;
         const Span<T> so(dx, a.V);
         if (lane < kEdges && so.edge(lane) >= 0) put(dx + so.edge(lane), 0.f);
         char* to = reinterpret_cast<char*>(dx + so.head);
@@ -1350,6 +1387,26 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
       }
       slot = slot == stages ? 0 : slot + 1;
     }
+    // the terms of this CTA's tokens: thread 0 wrote what their rows left
+    ring_sync();
+    double2 terms = make_double2(0.0, 0.0);
+    if (rank == 0 && ok)
+      for (int64_t job = first + tid * step; job < total; job += kRingThreads * step) {
+        const double2 v = token_terms<OBJ>(a, a.list[job]);
+        terms.x += v.x;
+        terms.y += v.y;
+      }
+    terms.x = warp_sum(terms.x);
+    terms.y = warp_sum(terms.y);
+    if (lane == 0) red_t[warp] = terms;
+    ring_sync();
+    if (tid == 0) {
+      for (int j = 1; j < kRingWarps; ++j) {
+        terms.x += red_t[j].x;
+        terms.y += red_t[j].y;
+      }
+      a.part[blockIdx.x] = terms;
+    }
   }
   if (cs > 1) ptx::cluster_sync();  // no CTA leaves while another may still write to it
 }
@@ -1448,105 +1505,115 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
   }
 }
 
-// The tokens' terms in fp64, from what the rows left; the CTAs' sums are added in order by the
-// CTA that ends last.
+// Both sums over a CTA of 32 N threads, in its thread 0.
+template <int N>
+__device__ __forceinline__ double2 cta_sum(double2 v, double2* red) {
+  v.x = warp_sum(v.x);
+  v.y = warp_sum(v.y);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    for (int w = 1; w < N; ++w) {
+      v.x += red[w].x;
+      v.y += red[w].y;
+    }
+  return v;
+}
+
+// Whether this CTA is the last of the grid to have written its partial sum.
+__device__ __forceinline__ bool last_to_write(const RowArgs& a, double2 v, bool* s_last) {
+  if (threadIdx.x == 0) {
+    a.part[blockIdx.x] = v;
+    __threadfence();
+    *s_last = atomicAdd(&a.head->ticket, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (*s_last) __threadfence();
+  return *s_last;
+}
+
+// The partial sums added in their order: loss and KL.
+template <int N>
+__device__ __forceinline__ void sum_parts(const RowArgs& a, int n, double2* red) {
+  double2 v = make_double2(0.0, 0.0);
+  for (int i = threadIdx.x; i < n; i += 32 * N) {
+    const double2 p = __ldcg(&a.part[i]);
+    v.x += p.x;
+    v.y += p.y;
+  }
+  v = cta_sum<N>(v, red);
+  if (threadIdx.x == 0) {
+    *a.loss = static_cast<float>(v.x);
+    if (a.kl) *a.kl = static_cast<float>(v.y);
+  }
+}
+
+// The tokens' terms after direct_kernel or stream_kernel; the CTA that ends last adds up.
 template <int OBJ>
 __global__ void __launch_bounds__(kTokenThreads) token_kernel(RowArgs a) {
-  __shared__ double red[kTokenThreads / 32];
+  __shared__ double2 red[kTokenThreads / 32], red2[kTokenThreads / 32];
   __shared__ bool s_last;
   ptx::griddep_wait();
   const int64_t r = blockIdx.x * static_cast<int64_t>(kTokenThreads) + threadIdx.x;
-  double loss = 0.0, kl = 0.0;
+  double2 v = make_double2(0.0, 0.0);
   int64_t target;
-  if (r < a.T && row_counts(a, r, target)) {
-    const RowStat st = a.row[r];
-    const double w = token_weight(a, r);
-    const double log_s = log(static_cast<double>(st.s));
-    if (OBJ == kDistill) {
-      // sum_k p_k (log p_k - log q_k), p_k = p'_k / t
-      const double t = st.x;
-      if (t != 0.0)
-        loss = w / (a.inv_tau * a.inv_tau) * (st.a / t * a.inv_tau - log(t) + log_s);
-    } else {
-      const double lp = (static_cast<double>(st.x) - st.m) * a.inv_tau - log_s;
-      a.logps[r] = static_cast<float>(lp);
-      const double coef = policy_token<double, true>(a, load_token(a, r), lp, &loss, &kl);
-      if (a.coef) a.coef[r] = static_cast<float>(w * coef);
-      if (a.stats) a.stats[r] = make_float2(st.m, 1.f / st.s);
-      loss *= w;
-      kl *= w;
-    }
-  } else if (OBJ == kPolicy && r < a.T) {
-    a.logps[r] = 0.f;
-    if (a.coef) a.coef[r] = 0.f;
-    if (a.stats) a.stats[r] = make_float2(0.f, 0.f);
+  if (r < a.T) {
+    if (row_counts(a, r, target))
+      v = token_terms<OBJ>(a, r);
+    else if (OBJ == kPolicy)
+      zero_outputs(a, r);
   }
-  loss = block_sum_d(loss, red);
-  kl = block_sum_d(kl, red);
-  if (threadIdx.x == 0) {
-    a.part[blockIdx.x] = make_double2(loss, kl);
-    __threadfence();
-    s_last = atomicAdd(&a.head->ticket, 1u) == gridDim.x - 1;
-  }
-  __syncthreads();
-  if (!s_last) return;
-  __threadfence();
-  loss = kl = 0.0;
-  for (unsigned i = threadIdx.x; i < gridDim.x; i += kTokenThreads) {
-    const double2 p = __ldcg(&a.part[i]);
-    loss += p.x;
-    kl += p.y;
-  }
-  loss = block_sum_d(loss, red);
-  kl = block_sum_d(kl, red);
-  if (threadIdx.x == 0) {
-    *a.loss = static_cast<float>(loss);
-    if (a.kl) *a.kl = static_cast<float>(kl);
-  }
+  v = cta_sum<kTokenThreads / 32>(v, red);
+  if (last_to_write(a, v, &s_last)) sum_parts<kTokenThreads / 32>(a, gridDim.x, red2);
+}
+
+// The sums that the CTAs of ring_kernel left.
+__global__ void __launch_bounds__(256) finish_kernel(RowArgs a, int n) {
+  __shared__ double2 red[8];
+  ptx::griddep_wait();
+  sum_parts<8>(a, n, red);
 }
 
 // One CTA per pair: the two sequences' summed log ratios, the pair's loss and dL/dlp of its
-// tokens.
-__global__ void __launch_bounds__(256) pair_kernel(RowArgs a, int64_t P, double beta,
-                                                   double smooth, float* rewards) {
-  __shared__ double red[8];
+// tokens; the CTA that ends last adds the losses up.
+constexpr int kPairThreads = 512;
+__global__ void __launch_bounds__(kPairThreads) pair_kernel(RowArgs a, int64_t P, double beta,
+                                                            double smooth, float* rewards) {
+  constexpr int kW = kPairThreads / 32;
+  __shared__ double2 red[kW], red2[kW];
+  __shared__ float s_dh;
+  __shared__ bool s_last;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  ptx::griddep_wait();
   const int64_t p = blockIdx.x, S = a.T / (2 * P);
-  double R[2];
-  for (int side = 0; side < 2; ++side) {
-    const int64_t b = p + side * P;
-    double sum = 0.0;
-    for (int64_t t = threadIdx.x; t < S; t += blockDim.x) {
-      const int64_t r = b * S + t;
-      if (a.targets[r] == a.ignore) continue;
-      sum += a.lp64[r] - (a.ref_logps ? static_cast<double>(a.ref_logps[r]) : 0.0);
-    }
-    R[side] = beta * block_sum_d(sum, red);
+  double2 sum = make_double2(0.0, 0.0);
+  for (int64_t i = threadIdx.x; i < 2 * S; i += kPairThreads) {
+    const bool side = i >= S;
+    const int64_t r = side ? (p + P) * S + i - S : p * S + i;
+    if (a.targets[r] == a.ignore) continue;
+    const double d = a.lp64[r] - (a.ref_logps ? static_cast<double>(a.ref_logps[r]) : 0.0);
+    sum.x += side ? 0.0 : d;
+    sum.y += side ? d : 0.0;
   }
-  const double h = R[0] - R[1];
-  // sigma(-h) = 1 / (1 + e^h)
-  const double dh = (smooth / (1.0 + exp(-h)) - (1.0 - smooth) / (1.0 + exp(h))) * beta /
-                    static_cast<double>(P);
+  sum = cta_sum<kW>(sum, red);
+  double2 loss = make_double2(0.0, 0.0);
   if (threadIdx.x == 0) {
-    rewards[p] = static_cast<float>(R[0]);
-    rewards[p + P] = static_cast<float>(R[1]);
-    a.part[p] = make_double2(
-        ((1.0 - smooth) * softplus(-h) + smooth * softplus(h)) / static_cast<double>(P), 0.0);
+    const double won = beta * sum.x, lost = beta * sum.y, h = won - lost;
+    rewards[p] = static_cast<float>(won);
+    rewards[p + P] = static_cast<float>(lost);
+    loss.x = ((1.0 - smooth) * softplus(-h) + smooth * softplus(h)) / static_cast<double>(P);
+    // sigma(-h) = 1 / (1 + e^h)
+    s_dh = static_cast<float>((smooth / (1.0 + exp(-h)) - (1.0 - smooth) / (1.0 + exp(h))) * beta /
+                              static_cast<double>(P));
   }
-  for (int side = 0; side < 2; ++side)
-    for (int64_t t = threadIdx.x; t < S; t += blockDim.x) {
-      const int64_t r = (p + side * P) * S + t;
-      a.coef[r] = a.targets[r] == a.ignore ? 0.f : static_cast<float>(side ? -dh : dh);
-    }
-}
-
-// The pairs' losses added in a fixed order.
-__global__ void __launch_bounds__(256) pair_sum_kernel(const double2* part, int64_t n,
-                                                       float* loss) {
-  __shared__ double red[8];
-  double l = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += blockDim.x) l += part[i].x;
-  l = block_sum_d(l, red);
-  if (threadIdx.x == 0) *loss = static_cast<float>(l);
+  __syncthreads();
+  const float dh = s_dh;
+  for (int64_t i = threadIdx.x; i < 2 * S; i += kPairThreads) {
+    const bool side = i >= S;
+    const int64_t r = side ? (p + P) * S + i - S : p * S + i;
+    a.coef[r] = a.targets[r] == a.ignore ? 0.f : (side ? -dh : dh);
+  }
+  if (last_to_write(a, loss, &s_last)) sum_parts<kW>(a, gridDim.x, red2);
 }
 
 // Gradient rows from saved statistics: k (1[v = target] - q_v). A group of G threads takes
@@ -1565,9 +1632,19 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
   const T* x = static_cast<const T*>(a.x) + a.in.at(r);
   T* dx = static_cast<T*>(a.dx) + a.out.at(r);
   const int64_t target = a.targets[r];
-  if (a.zeros_done && target == a.ignore) return;
-  const float k =
-      target == a.ignore ? 0.f : a.g[r] * grad_factor(a) * static_cast<float>(a.inv_tau);
+  const bool counts = target != a.ignore;
+  if (a.zeros_done && !counts) return;
+  const Span<T> sp(x, a.V);
+  const uint4* xv = sp.vecs(x);
+  uint4 w[kBwdU];
+  if (counts) {
+    // the input is nobody's output: it is on its way before pair_kernel has ended
+#pragma unroll
+    for (int u = 0; u < kBwdU; ++u)
+      if (v0 + u * G < sp.nvec) w[u] = ld16(xv + v0 + u * G);
+  }
+  ptx::griddep_wait();
+  const float k = counts ? a.g[r] * grad_factor(a) * static_cast<float>(a.inv_tau) : 0.f;
   if (k == 0.f) {
     // zeros need no input: whole vectors of the output's own phase
     const Span<T> so(dx, a.V);
@@ -1578,12 +1655,6 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
     if (chunk == 0 && tid < kEdges && so.edge(tid) >= 0) put(dx + so.edge(tid), 0.f);
     return;
   }
-  const Span<T> sp(x, a.V);
-  const uint4* xv = sp.vecs(x);
-  uint4 w[kBwdU];
-#pragma unroll
-  for (int u = 0; u < kBwdU; ++u)
-    if (v0 + u * G < sp.nvec) w[u] = ld16(xv + v0 + u * G);
   const float2 st = a.stats[r];
   const bool far = far_max(st.x, a.c);
   const ExpScale ks(far ? 0.f : st.x, a.c);
@@ -1647,8 +1718,7 @@ int make_rows(RowArgs& a, const void* x, int64_t n0, int64_t n1, int64_t ld0, in
   const double c = 1.4426950408889634 / temperature;
   a.c_full = c;
   a.c = static_cast<float>(c);
-  if (static_cast<double>(a.c) >= c) a.c = std::nextafterf(a.c, 0.f);
-  a.c_lo = static_cast<float>(c - static_cast<double>(a.c));  // > 0
+  a.c_lo = static_cast<float>(c - static_cast<double>(a.c));
   a.grad_scale = 1.f;
   return LEMA_OK;
 }
@@ -1671,8 +1741,10 @@ int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
 
 int64_t token_ctas(int64_t T) { return (T + kTokenThreads - 1) / kTokenThreads; }
 
-// Partial sums: one for each CTA of token_kernel, or for each pair.
-int64_t parts(int64_t n0, int64_t T) { return std::max(token_ctas(T), n0) + 1; }
+constexpr int64_t kMaxRing = 512;  // CTAs of ring_kernel, at most
+
+// Partial sums: one for each CTA of token_kernel or ring_kernel, or for each pair.
+int64_t parts(int64_t n0, int64_t T) { return std::max<int64_t>({token_ctas(T), n0, kMaxRing}); }
 
 int64_t ws_bytes_for(int64_t n0, int64_t T) {
   return kWsHead + round256(n0 * 4) + round256(T * 4) + round256(parts(n0, T) * 16) +
@@ -1748,24 +1820,23 @@ int launch_logprobs(const RowArgs& a, int x_f32, cudaStream_t s) {
 }
 
 template <typename T>
-int launch_logprobs_bwd_t(const RowArgs& a, int nvec, cudaStream_t s) {
+int launch_logprobs_bwd_t(const RowArgs& a, int nvec, bool after, cudaStream_t s) {
   const int g = warp_rows(nvec) ? 32 : kBwdThreads;
   const int chunks = std::max(1, (nvec + g * kBwdU - 1) / (g * kBwdU));
   const int64_t per = kBwdThreads / g, grid = (a.T * chunks + per - 1) / per;
   if (grid > INT32_MAX) return set_error(LEMA_ERR_UNSUPPORTED, "too many rows");
-  if (g == 32)
-    logprobs_bwd_kernel<T, 32><<<static_cast<unsigned>(grid), kBwdThreads, 0, s>>>(a, chunks);
-  else
-    logprobs_bwd_kernel<T, kBwdThreads>
-        <<<static_cast<unsigned>(grid), kBwdThreads, 0, s>>>(a, chunks);
+  const auto kern = g == 32 ? logprobs_bwd_kernel<T, 32> : logprobs_bwd_kernel<T, kBwdThreads>;
+  if (after) return launch_after(kern, grid, kBwdThreads, 0, 1, s, a, chunks);
+  kern<<<static_cast<unsigned>(grid), kBwdThreads, 0, s>>>(a, chunks);
   LEMA_CUDA_TRY(cudaGetLastError());
   return LEMA_OK;
 }
 
-int launch_logprobs_bwd(const RowArgs& a, int x_f32, cudaStream_t s) {
+// `after`: directly behind pair_kernel of the same call, which it may overlap.
+int launch_logprobs_bwd(const RowArgs& a, int x_f32, bool after, cudaStream_t s) {
   const int nvec = max_vecs(a, x_f32);
-  return x_f32 ? launch_logprobs_bwd_t<float>(a, nvec, s)
-               : launch_logprobs_bwd_t<__nv_bfloat16>(a, nvec, s);
+  return x_f32 ? launch_logprobs_bwd_t<float>(a, nvec, after, s)
+               : launch_logprobs_bwd_t<__nv_bfloat16>(a, nvec, after, s);
 }
 
 constexpr int kRingSmem = 108 * 1024;  // two CTAs an SM
@@ -1817,10 +1888,11 @@ int launch_ring(const RowArgs& a, int cs, int per, cudaStream_t s) {
     smem = kZeroBytes + stages * kChunk * 16 + (stages + 1) * a.K * 12;
     if (smem <= kRingSmem) break;
   }
-  int clusters = 2 * device_sm_count();
+  int clusters = std::min<int>(2 * device_sm_count(), kMaxRing);
   if (cs > 1 && (rc = resident_clusters(kern, cs, smem, &clusters))) return rc;
-  const int64_t n = std::min<int64_t>(a.T, clusters);
-  return launch_after(kern, n * cs, kRingThreads + 32, smem, cs, s, a, cs, per, stages);
+  const int64_t n = std::min<int64_t>(a.T, std::min<int64_t>(clusters, kMaxRing / cs)) * cs;
+  rc = launch_after(kern, n, kRingThreads + 32, smem, cs, s, a, cs, per, stages);
+  return rc ? rc : launch_after(finish_kernel, 1, 256, 0, 1, s, a, static_cast<int>(n));
 }
 
 template <typename T, int OBJ, int G, int NV>
@@ -1837,7 +1909,7 @@ int launch_direct(const RowArgs& a, int64_t grid, int smem, cudaStream_t s) {
 // How a row is held, by the vectors it spans. kNv vectors are the 64 elements that a thread
 // keeps as fp32.
 template <typename T, int OBJ>
-int launch_rows(const RowArgs& a, int nvec, cudaStream_t s) {
+int launch_rows(const RowArgs& a, int nvec, bool* done, cudaStream_t s) {
   constexpr int kNv = 64 / Vec<T>::kE;
   const int teacher = a.K * 12;
   if (nvec <= 128 * kNv) {
@@ -1859,26 +1931,25 @@ int launch_rows(const RowArgs& a, int nvec, cudaStream_t s) {
   while (cs < kMaxCluster && a.T * cs * 2 <= device_sm_count() &&
          nvec >= cs * 2 * kRingThreads)
     cs *= 2;
+  *done = true;
   return launch_ring<T, OBJ>(a, cs, (nvec + cs - 1) / cs, s);
 }
 
 // The list of rows, their statistics and gradients, the tokens' terms.
 template <int OBJ>
 int launch_loss(const RowArgs& a, int x_f32, cudaStream_t s) {
-  // one CTA lists 8192 rows in about the time that clearing the counters first would take
-  int64_t ctas = 1;
-  if (a.T > kCountBlock) {
-    ctas = std::min<int64_t>((a.T + kCountBlock - 1) / kCountBlock, device_sm_count());
-    LEMA_CUDA_TRY(cudaMemsetAsync(a.head, 0, kWsHead + (a.per_sequence ? a.n0 * 4 : 0), s));
-  }
+  const int64_t ctas = std::max<int64_t>(1, (a.T + kCountBlock - 1) / kCountBlock);
+  if (ctas > 1 && a.per_sequence) LEMA_CUDA_TRY(cudaMemsetAsync(a.seq_count, 0, a.n0 * 4, s));
   count_kernel<<<static_cast<unsigned>(ctas), kCountThreads, 0, s>>>(a);
   LEMA_CUDA_TRY(cudaGetLastError());
+  bool done = false;  // the tokens' terms are on their way
   if (a.T > 0) {
     const int nvec = max_vecs(a, x_f32);
-    const int rc = x_f32 ? launch_rows<float, OBJ>(a, nvec, s)
-                         : launch_rows<__nv_bfloat16, OBJ>(a, nvec, s);
+    const int rc = x_f32 ? launch_rows<float, OBJ>(a, nvec, &done, s)
+                         : launch_rows<__nv_bfloat16, OBJ>(a, nvec, &done, s);
     if (rc) return rc;
   }
+  if (done) return LEMA_OK;
   return launch_after(token_kernel<OBJ>, std::max<int64_t>(1, token_ctas(a.T)), kTokenThreads, 0,
                       1, s, a);
 }
@@ -1945,7 +2016,7 @@ extern "C" int lema_token_logprobs_bwd(const void* x, int32_t x_f32, int64_t n0,
   if ((rc = set_stats(a, stats))) return rc;
   a.g = dlogps;
   a.upstream = upstream;
-  return launch_logprobs_bwd(a, x_f32, static_cast<cudaStream_t>(stream));
+  return launch_logprobs_bwd(a, x_f32, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int lema_preference_loss(const void* x, int32_t x_f32, int64_t n0, int64_t n1,
@@ -1974,17 +2045,20 @@ extern "C" int lema_preference_loss(const void* x, int32_t x_f32, int64_t n0, in
   if ((rc = set_stats(a, stats))) return rc;
   a.coef = coef;
   auto s = static_cast<cudaStream_t>(stream);
-  if (a.T > 0 && (rc = launch_logprobs<true>(a, x_f32, s))) return rc;
-  pair_kernel<<<static_cast<unsigned>(n0 / 2), 256, 0, s>>>(a, n0 / 2, beta, label_smoothing,
-                                                            rewards);
-  LEMA_CUDA_TRY(cudaGetLastError());
-  pair_sum_kernel<<<1, 256, 0, s>>>(a.part, n0 / 2, loss);
-  LEMA_CUDA_TRY(cudaGetLastError());
+  a.loss = loss;
+  if (a.T > 0) {
+    if ((rc = launch_logprobs<true>(a, x_f32, s))) return rc;
+  } else {
+    LEMA_CUDA_TRY(cudaMemsetAsync(a.head, 0, sizeof(WsHead), s));
+  }
+  if ((rc = launch_after(pair_kernel, n0 / 2, kPairThreads, 0, 1, s, a, n0 / 2, beta,
+                         label_smoothing, rewards)))
+    return rc;
   if (dx == nullptr || a.T == 0) return LEMA_OK;
   a.g = coef;
   a.zeros_done = 1;
   a.grad_scale = static_cast<float>(grad_scale);
-  return launch_logprobs_bwd(a, x_f32, s);
+  return launch_logprobs_bwd(a, x_f32, true, s);
 }
 
 extern "C" int lema_policy_loss(const void* x, int32_t x_f32, int64_t n0, int64_t n1, int64_t ld0,
