@@ -273,14 +273,13 @@ __device__ __forceinline__ void shift_vec(uint4& w, float m) {
 // on [-1/2, 1/2], where its argument is brought here. Elements are kept above n - 120, which
 // is nothing beside the maximum. NaNs are looked for apart.
 struct WholeScale {
-  uint64_t c, c_lo, up, down;  // 1.5 * 2^23 - n, added and taken off: rounds to a whole number
+  uint64_t c, c_lo, up;  // 1.5 * 2^23 - n, added and taken off: rounds to a whole number
   __device__ __forceinline__ WholeScale(float n, float c_, float c_lo_)
-      : c(f2_splat(c_)), c_lo(f2_splat(c_lo_)), up(f2_splat(12582912.f - n)),
-        down(f2_splat(n - 12582912.f)) {}
+      : c(f2_splat(c_)), c_lo(f2_splat(c_lo_)), up(f2_splat(12582912.f - n)) {}
 };
 __device__ __forceinline__ uint64_t exp_pair_whole(uint64_t x, const WholeScale& k) {
   const uint64_t t = f2_fma(x, k.c, k.up);
-  const uint64_t minus_u = f2_fma(f2_add(t, k.down), f2_splat(-1.f), f2_splat(0.f));
+  const uint64_t minus_u = f2_fma(t, f2_splat(-1.f), k.up);
   float f0, f1, t0, t1;
   f2_unpack(f2_fma(x, k.c_lo, f2_fma(x, k.c, minus_u)), f0, f1);
   f2_unpack(t, t0, t1);
@@ -366,9 +365,9 @@ __device__ __forceinline__ void group_sync() {
     __syncthreads();
 }
 
-// Maximum of a row and sum of exp((x - m) / tau) from the (m, s) of a group's threads; every
-// thread gets both. WHOLE: their sums are about whole_max of their own maxima (about the maximum
-// itself when far_max). Sums meet in fp64.
+// Maximum of a row and sum of exp((x - m) / tau) from the (m, s) of a group's threads, for every
+// thread. WHOLE: the sums are about whole_max of their own maxima (about the maximum itself
+// when far_max), and the row's is about its own: see about_max. Sums meet in fp64.
 template <int G, bool WHOLE>
 __device__ __forceinline__ void group_combine(float& m, double& s, const RowArgs& a, float* redf,
                                               double* redd) {
@@ -396,9 +395,13 @@ __device__ __forceinline__ void group_combine(float& m, double& s, const RowArgs
 #pragma unroll
     for (int w = 1; w < G / 32; ++w) s += redd[w];
   }
-  // from about n to about m; a row of -inf alone is NaN
-  if (!far) s *= exp2(static_cast<double>(n) - static_cast<double>(m) * a.c_full);
   if (m == -INFINITY) s = NAN;
+}
+// The logarithm that takes a sum about whole_max of m to one about m.
+__device__ __forceinline__ double about_max(float m, const RowArgs& a) {
+  if (far_max(m, a.c)) return 0.0;
+  return (static_cast<double>(whole_max(m, a.c)) - static_cast<double>(m) * a.c_full) *
+         0.6931471805599453;
 }
 
 // One thread's share of a row's maximum and sum: its edge and the vectors tid, tid + G, ..., in
@@ -664,7 +667,7 @@ __device__ __forceinline__ void zero_row(const RowArgs& a, int64_t r, int tid) {
 
 // token_logprobs: a group of G threads a row, a warp for short rows (one CTA a row leaves most
 // of its threads without a vector there).
-constexpr int kStatThreads = 256;
+constexpr int kStatThreads = 128;
 template <typename T, int G, bool WHOLE>
 __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
   __shared__ float redf[kStatThreads / 32];
@@ -688,16 +691,17 @@ __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
   const Span<T> sp(x, a.V);
   float m;
   double s;
-  thread_stats<T, G, 4, WHOLE>(x, sp, tid, a.c, a.c_lo, m, s);
+  thread_stats<T, G, 8, WHOLE>(x, sp, tid, a.c, a.c_lo, m, s);
   group_combine<G, WHOLE>(m, s, a, redf, redd);
   if (tid == 0) {
+    const double up = WHOLE ? about_max(m, a) : 0.0, log_s = log(s) + up;
     const double lp =
-        ok ? (static_cast<double>(xt) - m) * a.inv_tau + (WHOLE ? ex2_error(xt, a) : 0.0) - log(s)
+        ok ? (static_cast<double>(xt) - m) * a.inv_tau + (WHOLE ? ex2_error(xt, a) : 0.0) - log_s
            : NAN;
     if (!ok) atomicMax(a.err, static_cast<int32_t>(kDevErrIndex));
     a.logps[r] = static_cast<float>(lp);
     if (a.lp64) a.lp64[r] = lp;
-    if (a.stats) a.stats[r] = make_float2(m, static_cast<float>(1.0 / s));
+    if (a.stats) a.stats[r] = make_float2(m, static_cast<float>(1.0 / s) * expf(static_cast<float>(-up)));
   }
 }
 
@@ -1625,9 +1629,10 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
   constexpr int E = Vec<T>::kE;
   const int tid = threadIdx.x % G;
   const int64_t unit = blockIdx.x * int64_t{kBwdThreads / G} + threadIdx.x / G;
-  const int64_t r = unit / chunks;
-  if (r >= a.T) return;
-  const int chunk = static_cast<int>(unit - r * chunks);
+  if (unit >= a.T * chunks) return;
+  // behind the statistics: from the last row on, which L2 still holds
+  const int64_t at_row = unit / chunks, r = a.zeros_done ? a.T - 1 - at_row : at_row;
+  const int chunk = static_cast<int>(unit - at_row * chunks);
   const int v0 = chunk * (G * kBwdU) + tid;
   const T* x = static_cast<const T*>(a.x) + a.in.at(r);
   T* dx = static_cast<T*>(a.dx) + a.out.at(r);

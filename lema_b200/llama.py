@@ -290,7 +290,7 @@ class LlamaBlock(nn.Module):
         for name in ("q_proj", "k_proj", "v_proj"):
             m = getattr(att, name)
             lora.append((hn @ m.lora_A.transpose(0, 1) @ m.lora_B.transpose(0, 1)) * m.scaling
-                        if isinstance(m, LoRALinear) else None)
+                        if isinstance(m, LoRALinear) and m.enabled else None)
         qr, kr, vc = ops.RopeQKVFn.apply(q, k, v, *lora, cos.reshape(-1, d), sin.reshape(-1, d),
                                          S, sh.heads, sh.kv_heads, d)
         qv = qr.view(B, S, sh.heads, d).transpose(1, 2)

@@ -154,6 +154,10 @@ class LoRALinear(nn.Module):
         self.lora_A = lora_A
         self.lora_B = lora_B
 
+    # False: the base layer alone, the frozen model that preference and policy
+    # losses refer to.
+    enabled = True
+
     @property
     def in_features(self) -> int:
         return self.base_layer.in_features
@@ -164,5 +168,7 @@ class LoRALinear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         result = self.base_layer(x)
+        if not self.enabled:
+            return result
         lora_out = (x @ self.lora_A.transpose(0, 1) @ self.lora_B.transpose(0, 1)) * self.scaling
         return result + lora_out

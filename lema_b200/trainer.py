@@ -14,7 +14,8 @@
   bytes (by default a quarter of the memory free when the trainer is built),
   offloading only the rest;
 * head + loss (reference :151-162): final RMSNorm, bf16 lm_head, shifted
-  cross entropy, backward to the last hidden state;
+  cross entropy (or a preference, policy or distillation objective, see
+  ``objectives``), backward to the last hidden state;
 * backward in reverse (reference :125-173): the saved input is restored on the
   H2D stream, the block is re-run with grad and back-propagated; the two
   blocks still resident at the turnaround are reused without re-upload; each
@@ -44,6 +45,8 @@ import torch.nn.functional as F
 
 from . import ops
 from .llama import LlamaBlock, LlamaHead, LlamaShape, apply_lora, rope_cos_sin
+from .modules import LoRALinear
+from .objectives import next_targets
 from .tensorstore import ActivationCheckpointStore, WeightSegments
 
 
@@ -301,10 +304,45 @@ class StreamedLoraTrainer:
         if layer >= len(self.resident):
             self.ws.release(layer % self.nslots)
 
+    # ---- scoring ---------------------------------------------------------------
+    @torch.no_grad()
+    def token_logprobs(self, ids: torch.Tensor, labels: torch.Tensor | None = None,
+                       adapters: bool = True, temperature: float = 1.0) -> torch.Tensor:
+        """Log-probabilities [batch, seq] fp32 that the model gives the next token of
+        each position (0 where it has none or its label is -100), by one streamed
+        forward. ``adapters=False`` leaves the LoRA adapters out: the frozen model
+        that preference and policy objectives refer to."""
+        self.errors.check()
+        dev = self.device
+        ids = ids.to(dev, non_blocking=True)
+        labels = ids if labels is None else labels.to(dev, non_blocking=True)
+        lora = [m for blk in self.blocks for m in blk.modules() if isinstance(m, LoRALinear)]
+        ahead = self.nslots - 1
+        for m in lora:
+            m.enabled = adapters
+        try:
+            h = self.embed(ids)
+            for k in range(min(ahead, self.L)):
+                self._ensure(k)
+            for i in range(self.L):
+                if i + ahead < self.L:
+                    self._ensure(i + ahead)
+                h = self._bind(i)(h, self.cos, self.sin)
+                self._release(i)
+            logps = ops.token_logprobs(self.head(h), next_targets(labels),
+                                       temperature=temperature)
+        finally:
+            for m in lora:
+                m.enabled = True
+        self.errors.arm(torch.cuda.current_stream(dev).cuda_stream)
+        return logps
+
     # ---- one step ------------------------------------------------------------
-    def train_step(self, ids: torch.Tensor, labels: torch.Tensor | None = None) -> torch.Tensor:
+    def train_step(self, ids: torch.Tensor, labels: torch.Tensor | None = None,
+                   objective=None) -> torch.Tensor:
         """One optimizer step on a [batch, seq] micro-batch of token ids (device or
-        pinned host). Returns the loss as a 0-d device tensor."""
+        pinned host). Returns the loss as a 0-d device tensor. ``objective`` (see
+        ``lema_b200.objectives``) takes the place of the shifted cross entropy."""
         self.errors.check()
         dev = self.device
         ids = ids.to(dev, non_blocking=True)
@@ -328,10 +366,15 @@ class StreamedLoraTrainer:
         # head + loss
         h = h.detach().requires_grad_(True)
         logits = self.head(h)
-        loss = F.cross_entropy(logits[:, :-1].reshape(-1, logits.shape[-1]),
-                               labels[:, 1:].reshape(-1))
         # the reference divides by the accumulation count (src/lema/_trainer.py:156)
-        (loss / self.grad_accum).backward()
+        if objective is None:
+            loss = F.cross_entropy(logits[:, :-1].reshape(-1, logits.shape[-1]),
+                                   labels[:, 1:].reshape(-1))
+            (loss / self.grad_accum).backward()
+        else:
+            loss, dlogits = objective(logits.detach(), next_targets(labels), 1 / self.grad_accum)
+            torch.autograd.backward(logits, dlogits)
+            del dlogits
         self.micro_step += 1
         stepping = self.micro_step % self.grad_accum == 0
         grad = h.grad

@@ -14,6 +14,13 @@ def logprobs(rows=ROWS, targets=FAKE, tau=1.0, logps=FAKE):
     return N.lib().lema_token_logprobs(*rows, targets, -100, tau, logps, None, None)
 
 
+@pytest.fixture(autouse=True)
+def _no_error_left():
+    yield
+    logprobs((None, 0, 0, 3, 300, 100, 100))     # a call that succeeds clears the message
+    assert N.last_error() == ""
+
+
 def test_rows():
     assert logprobs((None, 0, 0, 3, 300, 100, 100)) == N.LEMA_OK       # no rows: nothing to do
     assert logprobs((None, 0, 2, 0, 300, 100, 100)) == N.LEMA_OK
@@ -94,3 +101,20 @@ def test_rows_that_overlap_are_found():
     assert not ops._rows_disjoint(base[:1].expand(4, 6, 8))
     assert not ops._rows_disjoint(base.transpose(1, 2))
     assert not ops._rows_disjoint(base.as_strided((4, 6, 8), (48, 7, 1)))
+
+
+def test_next_targets():
+    from lema_b200.objectives import next_targets
+    labels = torch.tensor([[5, 6, -100, 7], [1, 2, 3, 4]])
+    assert next_targets(labels).tolist() == [[6, -100, 7, -100], [2, 3, 4, -100]]
+
+
+def test_adapters_can_be_left_out():
+    from lema_b200.modules import LoRALinear
+    base = torch.nn.Linear(8, 6, bias=False)
+    m = LoRALinear(base, 2, 4.0, dtype=torch.float32)
+    torch.nn.init.normal_(m.lora_B)
+    x = torch.randn(3, 8)
+    assert not torch.equal(m(x), base(x))
+    m.enabled = False
+    assert torch.equal(m(x), base(x)) and LoRALinear.enabled
