@@ -38,8 +38,13 @@ constexpr int kMaxTeacher = 1024;
 // Rows of logits: row r starts (r / n1) * ld0 + (r % n1) * ld1 elements behind the base.
 struct RowMap {
   int64_t n1, ld0, ld1;
+  // Row numbers fit 32 bits, which divide several times faster than 64.
+  __device__ __forceinline__ uint32_t seq(int64_t r) const {
+    return static_cast<uint32_t>(r) / static_cast<uint32_t>(n1);
+  }
   __device__ __forceinline__ int64_t at(int64_t r) const {
-    return (r / n1) * ld0 + (r % n1) * ld1;
+    const uint32_t b = seq(r);
+    return b * ld0 + (r - b * n1) * ld1;
   }
 };
 
@@ -97,7 +102,7 @@ struct RowArgs {
   int32_t ids_i32;
   const void* teacher_logits;
   int32_t tl_f32;
-  int32_t K;
+  int32_t K, K4;                 // entries a row, rounded up to four
   const uint8_t* mask;           // [T], may be null
   // backward from saved statistics
   const float* g;                // [T] gradient of each row's log-probability (or row weight)
@@ -489,7 +494,7 @@ __device__ __forceinline__ double softplus(double x) {
 
 // 1 / (the number of tokens a token's term is divided by).
 __device__ __forceinline__ double token_weight(const RowArgs& a, int64_t r) {
-  const int64_t n = a.per_sequence ? a.n0 * a.seq_count[r / a.in.n1] : a.head->total;
+  const int64_t n = a.per_sequence ? a.n0 * a.seq_count[a.in.seq(r)] : a.head->total;
   return 1.0 / static_cast<double>(n);
 }
 
@@ -498,19 +503,20 @@ struct Token {
   float adv, old, ref;
 };
 __device__ __forceinline__ Token load_token(const RowArgs& a, int64_t r) {
-  const int64_t b = r / a.in.n1, t = r % a.in.n1;
+  const int64_t b = a.in.seq(r), t = r - b * a.in.n1;
   return Token{a.adv[b * a.adv_s0 + t * a.adv_s1], a.old_logps ? a.old_logps[r] : 0.f,
                a.ref_logps ? a.ref_logps[r] : 0.f};
 }
 
 // dL/dlp of one token of the clipped policy loss over its weight, and (LOSS) its loss and KL.
 // F = double for what is returned, float for the gradient's coefficient.
-template <typename F, bool LOSS>
+template <typename F, bool LOSS, bool FAST = false>
 __device__ __forceinline__ F policy_token(const RowArgs& a, const Token& tk, F lp, F* loss,
                                           F* kl) {
   const F A = tk.adv;
   // on-policy the ratio is 1, and NaN for a log-probability that is not finite
-  const F ratio = exp(lp - (a.old_logps ? static_cast<F>(tk.old) : lp));
+  const F up = lp - (a.old_logps ? static_cast<F>(tk.old) : lp);
+  const F ratio = FAST ? static_cast<F>(__expf(static_cast<float>(up))) : exp(up);
   const F lo = static_cast<F>(1.0 - a.clip_lo), hi = static_cast<F>(1.0 + a.clip_hi);
   const F bent = ratio < lo ? lo : (ratio > hi ? hi : ratio);  // a NaN ratio stays NaN
   const F plain = ratio * A, clipped = bent * A;
@@ -519,7 +525,7 @@ __device__ __forceinline__ F policy_token(const RowArgs& a, const Token& tk, F l
   F d_kl = F(0);
   if (a.ref_logps) {
     const F d = static_cast<F>(tk.ref) - lp;
-    const F e = expm1(d);
+    const F e = FAST ? static_cast<F>(__expf(static_cast<float>(d)) - 1.f) : expm1(d);
     d_kl = e - d;
     coef -= static_cast<F>(a.kl_coef) * e;
   }
@@ -582,9 +588,9 @@ __global__ void __launch_bounds__(kCountThreads) count_kernel(RowArgs a) {
     ballot[j] = __ballot_sync(0xffffffffu, in[j]);
     if (lane == 0) s_cell[j * 32 + warp] = __popc(ballot[j]);
     if (a.per_sequence) {
-      const int64_t r = r0 + j * kCountThreads + tid, b = r / a.in.n1;
+      const int64_t r = r0 + j * kCountThreads + tid, b = a.in.seq(r);
       // a warp inside one sequence adds once
-      const bool one = (r - lane) / a.in.n1 == (r - lane + 31) / a.in.n1;
+      const bool one = __all_sync(0xffffffffu, __shfl_sync(0xffffffffu, b, 0) == b);
       if (one ? lane == 0 && ballot[j] != 0 : in[j])
         atomicAdd(&a.seq_count[b], one ? __popc(ballot[j]) : 1);
     }
@@ -753,6 +759,10 @@ __device__ __forceinline__ TeacherSums teacher_weights(const RowArgs& a, int64_t
       }
     }
   }
+  for (int k = a.K + lane; k < a.K4; k += 32) {
+    s_p[k] = 0.f;
+    s_id[k] = -1;
+  }
   tm = warp_max(tm);
   double sum = 0.0, d_sum = 0.0;
   bool bad = false;
@@ -777,13 +787,22 @@ __device__ __forceinline__ TeacherSums teacher_weights(const RowArgs& a, int64_t
 }
 
 // The value of a gradient row at an entry's index: k (q - p), p the sum of the entries that hold
-// this index, in their order, so that entries which repeat it write the same value.
+// this index, always in the same order, so that entries which repeat it write the same value.
+// Four entries a read; those behind the last hold no index.
 __device__ __forceinline__ float teacher_value(const RowArgs& a, int32_t id, const float* s_p,
                                                const int32_t* s_id, float q, float inv_t,
                                                float k) {
-  float p = 0.f;
-  for (int i = 0; i < a.K; ++i) p += s_id[i] == id ? s_p[i] : 0.f;
-  return k * (q - p * inv_t);
+  float p0 = 0.f, p1 = 0.f, p2 = 0.f, p3 = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < a.K4; i += 4) {
+    const int4 d = *reinterpret_cast<const int4*>(s_id + i);
+    const float4 p = *reinterpret_cast<const float4*>(s_p + i);
+    p0 += d.x == id ? p.x : 0.f;
+    p1 += d.y == id ? p.y : 0.f;
+    p2 += d.z == id ? p.z : 0.f;
+    p3 += d.w == id ? p.w : 0.f;
+  }
+  return k * (q - ((p0 + p1) + (p2 + p3)) * inv_t);
 }
 
 // k of a distilled row: tau over the number of rows, 0 for a row without an entry.
@@ -794,11 +813,16 @@ __device__ __forceinline__ float teacher_coef(const TeacherSums& t, float share)
   return t.bad ? NAN : (t.t_sum == 0.f ? 0.f : share);
 }
 
-// k of a token of the policy loss.
+// k of a token of the policy loss, for its gradient row alone. A bf16 row is rounded to 2^-9, so
+// the approximate logarithm and exponentials (2e-6 at worst here) serve it; they cut what every
+// thread of a row waits for from 1200 to 500 cycles.
+template <typename T>
 __device__ __forceinline__ float policy_coef(const RowArgs& a, const Token& tk, float xt, float m,
                                              float s, float w) {
-  const float lp = (xt - m) * static_cast<float>(a.inv_tau) - logf(s);
-  return policy_token<float, false>(a, tk, lp, nullptr, nullptr) * w;
+  const float d = (xt - m) * static_cast<float>(a.inv_tau);
+  if (sizeof(T) == 4)
+    return policy_token<float, false>(a, tk, d - logf(s), nullptr, nullptr) * w;
+  return policy_token<float, false, true>(a, tk, d - __logf(s), nullptr, nullptr) * w;
 }
 
 __device__ __forceinline__ float grad_factor(const RowArgs& a) {
@@ -822,9 +846,9 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   __shared__ TeacherSums s_t[kGroups];
   extern __shared__ __align__(16) char smem[];
   const int tid = threadIdx.x % G, group = threadIdx.x / G, warp = tid >> 5;
-  float* s_p = reinterpret_cast<float*>(smem) + group * 3 * a.K;
-  float* s_x = s_p + a.K;
-  int32_t* s_id = reinterpret_cast<int32_t*>(s_x + a.K);
+  float* s_p = reinterpret_cast<float*>(smem) + group * 3 * a.K4;
+  float* s_x = s_p + a.K4;
+  int32_t* s_id = reinterpret_cast<int32_t*>(s_x + a.K4);
   ptx::griddep_wait();
   const int64_t r = blockIdx.x * int64_t{kGroups} + group;
   if (r >= a.T) return;
@@ -903,7 +927,7 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
       a.row[r] = RowStat{m, s, t.t_sum, 0.f, t.about(m)};
     }
   } else {
-    k = policy_coef(a, tk, xt, m, s, weight);
+    k = policy_coef<T>(a, tk, xt, m, s, weight);
     if (tid == 0) {
       if (!ok) note_bad_index(a);
       a.row[r] = RowStat{m, s, xt, 0.f, 0.0};
@@ -1059,8 +1083,8 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
   uint4* zeros = reinterpret_cast<uint4*>(smem);
   uint4* ring = zeros + kZeroBytes / 16;  // [stages][kChunk]
   float* s_p0 = reinterpret_cast<float*>(ring + stages * kChunk);
-  float* s_x0 = s_p0 + (stages + 1) * a.K;  // each [stages + 1][K]
-  int32_t* s_id0 = reinterpret_cast<int32_t*>(s_x0 + (stages + 1) * a.K);
+  float* s_x0 = s_p0 + (stages + 1) * a.K4;  // each [stages + 1][K4]
+  int32_t* s_id0 = reinterpret_cast<int32_t*>(s_x0 + (stages + 1) * a.K4);
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], exchanged[2];
   // A row's numbers come with its first chunk and are used until its end. The producer is at
   // most `stages` rows ahead of a row whose first chunk every warp has read, and a warp reads
@@ -1174,8 +1198,9 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
                 inf->edge[lane] = e >= 0 ? to_f(x[e]) : -INFINITY;
               }
               if (OBJ == kDistill) {
-                const TeacherSums t = teacher_weights<T>(a, r, x, lane, s_p0 + slot * a.K,
-                                                         s_x0 + slot * a.K, s_id0 + slot * a.K);
+                const TeacherSums t = teacher_weights<T>(a, r, x, lane, s_p0 + slot * a.K4,
+                                                         s_x0 + slot * a.K4,
+                                                         s_id0 + slot * a.K4);
                 if (lane == 0) inf->t = t;
               }
             }
@@ -1230,10 +1255,10 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
       const RowInfo* inf = &info[slot];
       // the row's share into registers, and its maximum
       uint4 w[kRingVecs];
+      const int st_row = st;
       ok = ptx::mbar_wait(&full[st], phase) && ok;
       const int nv = inf->nv;
       const float xe = tid < kEdges ? inf->edge[tid] : -INFINITY;
-      float m = xe;
 #pragma unroll
       for (int c = 0; c < kRingVecs / kChunkVecs; ++c) {
         if (c == 0 || c * kChunk < nv) {
@@ -1247,16 +1272,25 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
               if (c * kChunk + j * kRingThreads + tid >= nv)
                 w[c * kChunkVecs + j] = neg_inf_vec<T>();
           }
-#pragma unroll
-          for (int j = 0; j < kChunkVecs; ++j) m = fmaxf(m, Vec<T>::max(w[c * kChunkVecs + j]));
-          __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(&empty[st]);
           if (++st == stages) {
             st = 0;
             phase ^= 1u;
           }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kChunkVecs; ++j) w[c * kChunkVecs + j] = neg_inf_vec<T>();
         }
       }
+      float m = xe;
+#pragma unroll
+      for (int j = 0; j < kRingVecs; ++j) m = fmaxf(m, Vec<T>::max(w[j]));
+      // every lane has its part of the chunks
+      __syncwarp();
+      if (lane == 0)
+        for (int c = 0, e = st_row; c == 0 || c * kChunk < nv; ++c) {
+          ptx::mbar_arrive(&empty[e]);
+          if (++e == stages) e = 0;
+        }
       m = warp_max(m);
       if (lane == 0) red_m[warp] = m;
       // one barrier for the maximum and for every thread's waits: all leave here, or none
@@ -1328,7 +1362,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
           a.row[inf->row] = RowStat{m_row, s, inf->t.t_sum, 0.f, inf->t.about(m_row)};
         }
       } else {
-        k = policy_coef(a, inf->tk, inf->xt, m_row, s, inf->w);
+        k = policy_coef<T>(a, inf->tk, inf->xt, m_row, s, inf->w);
         if (tid == 0 && rank == 0) {
           if (inf->target < 0) note_bad_index(a);
           a.row[inf->row] = RowStat{m_row, s, inf->xt, 0.f, 0.0};
@@ -1376,9 +1410,9 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
               put(dx + inf->target, k - ex2((inf->xt - m_row) * a.c) * inv_s * k);
           } else {
             ring_sync();
-            const float* s_p = s_p0 + slot * a.K;
-            const float* s_x = s_x0 + slot * a.K;
-            const int32_t* s_id = s_id0 + slot * a.K;
+            const float* s_p = s_p0 + slot * a.K4;
+            const float* s_x = s_x0 + slot * a.K4;
+            const int32_t* s_id = s_id0 + slot * a.K4;
             const float inv_t = 1.f / inf->t.t_sum;
             for (int j = tid; j < a.K; j += kRingThreads)
               if (s_id[j] >= 0 &&
@@ -1424,8 +1458,8 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
   constexpr int E = Vec<T>::kE;
   extern __shared__ __align__(16) char smem[];
   float* s_p = reinterpret_cast<float*>(smem);
-  float* s_x = s_p + a.K;
-  int32_t* s_id = reinterpret_cast<int32_t*>(s_x + a.K);
+  float* s_x = s_p + a.K4;
+  int32_t* s_id = reinterpret_cast<int32_t*>(s_x + a.K4);
   __shared__ float redf[kRowThreads / 32];
   __shared__ double redd[kRowThreads / 32];
   __shared__ TeacherSums s_t;
@@ -1461,7 +1495,7 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
         a.row[r] = RowStat{m, s, s_t.t_sum, 0.f, s_t.about(m)};
       }
     } else {
-      k = policy_coef(a, load_token(a, r), xt, m, s,
+      k = policy_coef<T>(a, load_token(a, r), xt, m, s,
                       static_cast<float>(token_weight(a, r) * a.inv_tau));
       if (tid == 0) {
         if (!ok) note_bad_index(a);
@@ -1890,7 +1924,7 @@ int launch_ring(const RowArgs& a, int cs, int per, cudaStream_t s) {
   if (rc) return rc;
   int stages = kMaxStages, smem = 0;
   for (;; --stages) {
-    smem = kZeroBytes + stages * kChunk * 16 + (stages + 1) * a.K * 12;
+    smem = kZeroBytes + stages * kChunk * 16 + (stages + 1) * a.K4 * 12;
     if (smem <= kRingSmem) break;
   }
   int clusters = std::min<int>(2 * device_sm_count(), kMaxRing);
@@ -1916,7 +1950,7 @@ int launch_direct(const RowArgs& a, int64_t grid, int smem, cudaStream_t s) {
 template <typename T, int OBJ>
 int launch_rows(const RowArgs& a, int nvec, bool* done, cudaStream_t s) {
   constexpr int kNv = 64 / Vec<T>::kE;
-  const int teacher = a.K * 12;
+  const int teacher = a.K4 * 12;
   if (nvec <= 128 * kNv) {
     const bool warps = nvec <= 32 * kNv;
     const int64_t per = warps ? kDirectThreads / 32 : 1, grid = (a.T + per - 1) / per;
@@ -2127,6 +2161,7 @@ extern "C" int lema_distill_loss(const void* x, int32_t x_f32, int64_t n0, int64
   a.teacher_logits = teacher_logits;
   a.tl_f32 = tl_f32;
   a.K = static_cast<int32_t>(K);
+  a.K4 = (a.K + 3) / 4 * 4;
   a.mask = mask;
   a.grad_scale = static_cast<float>(grad_scale);
   a.upstream = upstream;
