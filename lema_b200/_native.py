@@ -150,7 +150,8 @@ def last_error() -> str:
 
 
 # Kernels each entry point launches (the checkpoint save launches one only in
-# its SM-store mode 1; its copy-engine mode and the restore launch none).
+# its SM-store mode 1; its copy-engine mode and the restore launch none; the policy and
+# distillation losses launch one more to list their rows when there are many).
 KERNELS_PER_CALL = {
     "lema_quantize_rows": 1, "lema_quantize_rows_f32": 1, "lema_quantize_per_token": 1,
     "lema_w8a8_gemm": 1, "lema_w8a8_linear_fwd": 2, "lema_w8a8_linear_fwd_noalloc": 2,
@@ -161,7 +162,7 @@ KERNELS_PER_CALL = {
     "lema_rope": 1, "lema_rope_qkv": 1, "lema_swiglu_quant": 1, "lema_swiglu_bwd": 1,
     "lema_adamw_requant_rows": 1, "lema_device_error_async": 1, "lema_attn_fwd": 1,
     "lema_attn_bwd": 3, "lema_token_logprobs": 1, "lema_token_logprobs_bwd": 1,
-    "lema_preference_loss": 2, "lema_policy_loss": 3, "lema_distill_loss": 3,
+    "lema_preference_loss": 2, "lema_policy_loss": 2, "lema_distill_loss": 2,
 }
 # Running count of this library's kernel launches issued by this process.
 kernel_launches = 0

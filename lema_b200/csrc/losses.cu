@@ -108,6 +108,7 @@ struct RowArgs {
   const float* g;                // [T] gradient of each row's log-probability (or row weight)
   const float* upstream;         // scalar, may be null
   int32_t zeros_done;            // the rows of zeros are written
+  int32_t self_count;            // no count_kernel ran: CTAs count for themselves
 };
 
 enum Objective { kLogp = 0, kPolicy = 1, kDistill = 2 };
@@ -492,10 +493,18 @@ __device__ __forceinline__ double softplus(double x) {
   return fmax(x, 0.0) + log1p(exp(-fabs(x)));
 }
 
+// How many rows count: in all, and (per_sequence) of each sequence.
+struct Counts {
+  int64_t total;
+  const int32_t* seq;
+};
+// Those that count_kernel left.
+__device__ __forceinline__ Counts listed_counts(const RowArgs& a) {
+  return Counts{a.head->total, a.seq_count};
+}
 // 1 / (the number of tokens a token's term is divided by).
-__device__ __forceinline__ double token_weight(const RowArgs& a, int64_t r) {
-  const int64_t n = a.per_sequence ? a.n0 * a.seq_count[a.in.seq(r)] : a.head->total;
-  return 1.0 / static_cast<double>(n);
+__device__ __forceinline__ double token_weight(const RowArgs& a, const Counts& n, int64_t r) {
+  return 1.0 / static_cast<double>(a.per_sequence ? a.n0 * n.seq[a.in.seq(r)] : n.total);
 }
 
 // What the clipped policy loss knows of a token besides its log-probability.
@@ -630,6 +639,22 @@ __global__ void __launch_bounds__(kCountThreads) count_kernel(RowArgs a) {
   }
 }
 
+// Few rows are counted by each CTA that needs the numbers, which saves the launch of
+// count_kernel (and its latency, which the first rows would wait for).
+constexpr int64_t kSelfRows = 1024;  // by the CTAs of direct_kernel and token_kernel
+
+// Rows from `from` on, n of them, that count: the share of thread t of G.
+template <int G>
+__device__ __forceinline__ int count_rows(const RowArgs& a, int64_t from, int64_t n, int t) {
+  int sum = 0;
+#pragma unroll 8
+  for (int64_t i = t; i < n; i += G) {
+    int64_t target;
+    sum += row_counts(a, from + i, target);
+  }
+  return sum;
+}
+
 // What a row that does not count leaves in the policy loss's outputs.
 __device__ __forceinline__ void zero_outputs(const RowArgs& a, int64_t r) {
   if (a.logps) a.logps[r] = 0.f;
@@ -640,7 +665,7 @@ __device__ __forceinline__ void zero_outputs(const RowArgs& a, int64_t r) {
 // One token's terms in fp64, from what its row left: its share of the loss and of the KL, its
 // log-probability, and what the backward needs.
 template <int OBJ>
-__device__ __forceinline__ double2 token_terms(const RowArgs& a, int64_t r) {
+__device__ __forceinline__ double2 token_terms(const RowArgs& a, const Counts& n, int64_t r) {
   const RowStat st = a.row[r];
   const double log_s = log(static_cast<double>(st.s));
   if (OBJ == kDistill) {
@@ -648,10 +673,11 @@ __device__ __forceinline__ double2 token_terms(const RowArgs& a, int64_t r) {
     const double t = st.x;
     if (t == 0.0) return make_double2(0.0, 0.0);
     return make_double2((st.a / t * a.inv_tau - log(t) + log_s) /
-                            (static_cast<double>(a.head->total) * a.inv_tau * a.inv_tau),
+                            (static_cast<double>(n.total) * a.inv_tau * a.inv_tau),
                         0.0);
   }
-  const double w = token_weight(a, r), lp = (static_cast<double>(st.x) - st.m) * a.inv_tau - log_s;
+  const double w = token_weight(a, n, r),
+               lp = (static_cast<double>(st.x) - st.m) * a.inv_tau - log_s;
   double loss, kl;
   const double coef = policy_token<double, true>(a, load_token(a, r), lp, &loss, &kl);
   a.logps[r] = static_cast<float>(lp);
@@ -688,7 +714,7 @@ __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
       a.logps[r] = 0.f;
       if (a.stats) a.stats[r] = make_float2(0.f, 0.f);
     }
-    zero_row<T, G>(a, r, tid);  // among reads: HBM takes writes alone at half the rate of both
+    zero_row<T, G>(a, r, tid);  // the gradient's kernel has the rest to write
     return;
   }
   const T* x = static_cast<const T*>(a.x) + a.in.at(r);
@@ -806,8 +832,8 @@ __device__ __forceinline__ float teacher_value(const RowArgs& a, int32_t id, con
 }
 
 // k of a distilled row: tau over the number of rows, 0 for a row without an entry.
-__device__ __forceinline__ float row_share(const RowArgs& a) {
-  return static_cast<float>(1.0 / (static_cast<double>(a.head->total) * a.inv_tau));
+__device__ __forceinline__ float row_share(const RowArgs& a, const Counts& n) {
+  return static_cast<float>(1.0 / (static_cast<double>(n.total) * a.inv_tau));
 }
 __device__ __forceinline__ float teacher_coef(const TeacherSums& t, float share) {
   return t.bad ? NAN : (t.t_sum == 0.f ? 0.f : share);
@@ -849,8 +875,24 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   float* s_p = reinterpret_cast<float*>(smem) + group * 3 * a.K4;
   float* s_x = s_p + a.K4;
   int32_t* s_id = reinterpret_cast<int32_t*>(s_x + a.K4);
+  __shared__ int32_t s_count[kDirectThreads / 32], s_seq[kGroups];
   ptx::griddep_wait();
   const int64_t r = blockIdx.x * int64_t{kGroups} + group;
+  Counts counts = listed_counts(a);
+  if (a.self_count) {
+    const uint32_t b = a.in.seq(min(r, a.T - 1));
+    int n = a.per_sequence ? count_rows<G>(a, b * a.in.n1, a.in.n1, tid)
+                           : count_rows<kDirectThreads>(a, 0, a.T, threadIdx.x);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((threadIdx.x & 31) == 0) s_count[threadIdx.x >> 5] = n;
+    __syncthreads();
+    n = 0;
+    for (int w = 0; w < kDirectThreads / 32; ++w)
+      if (!a.per_sequence || G > 32 || w == group) n += s_count[w];
+    if (tid == 0) s_seq[group] = n;
+    counts = Counts{n, s_seq + group - static_cast<int64_t>(b)};
+    __syncthreads();
+  }
   if (r >= a.T) return;
   int64_t target = -1;
   if (!row_counts(a, r, target)) {
@@ -872,7 +914,7 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   float weight = 0.f;
   if (OBJ == kPolicy) {
     tk = load_token(a, r);
-    weight = static_cast<float>(token_weight(a, r) * a.inv_tau);
+    weight = static_cast<float>(token_weight(a, counts, r) * a.inv_tau);
   } else if (warp == 0) {
     const TeacherSums t = teacher_weights<T>(a, r, x, tid, s_p, s_x, s_id);
     if (tid == 0) s_t[group] = t;
@@ -921,7 +963,7 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   float k;
   if (OBJ == kDistill) {
     const TeacherSums t = s_t[group];
-    k = teacher_coef(t, row_share(a));
+    k = teacher_coef(t, row_share(a, counts));
     if (tid == 0) {
       if (t.bad) note_bad_index(a);
       a.row[r] = RowStat{m, s, t.t_sum, 0.f, t.about(m)};
@@ -1075,6 +1117,76 @@ __device__ __forceinline__ void store_remote(uint32_t dst, float a, float b, uin
       : "memory");
 }
 
+// The rows of one CTA: every step-th of those that count, every grid-th of the others. Listed
+// by the CTA itself while they are few, in the order of count_kernel's list.
+constexpr int kOwnRows = 256;
+constexpr int kOwnSeqs = 256;
+// Below this the CTAs are quicker: at 1833 rows 164 us against 165, at 4096 99 against 97, at 8192
+// 175 against 165.
+constexpr int64_t kOwnTotal = 2048;
+struct OwnRows {
+  int32_t row[kOwnRows], rest[kOwnRows], seq[kOwnSeqs];
+};
+template <int THREADS>
+__device__ __forceinline__ int list_own(const RowArgs& a, uint32_t first, uint32_t step,
+                                        OwnRows* own) {
+  constexpr int kRows = 8, kWarps = THREADS / 32, kCells = kRows * kWarps;
+  static_assert(kCells == 64, "two cells a lane");
+  __shared__ int32_t s_cell[kCells];
+  __shared__ int32_t s_end;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (a.per_sequence)
+    for (int b = tid; b < kOwnSeqs; b += THREADS) own->seq[b] = 0;
+  int before = 0;  // counted rows of the blocks in front
+  const int T = static_cast<int>(a.T);
+  for (int r0 = 0; r0 < T; r0 += kRows * THREADS) {
+    bool in[kRows];
+    uint32_t ballot[kRows];
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const int r = r0 + j * THREADS + tid;
+      int64_t target;
+      in[j] = r < T && row_counts(a, r, target);
+    }
+    __syncthreads();  // the cells of the block in front are read, the sequences are cleared
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      ballot[j] = __ballot_sync(0xffffffffu, in[j]);
+      if (lane == 0) s_cell[j * kWarps + warp] = __popc(ballot[j]);
+      if (a.per_sequence && in[j])
+        atomicAdd(&own->seq[a.in.seq(r0 + j * THREADS + tid)], 1);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      const int n0 = s_cell[2 * lane], n1 = s_cell[2 * lane + 1];
+      int incl = n0 + n1;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      s_cell[2 * lane] = before + incl - n0 - n1;
+      s_cell[2 * lane + 1] = before + incl - n1;
+      if (lane == 31) s_end = before + incl;
+    }
+    __syncthreads();
+    before = s_end;
+#pragma unroll
+    for (int j = 0; j < kRows; ++j) {
+      const int r = r0 + j * THREADS + tid;
+      const uint32_t rank = s_cell[j * kWarps + warp] + __popc(ballot[j] & ((1u << lane) - 1u));
+      if (in[j]) {
+        if (rank % step == first) own->row[rank / step] = r;
+      } else if (r < T) {
+        const uint32_t z = r - rank;
+        if (z % gridDim.x == blockIdx.x) own->rest[z / gridDim.x] = r;
+      }
+    }
+  }
+  __syncthreads();
+  return before;
+}
+
 template <typename T, int OBJ>
 __global__ void __launch_bounds__(kRingThreads + 32, 2)
     ring_kernel(RowArgs a, int cs, int per, int stages) {
@@ -1111,8 +1223,18 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
   if (cs > 1) ptx::cluster_sync();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   ptx::griddep_wait();
-  const int64_t total = static_cast<int64_t>(a.head->total);
+  __shared__ OwnRows own;
   const int64_t first = blockIdx.x / cs, step = gridDim.x / cs;
+  Counts counts = listed_counts(a);
+  if (a.self_count)
+    counts = Counts{list_own<kRingThreads + 32>(a, static_cast<uint32_t>(first),
+                                                static_cast<uint32_t>(step), &own),
+                    own.seq};
+  const int64_t total = counts.total;
+  const int n_row = total > first ? static_cast<int>((total - first + step - 1) / step) : 0;
+  const auto row_of = [&](int i) {
+    return a.self_count ? own.row[i] : a.list[first + i * step];
+  };
 
   if (warp == kRingWarps) {
     // ---- producer: 32 rows' numbers at a time, then each row's copies
@@ -1120,20 +1242,24 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
     uint32_t phase = 0;
     bool ok = true, more = true;
     // The rows of zeros, dealt to every CTA, are written between the others by bulk copies from
-    // shared memory: HBM takes writes alone at 3.9 TB/s, reads and writes together at 6.5.
+    // shared memory, which cost the threads that hold rows nothing.
     const int64_t rest = a.T - total;
     const int n_zero = rest > blockIdx.x
                            ? static_cast<int>((rest - blockIdx.x + gridDim.x - 1) / gridDim.x)
                            : 0;
-    const int n_row = total > first ? static_cast<int>((total - first + step - 1) / step) : 0;
     int z = 0, done = 0;
-    const int32_t* z_list = a.list + total + blockIdx.x;
-    int32_t z_row = n_zero > 0 ? z_list[0] : 0;
+    const auto rest_of = [&](int i) {
+      return a.self_count
+                 ? own.rest[i]
+                 // from the end backwards, as count_kernel puts them down
+                 : a.list[a.T - 1 - blockIdx.x - i * static_cast<int64_t>(gridDim.x)];
+    };
+    int32_t z_row = n_zero > 0 ? rest_of(0) : 0;
     const auto zero_rows = [&](int until) {
       for (; z < until; ++z) {
         T* dx = static_cast<T*>(a.dx) + a.out.at(z_row);
         if (OBJ == kPolicy && lane == 0) zero_outputs(a, z_row);
-        if (z + 1 < n_zero) z_row = z_list[(z + 1) * static_cast<int64_t>(gridDim.x)];
+        if (z + 1 < n_zero) z_row = rest_of(z + 1);
         if (a.dx == nullptr) continue;
         const Span<T> so(dx, a.V);
         if (lane < kEdges && so.edge(lane) >= 0) put(dx + so.edge(lane), 0.f);
@@ -1144,15 +1270,14 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
         ptx::bulk_commit_group();
       }
     };
-    for (int64_t base = first; more && ok; base += 32 * step) {
-      const int64_t job = base + lane * step;
-      const bool live = job < total;
+    for (int base = 0; more && ok; base += 32) {
+      const bool live = base + lane < n_row;
       int64_t row = -1, x_at = 0, dx_at = 0;
       int32_t target = -1;
       Token tk{};
       float xt = NAN, w = 0.f;
       if (live) {
-        row = a.list[job];
+        row = row_of(base + lane);
         x_at = a.in.at(row);
         dx_at = a.out.at(row);
         if (OBJ == kPolicy) {
@@ -1162,9 +1287,9 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
             xt = to_f((static_cast<const T*>(a.x) + x_at)[t]);
           }
           tk = load_token(a, row);
-          w = static_cast<float>(token_weight(a, row) * a.inv_tau);
+          w = static_cast<float>(token_weight(a, counts, row) * a.inv_tau);
         } else {
-          w = row_share(a);
+          w = row_share(a, counts);
         }
       }
       const int n = __popc(__ballot_sync(0xffffffffu, live));
@@ -1429,8 +1554,8 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
     ring_sync();
     double2 terms = make_double2(0.0, 0.0);
     if (rank == 0 && ok)
-      for (int64_t job = first + tid * step; job < total; job += kRingThreads * step) {
-        const double2 v = token_terms<OBJ>(a, a.list[job]);
+      for (int i = tid; i < n_row; i += kRingThreads) {
+        const double2 v = token_terms<OBJ>(a, counts, row_of(i));
         terms.x += v.x;
         terms.y += v.y;
       }
@@ -1465,6 +1590,7 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
   __shared__ TeacherSums s_t;
   const int tid = threadIdx.x;
   ptx::griddep_wait();
+  const Counts counts = listed_counts(a);
   const float factor = grad_factor(a);
   for (int64_t r = blockIdx.x; r < a.T; r += gridDim.x) {
     int64_t target = -1;
@@ -1489,14 +1615,14 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
     const float s = static_cast<float>(sd), inv_s = 1.f / s;
     float k;
     if (OBJ == kDistill) {
-      k = teacher_coef(s_t, row_share(a));
+      k = teacher_coef(s_t, row_share(a, counts));
       if (tid == 0) {
         if (s_t.bad) note_bad_index(a);
         a.row[r] = RowStat{m, s, s_t.t_sum, 0.f, s_t.about(m)};
       }
     } else {
       k = policy_coef<T>(a, load_token(a, r), xt, m, s,
-                      static_cast<float>(token_weight(a, r) * a.inv_tau));
+                      static_cast<float>(token_weight(a, counts, r) * a.inv_tau));
       if (tid == 0) {
         if (!ok) note_bad_index(a);
         a.row[r] = RowStat{m, s, xt, 0.f, 0.0};
@@ -1591,17 +1717,43 @@ template <int OBJ>
 __global__ void __launch_bounds__(kTokenThreads) token_kernel(RowArgs a) {
   __shared__ double2 red[kTokenThreads / 32], red2[kTokenThreads / 32];
   __shared__ bool s_last;
+  __shared__ int32_t s_seq[kSelfRows], s_total;
   ptx::griddep_wait();
-  const int64_t r = blockIdx.x * static_cast<int64_t>(kTokenThreads) + threadIdx.x;
+  Counts counts = listed_counts(a);
+  if (a.self_count) {  // one CTA
+    for (int b = threadIdx.x; b < kSelfRows; b += kTokenThreads) s_seq[b] = 0;
+    if (threadIdx.x == 0) s_total = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int r = threadIdx.x; r < a.T; r += kTokenThreads) {
+      int64_t target;
+      if (!row_counts(a, r, target)) continue;
+      atomicAdd(&s_total, 1);
+      if (a.per_sequence) atomicAdd(&s_seq[a.in.seq(r)], 1);
+    }
+    __syncthreads();
+    counts = Counts{s_total, s_seq};
+  }
   double2 v = make_double2(0.0, 0.0);
-  int64_t target;
-  if (r < a.T) {
-    if (row_counts(a, r, target))
-      v = token_terms<OBJ>(a, r);
-    else if (OBJ == kPolicy)
+  for (int64_t r = blockIdx.x * static_cast<int64_t>(kTokenThreads) + threadIdx.x; r < a.T;
+       r += gridDim.x * static_cast<int64_t>(kTokenThreads)) {
+    int64_t target;
+    if (row_counts(a, r, target)) {
+      const double2 t = token_terms<OBJ>(a, counts, r);
+      v.x += t.x;
+      v.y += t.y;
+    } else if (OBJ == kPolicy) {
       zero_outputs(a, r);
+    }
   }
   v = cta_sum<kTokenThreads / 32>(v, red);
+  if (a.self_count) {
+    if (threadIdx.x == 0) {
+      *a.loss = static_cast<float>(v.x);
+      if (a.kl) *a.kl = static_cast<float>(v.y);
+    }
+    return;
+  }
   if (last_to_write(a, v, &s_last)) sum_parts<kTokenThreads / 32>(a, gridDim.x, red2);
 }
 
@@ -1811,11 +1963,12 @@ int set_ws(RowArgs& a, void* ws, int64_t ws_bytes) {
 // Whole vectors that a row holds, at most.
 int max_vecs(const RowArgs& a, int x_f32) { return a.V / (x_f32 ? 4 : 8); }
 
-// A launch that may begin while the kernel before it on the stream still runs (every kernel
-// launched so waits for that one before it touches what it wrote), in clusters of cs CTAs.
+// A launch in clusters of cs CTAs. `after`: it may begin while the kernel of this call before it
+// on the stream still runs (every kernel launched so waits for that one before it touches
+// what it wrote).
 template <typename... P, typename... A>
-int launch_after(void (*kern)(P...), int64_t grid, int threads, int smem, int cs, cudaStream_t s,
-                 A... args) {
+int launch(bool after, void (*kern)(P...), int64_t grid, int threads, int smem, int cs,
+           cudaStream_t s, A... args) {
   if (grid > INT32_MAX) return set_error(LEMA_ERR_UNSUPPORTED, "too many rows");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
@@ -1824,7 +1977,7 @@ int launch_after(void (*kern)(P...), int64_t grid, int threads, int smem, int cs
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].val.programmaticStreamSerializationAllowed = after ? 1 : 0;
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = static_cast<unsigned>(cs);
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
@@ -1865,10 +2018,7 @@ int launch_logprobs_bwd_t(const RowArgs& a, int nvec, bool after, cudaStream_t s
   const int64_t per = kBwdThreads / g, grid = (a.T * chunks + per - 1) / per;
   if (grid > INT32_MAX) return set_error(LEMA_ERR_UNSUPPORTED, "too many rows");
   const auto kern = g == 32 ? logprobs_bwd_kernel<T, 32> : logprobs_bwd_kernel<T, kBwdThreads>;
-  if (after) return launch_after(kern, grid, kBwdThreads, 0, 1, s, a, chunks);
-  kern<<<static_cast<unsigned>(grid), kBwdThreads, 0, s>>>(a, chunks);
-  LEMA_CUDA_TRY(cudaGetLastError());
-  return LEMA_OK;
+  return launch(after, kern, grid, kBwdThreads, 0, 1, s, a, chunks);
 }
 
 // `after`: directly behind pair_kernel of the same call, which it may overlap.
@@ -1878,7 +2028,7 @@ int launch_logprobs_bwd(const RowArgs& a, int x_f32, bool after, cudaStream_t s)
                : launch_logprobs_bwd_t<__nv_bfloat16>(a, nvec, after, s);
 }
 
-constexpr int kRingSmem = 108 * 1024;  // two CTAs an SM
+constexpr int kRingSmem = 104 * 1024;  // two CTAs an SM
 
 template <typename Kern>
 int allow_smem(Kern kern, int bytes, std::atomic<uint64_t>& done) {
@@ -1916,8 +2066,16 @@ int resident_clusters(Kern kern, int cs, int smem, int* out) {
   return LEMA_OK;
 }
 
+int launch_count(const RowArgs& a, cudaStream_t s) {
+  const int64_t ctas = std::max<int64_t>(1, (a.T + kCountBlock - 1) / kCountBlock);
+  if (ctas > 1 && a.per_sequence) LEMA_CUDA_TRY(cudaMemsetAsync(a.seq_count, 0, a.n0 * 4, s));
+  count_kernel<<<static_cast<unsigned>(ctas), kCountThreads, 0, s>>>(a);
+  LEMA_CUDA_TRY(cudaGetLastError());
+  return LEMA_OK;
+}
+
 template <typename T, int OBJ>
-int launch_ring(const RowArgs& a, int cs, int per, cudaStream_t s) {
+int launch_ring(RowArgs a, int cs, int per, cudaStream_t s) {
   auto kern = ring_kernel<T, OBJ>;
   static std::atomic<uint64_t> done{0};
   int rc = allow_smem(kern, kRingSmem, done);
@@ -1930,8 +2088,11 @@ int launch_ring(const RowArgs& a, int cs, int per, cudaStream_t s) {
   int clusters = std::min<int>(2 * device_sm_count(), kMaxRing);
   if (cs > 1 && (rc = resident_clusters(kern, cs, smem, &clusters))) return rc;
   const int64_t n = std::min<int64_t>(a.T, std::min<int64_t>(clusters, kMaxRing / cs)) * cs;
-  rc = launch_after(kern, n, kRingThreads + 32, smem, cs, s, a, cs, per, stages);
-  return rc ? rc : launch_after(finish_kernel, 1, 256, 0, 1, s, a, static_cast<int>(n));
+  a.self_count = a.T <= kOwnTotal && a.T <= kOwnRows * (n / cs) &&
+                 (!a.per_sequence || a.n0 <= kOwnSeqs);
+  if (!a.self_count && (rc = launch_count(a, s))) return rc;
+  rc = launch(!a.self_count, kern, n, kRingThreads + 32, smem, cs, s, a, cs, per, stages);
+  return rc ? rc : launch(true, finish_kernel, 1, 256, 0, 1, s, a, static_cast<int>(n));
 }
 
 template <typename T, int OBJ, int G, int NV>
@@ -1942,16 +2103,21 @@ int launch_direct(const RowArgs& a, int64_t grid, int smem, cudaStream_t s) {
     const int rc = allow_smem(kern, kDirectThreads / G * kMaxTeacher * 12, done);
     if (rc) return rc;
   }
-  return launch_after(kern, grid, kDirectThreads, smem, 1, s, a);
+  return launch(!a.self_count, kern, grid, kDirectThreads, smem, 1, s, a);
 }
 
 // How a row is held, by the vectors it spans. kNv vectors are the 64 elements that a thread
-// keeps as fp32.
+// keeps as fp32. Sets self_count for token_kernel, or *done where it is not needed.
 template <typename T, int OBJ>
-int launch_rows(const RowArgs& a, int nvec, bool* done, cudaStream_t s) {
+int launch_rows(RowArgs& a, int nvec, bool* done, cudaStream_t s) {
   constexpr int kNv = 64 / Vec<T>::kE;
   const int teacher = a.K4 * 12;
   if (nvec <= 128 * kNv) {
+    a.self_count = a.T <= kSelfRows;
+    if (!a.self_count) {
+      const int rc = launch_count(a, s);
+      if (rc) return rc;
+    }
     const bool warps = nvec <= 32 * kNv;
     const int64_t per = warps ? kDirectThreads / 32 : 1, grid = (a.T + per - 1) / per;
     const int smem = static_cast<int>(per) * teacher;
@@ -1963,9 +2129,13 @@ int launch_rows(const RowArgs& a, int nvec, bool* done, cudaStream_t s) {
   }
   int cs = 1;
   while (cs < kMaxCluster && nvec > cs * kRingCap) cs *= 2;
-  if (nvec > cs * kRingCap)
-    return launch_after(stream_kernel<T, OBJ>, std::min<int64_t>(a.T, 2 * device_sm_count()),
-                        kRowThreads, teacher, 1, s, a);
+  if (nvec > cs * kRingCap) {
+    const int rc = launch_count(a, s);
+    return rc ? rc
+              : launch(true, stream_kernel<T, OBJ>,
+                       std::min<int64_t>(a.T, 2 * device_sm_count()), kRowThreads, teacher, 1, s,
+                       a);
+  }
   // few rows: spread each while SMs would be idle and every thread still has a vector
   while (cs < kMaxCluster && a.T * cs * 2 <= device_sm_count() &&
          nvec >= cs * 2 * kRingThreads)
@@ -1976,21 +2146,19 @@ int launch_rows(const RowArgs& a, int nvec, bool* done, cudaStream_t s) {
 
 // The list of rows, their statistics and gradients, the tokens' terms.
 template <int OBJ>
-int launch_loss(const RowArgs& a, int x_f32, cudaStream_t s) {
-  const int64_t ctas = std::max<int64_t>(1, (a.T + kCountBlock - 1) / kCountBlock);
-  if (ctas > 1 && a.per_sequence) LEMA_CUDA_TRY(cudaMemsetAsync(a.seq_count, 0, a.n0 * 4, s));
-  count_kernel<<<static_cast<unsigned>(ctas), kCountThreads, 0, s>>>(a);
-  LEMA_CUDA_TRY(cudaGetLastError());
+int launch_loss(RowArgs a, int x_f32, cudaStream_t s) {
   bool done = false;  // the tokens' terms are on their way
+  a.self_count = 1;
   if (a.T > 0) {
     const int nvec = max_vecs(a, x_f32);
+    a.self_count = 0;
     const int rc = x_f32 ? launch_rows<float, OBJ>(a, nvec, &done, s)
                          : launch_rows<__nv_bfloat16, OBJ>(a, nvec, &done, s);
     if (rc) return rc;
   }
   if (done) return LEMA_OK;
-  return launch_after(token_kernel<OBJ>, std::max<int64_t>(1, token_ctas(a.T)), kTokenThreads, 0,
-                      1, s, a);
+  const int64_t ctas = a.self_count ? 1 : token_ctas(a.T);
+  return launch(a.T > 0, token_kernel<OBJ>, ctas, kTokenThreads, 0, 1, s, a);
 }
 
 // Statistics are read and written as pairs.
@@ -2090,7 +2258,7 @@ extern "C" int lema_preference_loss(const void* x, int32_t x_f32, int64_t n0, in
   } else {
     LEMA_CUDA_TRY(cudaMemsetAsync(a.head, 0, sizeof(WsHead), s));
   }
-  if ((rc = launch_after(pair_kernel, n0 / 2, kPairThreads, 0, 1, s, a, n0 / 2, beta,
+  if ((rc = launch(true, pair_kernel, n0 / 2, kPairThreads, 0, 1, s, a, n0 / 2, beta,
                          label_smoothing, rewards)))
     return rc;
   if (dx == nullptr || a.T == 0) return LEMA_OK;
