@@ -1304,18 +1304,24 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
         const int nv = j < n ? max(0, min(per, sp.nvec - start)) : 0;
         const uint4* from = sp.vecs(x) + start;
         RowInfo* inf = &info[slot];
-        // at least one chunk, which brings the numbers
-        int c = 0;
-        do {
-          if (i >= stages) ok = ptx::mbar_wait(&empty[st], phase ^ 1u);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int m = min(kChunk, nv - c);
-          if (lane == 0 && m > 0) {
-            mbar_expect_tx(&full[st], m * 16u);
-            bulk_load(ring + st * kChunk, from + c, m * 16u, &full[st]);
+        // The first chunk brings the numbers, and there is one even without vectors. The copies
+        // for which there is room go out before the numbers are put together.
+        const int chunks = max(1, (nv + kChunk - 1) / kChunk);
+        const int st_row = st;
+        bool numbers = false;
+        for (int c = 0; c < chunks || !numbers; ++c) {
+          bool room = c < chunks && i < stages;
+          if (!room && c < chunks) {
+            room = numbers || c == 0 ? ptx::mbar_wait(&empty[st], phase ^ 1u)
+                                     : ptx::mbar_try_wait(&empty[st], phase ^ 1u);
+            room = __all_sync(0xffffffffu, room);
+            if (!room && (numbers || c == 0)) {
+              ok = false;
+              break;
+            }
           }
-          if (c == 0) {
+          if (!room) {
+            // all copies are out, or the next has to wait: the numbers
             if (j < n) {
               if (lane < kEdges) {
                 const int e = rank == 0 ? sp.edge(lane) : -1;
@@ -1347,15 +1353,25 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
               inf->tk = tk;
             }
             __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&full[st_row]);
+            numbers = true;
+            --c;  // this chunk again, with a wait
+            continue;
           }
-          if (lane == 0) ptx::mbar_arrive(&full[st]);
+          const int m = min(kChunk, nv - c * kChunk);
+          if (lane == 0) {
+            if (m > 0) {
+              mbar_expect_tx(&full[st], m * 16u);
+              bulk_load(ring + st * kChunk, from + c * kChunk, m * 16u, &full[st]);
+            }
+            if (c > 0) ptx::mbar_arrive(&full[st]);
+          }
           ++i;
           if (++st == stages) {
             st = 0;
             phase ^= 1u;
           }
-          c += kChunk;
-        } while (c < nv);
+        }
         slot = slot == stages ? 0 : slot + 1;
         ++done;
         if (n_zero > 0 && j < n)
