@@ -48,8 +48,8 @@ struct RowMap {
   }
 };
 
-// Workspace: head, counted rows of each sequence, the list of rows, partial sums of
-// token_kernel's CTAs, what each row leaves for it.
+// Workspace: head, counted rows of each sequence, the list of rows, partial sums, what each
+// row leaves for its token's terms (preference: its log-probability).
 struct WsHead {
   int64_t total;    // rows that count
   uint32_t ticket;  // CTAs of token_kernel or pair_kernel that are done
@@ -76,10 +76,10 @@ struct RowArgs {
   int64_t ignore;
   float* logps;                  // [T]
   float2* stats;                 // [T] (m, 1 / s), may be null
-  float* coef;                   // [T], may be null: dL/dlp (policy), row weight (distill)
+  float* coef;                   // [T] dL/dlp, may be null
   RowStat* row;                  // [T]
   double* lp64;                  // [T] log-probabilities (preference)
-  double2* part;                 // (loss, kl) of each CTA of token_kernel / of each pair
+  double2* part;                 // (loss, kl) of each CTA that adds tokens' terms, or pair
   void* dx;                      // null: no gradient
   RowMap out;
   float grad_scale;
@@ -105,13 +105,13 @@ struct RowArgs {
   int32_t K, K4;                 // entries a row, rounded up to four
   const uint8_t* mask;           // [T], may be null
   // backward from saved statistics
-  const float* g;                // [T] gradient of each row's log-probability (or row weight)
+  const float* g;                // [T] gradient of each row's log-probability
   const float* upstream;         // scalar, may be null
   int32_t zeros_done;            // the rows of zeros are written
   int32_t self_count;            // no count_kernel ran: CTAs count for themselves
 };
 
-enum Objective { kLogp = 0, kPolicy = 1, kDistill = 2 };
+enum Objective { kPolicy = 1, kDistill = 2 };
 
 __device__ __forceinline__ float ex2(float x) {
   float r;
@@ -175,7 +175,7 @@ struct Vec<float> {
   }
   static __device__ __forceinline__ float max_nan(const uint4& v) {
     return max_or_nan(max_or_nan(__uint_as_float(v.x), __uint_as_float(v.y)),
-                            max_or_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
+                      max_or_nan(__uint_as_float(v.z), __uint_as_float(v.w)));
   }
   static __device__ __forceinline__ uint4 pack(const uint64_t (&p)[2]) {
     float a, b, c, d;
@@ -246,7 +246,8 @@ __device__ __forceinline__ float whole_max(float m, float c) {
 }
 // 2^n for whole n <= 0.
 __device__ __forceinline__ float exp2_whole(float n) {
-  return n < -126.f ? 0.f : __uint_as_float(static_cast<uint32_t>(static_cast<int>(n) + 127) << 23);
+  if (n < -126.f) return 0.f;
+  return __uint_as_float(static_cast<uint32_t>(static_cast<int>(n) + 127) << 23);
 }
 __device__ __forceinline__ bool far_max(float m, float c) {
   return fabsf(m * c) > 2048.f && m != -INFINITY;
@@ -352,16 +353,6 @@ __device__ __forceinline__ F warp_sum(F v) {
   return v;
 }
 
-__device__ __forceinline__ double block_sum_d(double v, double* red) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double r = red[0];
-  for (int w = 1; w < static_cast<int>(blockDim.x >> 5); ++w) r += red[w];
-  return r;
-}
-
 // Barrier of a group of G threads: a warp, or the whole CTA.
 template <int G>
 __device__ __forceinline__ void group_sync() {
@@ -391,7 +382,8 @@ __device__ __forceinline__ void group_combine(float& m, double& s, const RowArgs
   // a thread that saw only -inf adds nothing
   const bool far = !WHOLE || far_max(m, a.c);
   const float n = whole_max(m, a.c);
-  const float f = far || far_max(mt, a.c) ? ex2((mt - m) * a.c) : exp2_whole(whole_max(mt, a.c) - n);
+  const float f = far || far_max(mt, a.c) ? ex2((mt - m) * a.c)
+                                          : exp2_whole(whole_max(mt, a.c) - n);
   s *= mt == -INFINITY ? 0.0 : static_cast<double>(f);
   s = warp_sum(s);
   if (G > 32) {
@@ -733,7 +725,8 @@ __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
     if (!ok) atomicMax(a.err, static_cast<int32_t>(kDevErrIndex));
     a.logps[r] = static_cast<float>(lp);
     if (a.lp64) a.lp64[r] = lp;
-    if (a.stats) a.stats[r] = make_float2(m, static_cast<float>(1.0 / s) * expf(static_cast<float>(-up)));
+    if (a.stats)
+      a.stats[r] = make_float2(m, static_cast<float>(1.0 / s) * expf(static_cast<float>(-up)));
   }
 }
 
@@ -1403,6 +1396,12 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
 #pragma unroll
       for (int c = 0; c < kRingVecs / kChunkVecs; ++c) {
         if (c == 0 || c * kChunk < nv) {
+          if (OBJ == kDistill && c >= stages) {
+            // many teacher entries leave a ring shorter than the row: this chunk takes the
+            // stage of one of the same row, which has to be free first
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(&empty[st]);
+          }
           if (c > 0) ok = ptx::mbar_wait(&full[st], phase) && ok;
           const uint4* buf = ring + st * kChunk + tid;
 #pragma unroll
@@ -1425,10 +1424,10 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
       float m = xe;
 #pragma unroll
       for (int j = 0; j < kRingVecs; ++j) m = fmaxf(m, Vec<T>::max(w[j]));
-      // every lane has its part of the chunks
+      // every lane has its part of the chunks: those still in the ring are free
       __syncwarp();
       if (lane == 0)
-        for (int c = 0, e = st_row; c == 0 || c * kChunk < nv; ++c) {
+        for (int c = 0, e = st_row; c < stages && (c == 0 || c * kChunk < nv); ++c) {
           ptx::mbar_arrive(&empty[e]);
           if (++e == stages) e = 0;
         }
@@ -1638,7 +1637,7 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
       }
     } else {
       k = policy_coef<T>(a, load_token(a, r), xt, m, s,
-                      static_cast<float>(token_weight(a, counts, r) * a.inv_tau));
+                         static_cast<float>(token_weight(a, counts, r) * a.inv_tau));
       if (tid == 0) {
         if (!ok) note_bad_index(a);
         a.row[r] = RowStat{m, s, xt, 0.f, 0.0};
@@ -2096,6 +2095,7 @@ int launch_ring(RowArgs a, int cs, int per, cudaStream_t s) {
   static std::atomic<uint64_t> done{0};
   int rc = allow_smem(kern, kRingSmem, done);
   if (rc) return rc;
+  // 9 stages without a teacher, 3 at its most entries, fewer than a row may have chunks
   int stages = kMaxStages, smem = 0;
   for (;; --stages) {
     smem = kZeroBytes + stages * kChunk * 16 + (stages + 1) * a.K4 * 12;

@@ -57,14 +57,14 @@ def check_logps(got, want, V):
     assert (err <= rel_s(V) + U * want.abs()).all(), err.max().item()
 
 
-def check_dx(got, x, q, k, mass, tau=1.0):
+def check_dx(got, x, q, k, mass, tau=1.0, mass_err=2 * U):
     """got = k (mass - q): k [rows] fp64, mass the row's point masses."""
     k = k[..., None]
     want = k * (mass - q)
     a_max = (x.double().amax(-1) - torch.where(x.isinf(), 0.0, x.double()).amin(-1)).max().item() \
         / tau * 1.4427
     rel_q = rel_s(x.shape[-1]) + (4 + 2.1 * min(a_max, 150.0)) * U
-    tol = (half_step(got.dtype) + 8 * U) * want.abs() + k.abs() * (q * rel_q + 2 * U * mass) + 1e-37
+    tol = (half_step(got.dtype) + 8 * U) * want.abs() + k.abs() * (q * rel_q + mass_err * mass) + 1e-37
     err = (got.double() - want).abs()
     assert (err <= tol).all(), (err - tol).max().item()
 
@@ -691,3 +691,89 @@ def test_many_rows(cuda_device, B, S, V, dtype):
         check_dx(dxd[b:b + 1], x[b:b + 1], q, kd * share, mass)
     assert abs(loss.item() - want) <= 4 * U * adv.abs().mean().item() + 2 * U * abs(want)
     assert abs(lossd.item() - wantd) <= rel_s(V) + 60 * U + 2 * U * abs(wantd)
+
+
+@pytest.mark.parametrize("B,S,V", [(600, 20, 300), (600, 15, 8500), (30, 30, 9001), (2, 3, 40000)])
+def test_many_sequences(cuda_device, B, S, V):
+    """Means over each sequence's tokens, whose counts differ, at row counts listed by one
+    CTA, by several and by every CTA for itself; sequences without a counted token."""
+    x, t, g = make(cuda_device, B, S, V, "bf16", ignore=0.4)
+    t[B // 2] = IGN
+    adv = torch.randn(B, S, device=x.device, generator=g)
+    loss, lps, _, dx = ops.policy_loss_grad(x, t, None, adv, reduction="sequence")
+    n = (t != IGN).sum(1, keepdim=True)
+    w = torch.where(t == IGN, 0.0, 1.0 / (B * n.clamp(min=1).double()))
+    want = -(w * adv.double()).sum().item()
+    assert abs(loss.item() - want) <= 2 * U * abs(want) + 1e-12
+    for b in range(0, B, 50):
+        e = min(B, b + 50)
+        lp, q = ref_logps(x[b:e], t[b:e])
+        check_logps(lps[b:e], lp, V)
+        check_dx(dx[b:e], x[b:e], q, -w[b:e] * adv[b:e].double(), onehot(t[b:e], V))
+    again = ops.policy_loss_grad(x, t, None, adv, reduction="sequence")
+    assert torch.equal(again[0], loss) and torch.equal(again[3], dx)
+
+
+@pytest.mark.parametrize("V", [9001, 40000, 300001])
+def test_long_rows_in_graphs(cuda_device, V):
+    """Captured and replayed on other inputs: rows held by one CTA, by clusters, and swept."""
+    dev = cuda_device
+    data = [make(dev, 4, 9, V, "bf16", seed=s) for s in range(2)]
+    tl = [torch.topk(x.float(), 40, -1) for x, _, _ in data]
+    adv = torch.randn(4, device=dev)
+
+    def all_of(x, t, v, i):
+        return (*ops.policy_loss_grad(x, t, None, adv, reduction="sequence"),
+                *ops.preference_loss_grad(x, t), *ops.distill_loss_grad(x, i, v, t != IGN))
+    want = [all_of(x, t, v, i) for (x, t, _), (v, i) in zip(data, tl)]
+    bufs = [data[0][0].clone(), data[0][1].clone(), tl[0][0].clone(), tl[0][1].clone()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = all_of(*bufs)
+    for k in (1, 0, 1):
+        for b, src in zip(bufs, (data[k][0], data[k][1], tl[k][0], tl[k][1])):
+            b.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, w in zip(got, want[k]):
+            assert torch.equal(a, w)
+
+
+def test_most_teacher_entries_on_long_rows(cuda_device):
+    """Entries that leave little room beside rows that fill a CTA and a cluster; each index
+    twice."""
+    for S, V, K in ((70, 32000, 512), (310, 32000, 512), (310, 32000, 300), (310, 20000, 220),
+                    (70, 70000, 512), (5, 100000, 512), (3, 250001, 512), (310, 9001, 512)):
+        x, _, _ = make(cuda_device, 1, S, V, "bf16")
+        val, ids = torch.topk(x.float(), K, -1)
+        ids, val = torch.cat([ids, ids.flip(-1)], -1), torch.cat([val, val.flip(-1) - 1], -1)
+        loss, dx = ops.distill_loss_grad(x, ids, val)
+        want, k, mass, q = ref_distill(x, ids, val, None, 1.0)
+        # A weight is off by 7 u (its exponent spans less than 7), 2 u (ex2), 37 u (the sum of
+        # 32 a lane and of the lanes) and 2 u (the division and the sum of two): 48 u. The terms
+        # p (log p - log q) take that times |log p - log q| < 2 or so, and 9 u of log p.
+        assert abs(loss.item() - want.item()) <= rel_s(V) + 110 * U + 2 * U * abs(want.item())
+        check_dx(dx, x, q, k, mass, mass_err=48 * U)
+
+
+@pytest.mark.parametrize("V", [5000, 9001, 70000])
+def test_far_rows(cuda_device, V):
+    """Logits and temperatures whose exponents leave the range of one reference, in rows kept
+    as exponentials, held by one CTA and shared by several."""
+    g = torch.Generator(device=cuda_device).manual_seed(V)
+    for dtype in (torch.bfloat16, torch.float32):
+        for lift, tau in ((0.0, 1e-3), (3e4, 1.0), (-3e4, 1.0), (30.0, 100.0), (1e30, 1.0)):
+            x = torch.randn(1, 6, V, device=cuda_device, generator=g)
+            # steps that the lifted values keep, the top of them a few apart
+            x = (x.round() * (max(lift * lift, 1.0) ** 0.5 / 128 if lift else 1.0) + lift).to(dtype)
+            t = torch.stack([x[0].float().argmax(-1), x[0].float().argmin(-1)], -1)[None]
+            t = torch.where(torch.arange(6, device=x.device) % 2 == 0, t[..., 0], t[..., 1])
+            adv = torch.ones(1, 6, device=x.device)
+            loss, lps, _, dx = ops.policy_loss_grad(x, t, None, adv, temperature=tau)
+            lp, q = ref_logps(x, t, tau)
+            # the difference of two values, times 1 / tau, is rounded thrice
+            tol = rel_s(V) + 12 * U + 4 * U * lp.abs()
+            assert ((lps.double() - lp).abs() <= tol).all()
+            # k = -1/6/tau (mass - q); the bound on q counts exponents up to 150
+            check_dx(dx, x, q, torch.full((1, 6), -1 / 6 / tau, dtype=torch.float64,
+                                          device=x.device), onehot(t, V), tau)
