@@ -17,6 +17,11 @@ repetitions), printing one JSON line per case.
         unaligned rows (4096 x 4100), the device-error snapshot; ``once``
         launches each (plus a GQA attention backward for its delta and dK/dV
         reduce kernels) a single time, untimed, for an ncu capture
+    python -m lema_b200.kernel_bench losses
+        the losses over vocabulary logits (log-probabilities, preference, clipped
+        policy, distillation with their gradients) at the training batch, at short
+        rows and at rows longer than a cluster holds; GB/s over the counted rows
+        read once and every gradient row written once
 """
 from __future__ import annotations
 
@@ -179,14 +184,41 @@ def misc(once: bool) -> None:
         torch.cuda.synchronize()
 
 
+def losses() -> None:
+    dev = torch.device("cuda:0")
+    flush = torch.empty(512 << 20, dtype=torch.uint8, device=dev)
+    for B, S, V, dtype in ((8, 512, 32000, torch.bfloat16), (8, 2048, 4096, torch.bfloat16),
+                           (32, 2048, 512, torch.bfloat16), (4, 256, 32000, torch.float32),
+                           (4, 256, 300000, torch.bfloat16)):
+        x = (2 * torch.randn(B, S, V, device=dev)).to(dtype)
+        t = torch.randint(0, V, (B, S), device=dev)
+        t[:, :S // 4] = -100                      # prompts
+        adv = torch.randn(B, device=dev)
+        val, idx = torch.topk(x[..., :256].float(), 64, -1)
+        once, both = (t != -100).sum().item() * V * x.element_size(), B * S * V * x.element_size()
+        for name, fn, nbytes in (
+                ("token_logprobs", lambda: ops.token_logprobs(x, t), once),
+                ("preference_loss_grad", lambda: ops.preference_loss_grad(x, t), once + both),
+                ("policy_loss_grad", lambda: ops.policy_loss_grad(x, t, None, adv), once + both),
+                ("distill_loss_grad", lambda: ops.distill_loss_grad(x, idx, val, t != -100),
+                 once + both)):
+            us = _time_us(fn, 9, flush)
+            print(json.dumps({"case": f"{name} {B} x {S} x {V} {str(dtype)[6:]}",
+                              "us": round(us, 1), "GBps": round(nbytes / us / 1e3, 1),
+                              "bytes": nbytes}), flush=True)
+        del x, t, val, idx
+
+
 def main(argv: list[str]) -> None:
-    if not argv or argv[0] not in ("attention", "producers", "misc"):
+    if not argv or argv[0] not in ("attention", "producers", "misc", "losses"):
         raise SystemExit("usage: python -m lema_b200.kernel_bench "
-                         "{attention [small | long] | producers | misc [once]}")
+                         "{attention [small | long] | producers | misc [once] | losses}")
     if argv[0] == "attention":
         attention(argv[1] if len(argv) > 1 else "")
     elif argv[0] == "producers":
         producers()
+    elif argv[0] == "losses":
+        losses()
     else:
         misc(len(argv) > 1 and argv[1] == "once")
     if _native.device_error() != 0:
