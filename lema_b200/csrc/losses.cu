@@ -1591,8 +1591,13 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
 
 // ---- rows too long for a cluster -----------------------------------------------------
 
-// One CTA a row, swept twice; the second sweep finds it in L2.
-constexpr int kRowThreads = 512;
+// One CTA a row, swept twice; the second sweep goes from the row's end, which is in L2 still,
+// back to its start. One CTA an SM: its rows of up to 0.8 MB fit in L2 together, those of two do
+// not. Bound by the latency of its reads, four 16-byte loads a thread: 768 rows of 300000 bf16
+// that count and 256 of zeros (1.08 GB with the gradient) take 305 us, 3.5 TB/s of what has to
+// move; two CTAs an SM of half the threads 316 us, a second sweep forwards with one load a
+// thread 407 us.
+constexpr int kRowThreads = 1024;
 template <typename T, int OBJ>
 __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
   constexpr int E = Vec<T>::kE;
@@ -1655,17 +1660,27 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
       const uint64_t kq2 = f2_splat(kq * ks.fix);
       const uint4* xv = sp.vecs(x);
       uint4* dv = reinterpret_cast<uint4*>(dx + sp.head);
-      for (int v = tid; v < sp.nvec; v += kRowThreads) {
-        uint64_t e[E / 2];
-        uint4 w = ld16(xv + v);
-        if (far) shift_vec<T>(w, m);
-        exp_vec<T>(w, ks, e);
+      constexpr int U = 4, kStep = U * kRowThreads;
+      for (int base = (sp.nvec - 1) / kStep * kStep + tid; base >= 0; base -= kStep) {
+        uint4 w[U];
 #pragma unroll
-        for (int i = 0; i < E / 2; ++i) e[i] = f2_mul(e[i], kq2);
-        if (same)
-          dv[v] = Vec<T>::pack(e);
-        else
-          store_apart<T>(dx + sp.head + static_cast<int64_t>(v) * E, Vec<T>::pack(e));
+        for (int u = 0; u < U; ++u)
+          if (base + u * kRowThreads < sp.nvec) w[u] = ld16(xv + base + u * kRowThreads);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int v = base + u * kRowThreads;
+          if (far) shift_vec<T>(w[u], m);
+          uint64_t e[E / 2];
+          exp_vec<T>(w[u], ks, e);
+#pragma unroll
+          for (int i = 0; i < E / 2; ++i) e[i] = f2_mul(e[i], kq2);
+          if (v < sp.nvec) {
+            if (same)
+              __stcs(dv + v, Vec<T>::pack(e));
+            else
+              store_apart<T>(dx + sp.head + static_cast<int64_t>(v) * E, Vec<T>::pack(e));
+          }
+        }
       }
       if (edge >= 0) put(dx + edge, ex2((xe - m) * a.c) * kq);
       if (OBJ == kPolicy) {
@@ -2149,7 +2164,7 @@ int launch_rows(RowArgs& a, int nvec, bool* done, cudaStream_t s) {
     const int rc = launch_count(a, s);
     return rc ? rc
               : launch(true, stream_kernel<T, OBJ>,
-                       std::min<int64_t>(a.T, 2 * device_sm_count()), kRowThreads, teacher, 1, s,
+                       std::min<int64_t>(a.T, device_sm_count()), kRowThreads, teacher, 1, s,
                        a);
   }
   // few rows: spread each while SMs would be idle and every thread still has a vector
