@@ -540,95 +540,115 @@ __device__ __forceinline__ F policy_token(const RowArgs& a, const Token& tk, F l
 // ---- kernels ---------------------------------------------------------------------
 
 // Lists the rows that enter the loss in their order (list[0 .. total)), then the others from the
-// end backwards, counts them for each sequence, and clears the ticket. A CTA lists kCountBlock
-// rows, after it has counted those in front of them by itself: the list's order, and with it
-// the order of every sum, is always the same. (seq_count is cleared before when there are
-// several CTAs.)
+// end backwards, counts them for each sequence, and clears the ticket. The CTAs of one cluster
+// count `chunk` rows each, add up the counts in front of their own and list theirs. The list's order, and
+// with it the order of every sum, is always the same. Two passes over the targets,
+// bound by their latency: 7.7 us at 16384 rows and 9.1 us at 65536 (CTAs that recount the rows
+// in front of theirs: 9.0 us and 19.7 us).
 constexpr int kCountThreads = 1024;
 constexpr int kCountRows = 8;
 constexpr int kCountBlock = kCountThreads * kCountRows;
-__global__ void __launch_bounds__(kCountThreads) count_kernel(RowArgs a) {
+constexpr int kCountCluster = 8;
+__global__ void __launch_bounds__(kCountThreads) count_kernel(RowArgs a, int32_t chunk) {
   constexpr int kCells = kCountRows * kCountThreads / 32;  // a warp's rows at one offset
   __shared__ int32_t s_cell[kCells];
-  __shared__ int32_t s_before;
+  __shared__ int32_t s_sum, s_end, s_cta[kCountCluster];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = blockIdx.x, ctas = gridDim.x;  // one cluster
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int64_t r0 = blockIdx.x * int64_t{kCountBlock};
+  const int64_t r0 = static_cast<int64_t>(rank) * chunk, r1 = min(a.T, r0 + chunk);
   bool in[kCountRows];
+  const auto load = [&](int64_t at) {
 #pragma unroll
-  for (int j = 0; j < kCountRows; ++j) {
-    const int64_t r = r0 + j * kCountThreads + tid;
-    int64_t target;
-    in[j] = r < a.T && row_counts(a, r, target);
-  }
+    for (int j = 0; j < kCountRows; ++j) {
+      const int64_t r = at + j * kCountThreads + tid;
+      int64_t target;
+      in[j] = r < r1 && row_counts(a, r, target);
+    }
+  };
   if (tid == 0) {
-    s_before = 0;
-    if (blockIdx.x == 0) a.head->ticket = 0;
+    s_sum = 0;
+    if (rank == 0) a.head->ticket = 0;
   }
-  if (a.per_sequence && gridDim.x == 1)
-    for (int64_t b = tid; b < a.n0; b += kCountThreads) a.seq_count[b] = 0;
-  __syncthreads();
-  if (r0 > 0) {
+  if (a.per_sequence)
+    for (int64_t b = rank * kCountThreads + tid; b < a.n0; b += ctas * kCountThreads)
+      a.seq_count[b] = 0;
+  int before = 0;
+  if (ctas > 1) {
     int n = 0;
-    for (int64_t q0 = 0; q0 < r0; q0 += kCountBlock) {
-      bool was[kCountRows];
+    for (int64_t at = r0; at < r1; at += kCountBlock) {
+      load(at);
 #pragma unroll
-      for (int j = 0; j < kCountRows; ++j) {
-        int64_t target;
-        was[j] = row_counts(a, q0 + j * kCountThreads + tid, target);
-      }
-#pragma unroll
-      for (int j = 0; j < kCountRows; ++j) n += was[j];
+      for (int j = 0; j < kCountRows; ++j) n += in[j];
     }
     n = __reduce_add_sync(0xffffffffu, n);
-    if (lane == 0) atomicAdd(&s_before, n);
+    __syncthreads();
+    if (lane == 0) atomicAdd(&s_sum, n);
+    __syncthreads();
+    if (tid < ctas)
+      asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(
+                       ptx::mapa_shared(ptx::smem_u32(&s_cta[rank]), tid)),
+                   "r"(s_sum)
+                   : "memory");
+    ptx::cluster_sync();
+    for (int j = 0; j < rank; ++j) before += s_cta[j];
+  } else {
+    load(r0);
+    __syncthreads();
   }
-  uint32_t ballot[kCountRows];
+  for (int64_t at = r0; at < r1; at += kCountBlock) {
+    if (chunk > kCountBlock) load(at);
+    uint32_t ballot[kCountRows];
 #pragma unroll
-  for (int j = 0; j < kCountRows; ++j) {
-    ballot[j] = __ballot_sync(0xffffffffu, in[j]);
-    if (lane == 0) s_cell[j * 32 + warp] = __popc(ballot[j]);
-    if (a.per_sequence) {
-      const int64_t r = r0 + j * kCountThreads + tid, b = a.in.seq(r);
-      // a warp inside one sequence adds once
-      const bool one = __all_sync(0xffffffffu, __shfl_sync(0xffffffffu, b, 0) == b);
-      if (one ? lane == 0 && ballot[j] != 0 : in[j])
-        atomicAdd(&a.seq_count[b], one ? __popc(ballot[j]) : 1);
+    for (int j = 0; j < kCountRows; ++j) {
+      ballot[j] = __ballot_sync(0xffffffffu, in[j]);
+      if (lane == 0) s_cell[j * 32 + warp] = __popc(ballot[j]);
+      if (a.per_sequence) {
+        const int64_t b = a.in.seq(min(at + j * kCountThreads + tid, a.T - 1));
+        // a warp inside one sequence adds once
+        const bool one = __all_sync(0xffffffffu, __shfl_sync(0xffffffffu, b, 0) == b);
+        if (one ? lane == 0 && ballot[j] != 0 : in[j])
+          atomicAdd(&a.seq_count[b], one ? __popc(ballot[j]) : 1);
+      }
     }
+    __syncthreads();
+    if (warp == 0) {
+      int n[kCells / 32], sum = 0;
+#pragma unroll
+      for (int j = 0; j < kCells / 32; ++j) {
+        n[j] = s_cell[lane * (kCells / 32) + j];
+        sum += n[j];
+      }
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += up;
+      }
+      int rank_of = before + incl - sum;
+#pragma unroll
+      for (int j = 0; j < kCells / 32; ++j) {
+        s_cell[lane * (kCells / 32) + j] = rank_of;
+        rank_of += n[j];
+      }
+      if (lane == 31) s_end = rank_of;
+    }
+    __syncthreads();
+    before = s_end;
+#pragma unroll
+    for (int j = 0; j < kCountRows; ++j) {
+      const int64_t r = at + j * kCountThreads + tid;
+      // counted rows in front of r
+      const int64_t rank_of = s_cell[j * 32 + warp] + __popc(ballot[j] & ((1u << lane) - 1u));
+      if (in[j])
+        a.list[rank_of] = static_cast<int32_t>(r);
+      else if (r < r1)
+        a.list[a.T - 1 - (r - rank_of)] = static_cast<int32_t>(r);
+    }
+    __syncthreads();
   }
-  __syncthreads();
-  if (warp == 0) {
-    int n[kCells / 32], sum = 0;
-#pragma unroll
-    for (int j = 0; j < kCells / 32; ++j) {
-      n[j] = s_cell[lane * (kCells / 32) + j];
-      sum += n[j];
-    }
-    int incl = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += up;
-    }
-    int at = s_before + incl - sum;
-#pragma unroll
-    for (int j = 0; j < kCells / 32; ++j) {
-      s_cell[lane * (kCells / 32) + j] = at;
-      at += n[j];
-    }
-    if (lane == 31 && blockIdx.x == gridDim.x - 1) a.head->total = at;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int j = 0; j < kCountRows; ++j) {
-    const int64_t r = r0 + j * kCountThreads + tid;
-    // counted rows in front of r
-    const int64_t rank = s_cell[j * 32 + warp] + __popc(ballot[j] & ((1u << lane) - 1u));
-    if (in[j])
-      a.list[rank] = static_cast<int32_t>(r);
-    else if (r < a.T)
-      a.list[a.T - 1 - (r - rank)] = static_cast<int32_t>(r);
-  }
+  // the last of them have no rows when there are few
+  if (rank == ctas - 1 && tid == 0) a.head->total = before;
 }
 
 // Few rows are counted by each CTA that needs the numbers, which saves the launch of
@@ -689,10 +709,12 @@ __device__ __forceinline__ void zero_row(const RowArgs& a, int64_t r, int tid) {
   if (tid < kEdges && so.edge(tid) >= 0) put(dx + so.edge(tid), 0.f);
 }
 
-// token_logprobs: a group of G threads a row, a warp for short rows (one CTA a row leaves most
-// of its threads without a vector there).
+// token_logprobs: a group of G threads a row, U vectors of a thread in flight. Long rows are bound
+// by DRAM's reads (4096 x 32000 bf16, three quarters of them counted: 36 us, 5.5 TB/s), short
+// ones by the latency of a row's chain of loads and reductions (65536 x 512: 26 us, 1.9 TB/s).
+// Several rows for each group, their targets loaded and logarithms taken together, gave nothing.
 constexpr int kStatThreads = 128;
-template <typename T, int G, bool WHOLE>
+template <typename T, int G, bool WHOLE, int U>
 __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
   __shared__ float redf[kStatThreads / 32];
   __shared__ double redd[kStatThreads / 32];
@@ -715,7 +737,7 @@ __global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
   const Span<T> sp(x, a.V);
   float m;
   double s;
-  thread_stats<T, G, 8, WHOLE>(x, sp, tid, a.c, a.c_lo, m, s);
+  thread_stats<T, G, U, WHOLE>(x, sp, tid, a.c, a.c_lo, m, s);
   group_combine<G, WHOLE>(m, s, a, redf, redd);
   if (tid == 0) {
     const double up = WHOLE ? about_max(m, a) : 0.0, log_s = log(s) + up;
@@ -2020,18 +2042,24 @@ int launch(bool after, void (*kern)(P...), int64_t grid, int threads, int smem, 
 // A warp a row while four vectors a lane hold it.
 bool warp_rows(int nvec) { return nvec <= 128; }
 
-template <typename T, bool WHOLE>
-int launch_logprobs_t(const RowArgs& a, int nvec, cudaStream_t s) {
-  if (warp_rows(nvec)) {
-    const int64_t per = kStatThreads / 32;
-    logprobs_kernel<T, 32, WHOLE>
-        <<<static_cast<unsigned>((a.T + per - 1) / per), kStatThreads, 0, s>>>(a);
-  } else {
-    logprobs_kernel<T, kStatThreads, WHOLE>
-        <<<static_cast<unsigned>(a.T), kStatThreads, 0, s>>>(a);
-  }
+template <typename T, int G, bool WHOLE, int U>
+int launch_logprobs_g(const RowArgs& a, cudaStream_t s) {
+  constexpr int64_t kRows = kStatThreads / G;
+  logprobs_kernel<T, G, WHOLE, U>
+      <<<static_cast<unsigned>((a.T + kRows - 1) / kRows), kStatThreads, 0, s>>>(a);
   LEMA_CUDA_TRY(cudaGetLastError());
   return LEMA_OK;
+}
+
+// As many vectors in flight as a thread has, 8 at most: with 8 for all, 65536 rows of 512 bf16
+// took 47 us instead of 26 and 16384 of 4096 took 44 instead of 31, most of their exponentials
+// those of absent vectors.
+template <typename T, bool WHOLE>
+int launch_logprobs_t(const RowArgs& a, int nvec, cudaStream_t s) {
+  if (nvec <= 32 * 2) return launch_logprobs_g<T, 32, WHOLE, 2>(a, s);
+  if (warp_rows(nvec)) return launch_logprobs_g<T, 32, WHOLE, 4>(a, s);
+  if (nvec <= kStatThreads * 4) return launch_logprobs_g<T, kStatThreads, WHOLE, 4>(a, s);
+  return launch_logprobs_g<T, kStatThreads, WHOLE, 8>(a, s);
 }
 
 template <bool WHOLE>
@@ -2097,11 +2125,10 @@ int resident_clusters(Kern kern, int cs, int smem, int* out) {
 }
 
 int launch_count(const RowArgs& a, cudaStream_t s) {
-  const int64_t ctas = std::max<int64_t>(1, (a.T + kCountBlock - 1) / kCountBlock);
-  if (ctas > 1 && a.per_sequence) LEMA_CUDA_TRY(cudaMemsetAsync(a.seq_count, 0, a.n0 * 4, s));
-  count_kernel<<<static_cast<unsigned>(ctas), kCountThreads, 0, s>>>(a);
-  LEMA_CUDA_TRY(cudaGetLastError());
-  return LEMA_OK;
+  const int ctas = a.T > kCountThreads ? kCountCluster : 1;
+  const int64_t warps = (a.T + 32 * ctas - 1) / (32 * ctas);  // of rows, for each CTA
+  return launch(false, count_kernel, ctas, kCountThreads, 0, ctas, s, a,
+                static_cast<int32_t>(warps * 32));
 }
 
 template <typename T, int OBJ>
