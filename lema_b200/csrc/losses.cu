@@ -541,8 +541,8 @@ __device__ __forceinline__ F policy_token(const RowArgs& a, const Token& tk, F l
 
 // Lists the rows that enter the loss in their order (list[0 .. total)), then the others from the
 // end backwards, counts them for each sequence, and clears the ticket. The CTAs of one cluster
-// count `chunk` rows each, add up the counts in front of their own and list theirs. The list's order, and
-// with it the order of every sum, is always the same. Two passes over the targets,
+// count `chunk` rows each, add up the counts in front of their own and list theirs. The list's
+// order, and with it the order of every sum, is always the same. Two passes over the targets,
 // bound by their latency: 7.7 us at 16384 rows and 9.1 us at 65536 (CTAs that recount the rows
 // in front of theirs: 9.0 us and 19.7 us).
 constexpr int kCountThreads = 1024;
@@ -2317,7 +2317,7 @@ extern "C" int lema_preference_loss(const void* x, int32_t x_f32, int64_t n0, in
     LEMA_CUDA_TRY(cudaMemsetAsync(a.head, 0, sizeof(WsHead), s));
   }
   if ((rc = launch(true, pair_kernel, n0 / 2, kPairThreads, 0, 1, s, a, n0 / 2, beta,
-                         label_smoothing, rewards)))
+                   label_smoothing, rewards)))
     return rc;
   if (dx == nullptr || a.T == 0) return LEMA_OK;
   a.g = coef;
@@ -2330,8 +2330,8 @@ extern "C" int lema_policy_loss(const void* x, int32_t x_f32, int64_t n0, int64_
                                 int64_t ld1, int64_t V, const int64_t* targets,
                                 int64_t ignore_index, double temperature, const float* old_logps,
                                 const float* advantages, int64_t adv_s0, int64_t adv_s1,
-                                const float* ref_logps, double clip_lo,
-                                double clip_hi, double kl_coef, int32_t per_sequence, double grad_scale, void* ws,
+                                const float* ref_logps, double clip_lo, double clip_hi,
+                                double kl_coef, int32_t per_sequence, double grad_scale, void* ws,
                                 int64_t ws_bytes, float* logps, float* stats, float* coef,
                                 float* loss, float* kl, void* dx, int64_t ldd0, int64_t ldd1,
                                 void* stream) {

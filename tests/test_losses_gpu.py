@@ -64,7 +64,8 @@ def check_dx(got, x, q, k, mass, tau=1.0, mass_err=2 * U):
     a_max = (x.double().amax(-1) - torch.where(x.isinf(), 0.0, x.double()).amin(-1)).max().item() \
         / tau * 1.4427
     rel_q = rel_s(x.shape[-1]) + (4 + 2.1 * min(a_max, 150.0)) * U
-    tol = (half_step(got.dtype) + 8 * U) * want.abs() + k.abs() * (q * rel_q + mass_err * mass) + 1e-37
+    tol = ((half_step(got.dtype) + 8 * U) * want.abs()
+           + k.abs() * (q * rel_q + mass_err * mass) + 1e-37)
     err = (got.double() - want).abs()
     assert (err <= tol).all(), (err - tol).max().item()
 
