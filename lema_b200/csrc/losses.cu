@@ -1202,7 +1202,8 @@ __device__ __forceinline__ int list_own(const RowArgs& a, uint32_t first, uint32
   return before;
 }
 
-template <typename T, int OBJ>
+// SHORT: fewer stages than a row may have chunks, for many teacher entries.
+template <typename T, int OBJ, bool SHORT>
 __global__ void __launch_bounds__(kRingThreads + 32, 2)
     ring_kernel(RowArgs a, int cs, int per, int stages) {
   constexpr int E = Vec<T>::kE;
@@ -1418,9 +1419,8 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
 #pragma unroll
       for (int c = 0; c < kRingVecs / kChunkVecs; ++c) {
         if (c == 0 || c * kChunk < nv) {
-          if (OBJ == kDistill && c >= stages) {
-            // many teacher entries leave a ring shorter than the row: this chunk takes the
-            // stage of one of the same row, which has to be free first
+          if (SHORT && c >= stages) {
+            // this chunk takes the stage of one of the same row, which has to be free first
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(&empty[st]);
           }
@@ -1449,7 +1449,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
       // every lane has its part of the chunks: those still in the ring are free
       __syncwarp();
       if (lane == 0)
-        for (int c = 0, e = st_row; c < stages && (c == 0 || c * kChunk < nv); ++c) {
+        for (int c = 0, e = st_row; (!SHORT || c < stages) && (c == 0 || c * kChunk < nv); ++c) {
           ptx::mbar_arrive(&empty[e]);
           if (++e == stages) e = 0;
         }
@@ -2087,6 +2087,9 @@ int launch_logprobs_bwd(const RowArgs& a, int x_f32, bool after, cudaStream_t s)
 }
 
 constexpr int kRingSmem = 104 * 1024;  // two CTAs an SM
+constexpr int ring_smem(int stages, int K4) {
+  return kZeroBytes + stages * kChunk * 16 + (stages + 1) * K4 * 12;
+}
 
 template <typename Kern>
 int allow_smem(Kern kern, int bytes, std::atomic<uint64_t>& done) {
@@ -2125,24 +2128,20 @@ int resident_clusters(Kern kern, int cs, int smem, int* out) {
 }
 
 int launch_count(const RowArgs& a, cudaStream_t s) {
-  const int ctas = a.T > kCountThreads ? kCountCluster : 1;
+  // a CTA that holds them all starts sooner, by 1.3 us at 4096 rows
+  const int ctas = a.T > kCountBlock ? kCountCluster : 1;
   const int64_t warps = (a.T + 32 * ctas - 1) / (32 * ctas);  // of rows, for each CTA
   return launch(false, count_kernel, ctas, kCountThreads, 0, ctas, s, a,
                 static_cast<int32_t>(warps * 32));
 }
 
-template <typename T, int OBJ>
-int launch_ring(RowArgs a, int cs, int per, cudaStream_t s) {
-  auto kern = ring_kernel<T, OBJ>;
+template <typename T, int OBJ, bool SHORT>
+int launch_ring(RowArgs a, int cs, int per, int stages, cudaStream_t s) {
+  auto kern = ring_kernel<T, OBJ, SHORT>;
   static std::atomic<uint64_t> done{0};
   int rc = allow_smem(kern, kRingSmem, done);
   if (rc) return rc;
-  // 9 stages without a teacher, 3 at its most entries, fewer than a row may have chunks
-  int stages = kMaxStages, smem = 0;
-  for (;; --stages) {
-    smem = kZeroBytes + stages * kChunk * 16 + (stages + 1) * a.K4 * 12;
-    if (smem <= kRingSmem) break;
-  }
+  const int smem = ring_smem(stages, a.K4);
   int clusters = std::min<int>(2 * device_sm_count(), kMaxRing);
   if (cs > 1 && (rc = resident_clusters(kern, cs, smem, &clusters))) return rc;
   const int64_t n = std::min<int64_t>(a.T, std::min<int64_t>(clusters, kMaxRing / cs)) * cs;
@@ -2151,6 +2150,18 @@ int launch_ring(RowArgs a, int cs, int per, cudaStream_t s) {
   if (!a.self_count && (rc = launch_count(a, s))) return rc;
   rc = launch(!a.self_count, kern, n, kRingThreads + 32, smem, cs, s, a, cs, per, stages);
   return rc ? rc : launch(true, finish_kernel, 1, 256, 0, 1, s, a, static_cast<int>(n));
+}
+
+// 9 stages without a teacher, 8 with 64 entries, 3 with 1024. Only where those are fewer than a
+// row may have chunks are they freed one by one, which costs a few instructions a chunk: 8 x 512
+// rows of 32000 with 64 entries take 96.0 us without and 97.3 us with them.
+template <typename T, int OBJ>
+int launch_ring(const RowArgs& a, int cs, int per, cudaStream_t s) {
+  int stages = kMaxStages;
+  while (ring_smem(stages, a.K4) > kRingSmem) --stages;
+  return OBJ == kDistill && stages < kRingVecs / kChunkVecs
+             ? launch_ring<T, OBJ, OBJ == kDistill>(a, cs, per, stages, s)
+             : launch_ring<T, OBJ, false>(a, cs, per, stages, s);
 }
 
 template <typename T, int OBJ, int G, int NV>
