@@ -698,14 +698,14 @@ __device__ __forceinline__ double2 token_terms(const RowArgs& a, const Counts& n
   return make_double2(w * loss, w * kl);
 }
 
-// A gradient row of zeros.
+// A gradient row of zeros, which L2 gives up first.
 template <typename T, int G>
 __device__ __forceinline__ void zero_row(const RowArgs& a, int64_t r, int tid) {
   if (a.dx == nullptr) return;
   T* dx = static_cast<T*>(a.dx) + a.out.at(r);
   const Span<T> so(dx, a.V);
   uint4* dv = reinterpret_cast<uint4*>(dx + so.head);
-  for (int v = tid; v < so.nvec; v += G) dv[v] = make_uint4(0u, 0u, 0u, 0u);
+  for (int v = tid; v < so.nvec; v += G) __stcs(dv + v, make_uint4(0u, 0u, 0u, 0u));
   if (tid < kEdges && so.edge(tid) >= 0) put(dx + so.edge(tid), 0.f);
 }
 
@@ -1860,6 +1860,10 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(RowArgs a, int64_t P
 
 // Gradient rows from saved statistics: k (1[v = target] - q_v). A group of G threads takes
 // G * kBwdU vectors of one row; nothing is reduced, so rows of any length keep every SM busy.
+// Bound by DRAM (4 x 333 x 50257 bf16, of which two thirds count: 226 MB in 38 us, 6.0 TB/s).
+// Behind the statistics it goes backwards and its stores are the first that L2 gives up, as are
+// the rows of zeros before it, so that it finds part of the input there: the preference loss over
+// 8 x 512 rows of 32000 takes 115 us, with plain stores 119.
 constexpr int kBwdThreads = 256;
 constexpr int kBwdU = 4;
 template <typename T, int G>
@@ -1919,7 +1923,7 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) e[i] = f2_mul(e[i], kq2);
     if (same)
-      dv[v] = Vec<T>::pack(e);
+      __stcs(dv + v, Vec<T>::pack(e));
     else
       store_apart<T>(dx + sp.head + static_cast<int64_t>(v) * E, Vec<T>::pack(e));
     if (tv >= 0 && tv / E == v) put(dx + target, k + ex2((xt - st.x) * a.c) * kq);
