@@ -331,12 +331,44 @@ __device__ __forceinline__ void st16_if(uint4* p, const uint4& v, bool yes) {
       : "memory");
 }
 
-// A vector whose output row starts at another phase within 16 bytes than the input row.
+// The vectors of a warp (one behind the other, those of the first lanes `in`) where the output row
+// starts at another phase within 16 bytes than the input row, as after logits[:, :-1] over an odd
+// vocabulary: each lane stores the aligned vector that its own and the next lane's make up, the
+// first and last lane the elements around. 8 x 512 rows of 32000 bf16: the policy loss takes
+// 230 us, with every element stored alone 378, at the same phase 124.
 template <typename T>
-__device__ __noinline__ void store_apart(T* dst, uint4 w) {
-  const T* e = reinterpret_cast<const T*>(&w);
+__device__ __noinline__ void store_apart(T* dst, uint4 w, bool in) {
+  const int lane = threadIdx.x & 31;
+  const int gap = static_cast<int>(-reinterpret_cast<uintptr_t>(dst) & 15u);  // bytes to 16
+  uint32_t a[8] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int j = 0; j < Vec<T>::kE; ++j) dst[j] = e[j];
+  for (int i = 0; i < 4; ++i) a[4 + i] = __shfl_down_sync(0xffffffffu, a[i], 1);
+  const bool next = __shfl_down_sync(0xffffffffu, in, 1) && lane < 31;
+  if (gap & 4) {
+#pragma unroll
+    for (int i = 0; i < 7; ++i) a[i] = a[i + 1];
+  }
+  if (gap & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) a[i] = a[i + 2];
+  }
+  uint4 o;
+  o.x = __funnelshift_r(a[0], a[1], (gap & 3) * 8);
+  o.y = __funnelshift_r(a[1], a[2], (gap & 3) * 8);
+  o.z = __funnelshift_r(a[2], a[3], (gap & 3) * 8);
+  o.w = __funnelshift_r(a[3], a[4], (gap & 3) * 8);
+  const int front = gap / static_cast<int>(sizeof(T));
+  if (in && next) *reinterpret_cast<uint4*>(dst + front) = o;
+  if (in && (lane == 0 || !next)) {
+    const T* we = reinterpret_cast<const T*>(&w);
+    const T* oe = reinterpret_cast<const T*>(&o);
+#pragma unroll
+    for (int j = 0; j < Vec<T>::kE; ++j) {
+      if (lane == 0 && j < front) dst[j] = we[j];
+      if (!next && j < Vec<T>::kE - front) dst[front + j] = oe[j];
+    }
+  }
+  __syncwarp();  // an element that another lane has stored may be replaced behind this
 }
 
 // ---- reductions ------------------------------------------------------------------
@@ -1004,18 +1036,19 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   const uint64_t kq2 = f2_splat(kq * ks.fix);
   const bool same = same_phase<T>(x, dx);
   uint4* dv = reinterpret_cast<uint4*>(dx + sp.head);
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = tid + i * G;
+  const auto scaled = [&](int i) {
 #pragma unroll
     for (int j = 0; j < E / 2; ++j) e[i][j] = f2_mul(e[i][j], kq2);
-    const uint4 o = Vec<T>::pack(e[i]);
-    if (v < sp.nvec) {
-      if (same)
-        dv[v] = o;
-      else
-        store_apart<T>(dx + sp.head + v * E, o);
-    }
+    return Vec<T>::pack(e[i]);
+  };
+  if (same) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (tid + i * G < sp.nvec) dv[tid + i * G] = scaled(i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      store_apart<T>(reinterpret_cast<T*>(dv + tid + i * G), scaled(i), tid + i * G < sp.nvec);
   }
   if (edge >= 0) put(dx + edge, ee * kq);
   if (OBJ == kPolicy) {
@@ -1034,28 +1067,34 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
 
 // ---- rows held by one CTA, or by the CTAs of a cluster ------------------------------
 
-// The same for longer rows. A persistent CTA, two of them an SM, holds a row or its share of one
-// in the registers of 224 threads. Its eighth warp, the producer, brings the next rows in through
-// a ring of shared memory with bulk copies, so that HBM is read and written without a pause, and
-// with them what else the rows need: their edges, the token's numbers or the teacher's entries. A
-// chunk of the ring is free as soon as it is in registers. Rows are held as they are, not as
-// exponentials, which are taken twice (for the sum and for the gradient): half the registers,
-// hence two CTAs an SM, one of which works while the other waits for its reductions.
+// The same for longer rows. A persistent CTA, two or three of them an SM, holds a row or its share
+// of one in the registers of seven or four warps. Its last warp, the producer, brings the next rows
+// in through a ring of shared memory with bulk copies, so that HBM is read and written without a
+// pause, and with them what else the rows need: their edges, the token's numbers or the teacher's
+// entries. A chunk of the ring is free as soon as it is in registers. Rows are held as they are,
+// not as exponentials, which are taken twice (for the sum and for the gradient): half the
+// registers, hence CTAs that work while others of the SM wait for their reductions.
 //
 // A cluster of cs CTAs shares rows too long for one, or few rows of any length; its CTAs exchange
 // maxima and sums through each other's shared memory.
 //
 // One CTA a row: 16 x 512 rows of 32000 bf16, two thirds of them counted (872 MB), take 159 us,
-// 5.5 TB/s, near what DRAM gives a mix of reads and writes (6.0 TB/s). Clusters: 3 x 611 rows of
-// 100277 (649 MB) take 164 us, 4.0 TB/s, bound by the exchange, some 2500 cycles a row in which
-// its CTAs wait; sweeping them twice takes 235 us. 11 or 15 warps a CTA instead of 7 gave the same.
-constexpr int kRingWarps = 7;
-constexpr int kRingThreads = kRingWarps * 32;
-constexpr int kRingVecs = 18;                            // a thread's vectors, at most
-constexpr int kChunkVecs = 3;                            // of them in a chunk
-constexpr int kChunk = kChunkVecs * kRingThreads;        // vectors
-constexpr int kRingCap = kRingVecs * kRingThreads;       // vectors of a share, at most
+// 5.5 TB/s, near what DRAM gives a mix of reads and writes (6.0 TB/s). Each row costs its CTAs some
+// 2 us of latency (two reductions, in a cluster the exchange) besides its bytes, so shares that
+// leave registers empty are slower: 3 x 611 rows of 100277 (649 MB, four CTAs, 78 percent full)
+// take 164 us, 4.0 TB/s; sweeping them twice takes 235 us. Rows held in shared memory instead, the
+// gradient of one behind the sums of the next, took 217 us, one or two CTAs an SM.
+constexpr int kRingVecs = 18;  // a thread's vectors, at most
+constexpr int kChunkVecs = 3;  // of them in a chunk
 constexpr int kMaxStages = 9;
+template <int WARPS>
+struct Ring {
+  static constexpr int kThreads = WARPS * 32;
+  static constexpr int kChunk = kChunkVecs * kThreads;  // vectors
+  static constexpr int kCap = kRingVecs * kThreads;     // vectors of a share, at most
+  static constexpr int kCtas = 16 / (WARPS + 1);        // an SM, of 128 registers a thread
+  static constexpr int kSmem = 208 * 1024 / kCtas - 2048 * (kCtas - 2);
+};
 constexpr int kZeroBytes = 8192;                         // source of the rows of zeros
 constexpr int kMaxCluster = 8;
 
@@ -1089,15 +1128,17 @@ __device__ __forceinline__ bool in_share(int head, int nvec, int start, int nv, 
   return i < head || i >= head + nvec * Vec<T>::kE ? rank == 0 : v >= 0 && v < nv;
 }
 // The thread that holds element i of its share.
-template <typename T>
+template <typename T, int THREADS>
 __device__ __forceinline__ int share_owner(const Span<T>& sp, int start, int i) {
   if (i < sp.head || i >= sp.head + sp.nvec * Vec<T>::kE) return sp.owner(i, 1);
-  return ((i - sp.head) / Vec<T>::kE - start) % kRingThreads;
+  return ((i - sp.head) / Vec<T>::kE - start) % THREADS;
 }
 
+template <int THREADS>
 __device__ __forceinline__ void ring_sync() {
-  asm volatile("bar.sync 1, %0;" ::"n"(kRingThreads) : "memory");
+  asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
 }
+template <int THREADS>
 __device__ __forceinline__ bool ring_all(bool ok) {
   uint32_t r;
   asm volatile(
@@ -1106,7 +1147,7 @@ __device__ __forceinline__ bool ring_all(bool ok) {
       "bar.red.and.pred q, 1, %2, p;\n\t"
       "selp.u32 %0, 1, 0, q;\n\t}\n"
       : "=r"(r)
-      : "r"(static_cast<uint32_t>(ok)), "n"(kRingThreads)
+      : "r"(static_cast<uint32_t>(ok)), "n"(THREADS)
       : "memory");
   return r != 0;
 }
@@ -1153,9 +1194,9 @@ struct OwnRows {
 template <int THREADS>
 __device__ __forceinline__ int list_own(const RowArgs& a, uint32_t first, uint32_t step,
                                         OwnRows* own) {
-  constexpr int kRows = 8, kWarps = THREADS / 32, kCells = kRows * kWarps;
-  static_assert(kCells == 64, "two cells a lane");
-  __shared__ int32_t s_cell[kCells];
+  constexpr int kWarps = THREADS / 32, kRows = 64 / kWarps;
+  constexpr int kCells = kRows * kWarps;  // two a lane, at most
+  __shared__ int32_t s_cell[64];
   __shared__ int32_t s_end;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (a.per_sequence)
@@ -1181,7 +1222,8 @@ __device__ __forceinline__ int list_own(const RowArgs& a, uint32_t first, uint32
     }
     __syncthreads();
     if (warp == 0) {
-      const int n0 = s_cell[2 * lane], n1 = s_cell[2 * lane + 1];
+      const int n0 = 2 * lane < kCells ? s_cell[2 * lane] : 0,
+                n1 = 2 * lane + 1 < kCells ? s_cell[2 * lane + 1] : 0;
       int incl = n0 + n1;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -1211,10 +1253,10 @@ __device__ __forceinline__ int list_own(const RowArgs& a, uint32_t first, uint32
 }
 
 // SHORT: fewer stages than a row may have chunks, for many teacher entries.
-template <typename T, int OBJ, bool SHORT>
-__global__ void __launch_bounds__(kRingThreads + 32, 2)
+template <typename T, int OBJ, int WARPS, bool SHORT>
+__global__ void __launch_bounds__((WARPS + 1) * 32, Ring<WARPS>::kCtas)
     ring_kernel(RowArgs a, int cs, int per, int stages) {
-  constexpr int E = Vec<T>::kE;
+  constexpr int E = Vec<T>::kE, kThreads = Ring<WARPS>::kThreads, kChunk = Ring<WARPS>::kChunk;
   extern __shared__ __align__(16) char smem[];
   uint4* zeros = reinterpret_cast<uint4*>(smem);
   uint4* ring = zeros + kZeroBytes / 16;  // [stages][kChunk]
@@ -1227,21 +1269,21 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
   // that after it is done with the row before: one slot more than stages.
   __shared__ RowInfo info[kMaxStages + 1];
   __shared__ Share share[2][kMaxCluster];
-  __shared__ float red_m[8], red_s[8];
-  __shared__ double2 red_t[8];
+  __shared__ float red_m[WARPS], red_s[WARPS];
+  __shared__ double2 red_t[WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = cs > 1 ? static_cast<int>(ptx::cluster_ctarank()) : 0;
   const int start = rank * per;  // this CTA's first vector of a row; rank 0 has the edges too
   if (tid == 0) {
     for (int i = 0; i < stages; ++i) {
       ptx::mbar_init(&full[i], 1);
-      ptx::mbar_init(&empty[i], kRingWarps);
+      ptx::mbar_init(&empty[i], WARPS);
     }
     ptx::mbar_init(&exchanged[0], 1);
     ptx::mbar_init(&exchanged[1], 1);
     ptx::fence_mbar_init();
   }
-  for (int i = tid; i < kZeroBytes / 16; i += kRingThreads + 32) zeros[i] = make_uint4(0, 0, 0, 0);
+  for (int i = tid; i < kZeroBytes / 16; i += kThreads + 32) zeros[i] = make_uint4(0, 0, 0, 0);
   ptx::fence_proxy_async_smem();  // bulk copies read them
   __syncthreads();
   if (cs > 1) ptx::cluster_sync();
@@ -1251,7 +1293,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
   const int64_t first = blockIdx.x / cs, step = gridDim.x / cs;
   Counts counts = listed_counts(a);
   if (a.self_count)
-    counts = Counts{list_own<kRingThreads + 32>(a, static_cast<uint32_t>(first),
+    counts = Counts{list_own<kThreads + 32>(a, static_cast<uint32_t>(first),
                                                 static_cast<uint32_t>(step), &own),
                     own.seq};
   const int64_t total = counts.total;
@@ -1260,7 +1302,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
     return a.self_count ? own.row[i] : a.list[first + i * step];
   };
 
-  if (warp == kRingWarps) {
+  if (warp == WARPS) {
     // ---- producer: 32 rows' numbers at a time, then each row's copies
     int i = 0, st = 0, slot = 0;  // chunks so far, the next one's stage, the next row's slot
     uint32_t phase = 0;
@@ -1370,7 +1412,7 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
               inf->target = target;
               inf->owner =
                   target >= 0 && in_share<T>(sp.head, sp.nvec, start, nv, rank, target)
-                      ? share_owner<T>(sp, start, target)
+                      ? share_owner<T, kThreads>(sp, start, target)
                       : -1;
               inf->xt = xt;
               inf->w = w;
@@ -1435,11 +1477,11 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
           if (c > 0) ok = ptx::mbar_wait(&full[st], phase) && ok;
           const uint4* buf = ring + st * kChunk + tid;
 #pragma unroll
-          for (int j = 0; j < kChunkVecs; ++j) w[c * kChunkVecs + j] = buf[j * kRingThreads];
+          for (int j = 0; j < kChunkVecs; ++j) w[c * kChunkVecs + j] = buf[j * kThreads];
           if (nv < (c + 1) * kChunk) {  // what the chunk does not fill is old
 #pragma unroll
             for (int j = 0; j < kChunkVecs; ++j)
-              if (c * kChunk + j * kRingThreads + tid >= nv)
+              if (c * kChunk + j * kThreads + tid >= nv)
                 w[c * kChunkVecs + j] = neg_inf_vec<T>();
           }
           if (++st == stages) {
@@ -1464,14 +1506,14 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
       m = warp_max(m);
       if (lane == 0) red_m[warp] = m;
       // one barrier for the maximum and for every thread's waits: all leave here, or none
-      if (!ring_all(ok)) {
+      if (!ring_all<kThreads>(ok)) {
         if (tid == 0) atomicMax(a.err, static_cast<int32_t>(kDevErrLossTimeout));
         break;
       }
       if (inf->row < 0) break;
       m = red_m[0];
 #pragma unroll
-      for (int j = 1; j < kRingWarps; ++j) m = fmaxf(m, red_m[j]);
+      for (int j = 1; j < WARPS; ++j) m = fmaxf(m, red_m[j]);
       const bool far = far_max(m, a.c);
       if (far) {
 #pragma unroll
@@ -1500,10 +1542,10 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
       f2_unpack(acc2, s, hi);
       s = warp_sum((s + hi) * ks.fix + ee);
       if (lane == 0) red_s[warp] = s;
-      ring_sync();
+      ring_sync<kThreads>();
       s = 0.f;
 #pragma unroll
-      for (int j = 0; j < kRingWarps; ++j) s += red_s[j];
+      for (int j = 0; j < WARPS; ++j) s += red_s[j];
       float scale = 1.f, m_row = m;
       if (cs > 1) {
         const uint32_t b = i & 1;
@@ -1559,14 +1601,14 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
             if (same) {
 #pragma unroll
               for (int j = 0; j < kChunkVecs; ++j) {
-                const int v = c * kChunk + j * kRingThreads;
+                const int v = c * kChunk + j * kThreads;
                 st16_if(dv + v, o[j], v + tid < nv);
               }
             } else {
 #pragma unroll
               for (int j = 0; j < kChunkVecs; ++j) {
-                const int v = c * kChunk + j * kRingThreads;
-                if (v + tid < nv) store_apart<T>(reinterpret_cast<T*>(dv + v), o[j]);
+                const int v = c * kChunk + j * kThreads;
+                store_apart<T>(reinterpret_cast<T*>(dv + v), o[j], v + tid < nv);
               }
             }
           }
@@ -1579,12 +1621,12 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
             if (tid == inf->owner)
               put(dx + inf->target, k - ex2((inf->xt - m_row) * a.c) * inv_s * k);
           } else {
-            ring_sync();
+            ring_sync<kThreads>();
             const float* s_p = s_p0 + slot * a.K4;
             const float* s_x = s_x0 + slot * a.K4;
             const int32_t* s_id = s_id0 + slot * a.K4;
             const float inv_t = 1.f / inf->t.t_sum;
-            for (int j = tid; j < a.K; j += kRingThreads)
+            for (int j = tid; j < a.K; j += kThreads)
               if (s_id[j] >= 0 &&
                   in_share<T>(inf->head, inf->nvec, start, nv, rank, s_id[j]))
                 put(dx + s_id[j],
@@ -1596,10 +1638,10 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
       slot = slot == stages ? 0 : slot + 1;
     }
     // the terms of this CTA's tokens: thread 0 wrote what their rows left
-    ring_sync();
+    ring_sync<kThreads>();
     double2 terms = make_double2(0.0, 0.0);
     if (rank == 0 && ok)
-      for (int i = tid; i < n_row; i += kRingThreads) {
+      for (int i = tid; i < n_row; i += kThreads) {
         const double2 v = token_terms<OBJ>(a, counts, row_of(i));
         terms.x += v.x;
         terms.y += v.y;
@@ -1607,9 +1649,9 @@ __global__ void __launch_bounds__(kRingThreads + 32, 2)
     terms.x = warp_sum(terms.x);
     terms.y = warp_sum(terms.y);
     if (lane == 0) red_t[warp] = terms;
-    ring_sync();
+    ring_sync<kThreads>();
     if (tid == 0) {
-      for (int j = 1; j < kRingWarps; ++j) {
+      for (int j = 1; j < WARPS; ++j) {
         terms.x += red_t[j].x;
         terms.y += red_t[j].y;
       }
@@ -1704,12 +1746,11 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
           exp_vec<T>(w[u], ks, e);
 #pragma unroll
           for (int i = 0; i < E / 2; ++i) e[i] = f2_mul(e[i], kq2);
-          if (v < sp.nvec) {
-            if (same)
-              __stcs(dv + v, Vec<T>::pack(e));
-            else
-              store_apart<T>(dx + sp.head + static_cast<int64_t>(v) * E, Vec<T>::pack(e));
-          }
+          if (!same)
+            store_apart<T>(dx + sp.head + static_cast<int64_t>(v) * E, Vec<T>::pack(e),
+                           v < sp.nvec);
+          else if (v < sp.nvec)
+            __stcs(dv + v, Vec<T>::pack(e));
         }
       }
       if (edge >= 0) put(dx + edge, ex2((xe - m) * a.c) * kq);
@@ -1921,20 +1962,33 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
   const bool ok = target >= 0 && target < a.V;
   const int tv = ok ? static_cast<int>(target) - sp.head : -1;  // its place behind the head
   const float xt = ok ? to_f(x[target]) : 0.f;
-#pragma unroll
-  for (int u = 0; u < kBwdU; ++u) {
-    const int v = v0 + u * G;
-    if (v >= sp.nvec) continue;
+  const auto scaled = [&](uint4 x16) {
     uint64_t e[E / 2];
-    if (far) shift_vec<T>(w[u], st.x);
-    exp_vec<T>(w[u], ks, e);
+    if (far) shift_vec<T>(x16, st.x);
+    exp_vec<T>(x16, ks, e);
 #pragma unroll
     for (int i = 0; i < E / 2; ++i) e[i] = f2_mul(e[i], kq2);
-    if (same)
-      __stcs(dv + v, Vec<T>::pack(e));
-    else
-      store_apart<T>(dx + sp.head + static_cast<int64_t>(v) * E, Vec<T>::pack(e));
+    return Vec<T>::pack(e);
+  };
+  const auto put_target = [&](int v) {
     if (tv >= 0 && tv / E == v) put(dx + target, k + ex2((xt - st.x) * a.c) * kq);
+  };
+  if (same) {
+#pragma unroll
+    for (int u = 0; u < kBwdU; ++u) {
+      const int v = v0 + u * G;
+      if (v >= sp.nvec) continue;
+      __stcs(dv + v, scaled(w[u]));
+      put_target(v);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < kBwdU; ++u) {
+      const int v = v0 + u * G;
+      if (v - tid >= sp.nvec) continue;  // for all of the group
+      store_apart<T>(reinterpret_cast<T*>(dv + v), scaled(w[u]), v < sp.nvec);
+      if (v < sp.nvec) put_target(v);
+    }
   }
   if (chunk == 0 && tid < kEdges && sp.edge(tid) >= 0) {
     const int i = sp.edge(tid);
@@ -2099,9 +2153,9 @@ int launch_logprobs_bwd(const RowArgs& a, int x_f32, bool after, cudaStream_t s)
                : launch_logprobs_bwd_t<__nv_bfloat16>(a, nvec, after, s);
 }
 
-constexpr int kRingSmem = 104 * 1024;  // two CTAs an SM
-constexpr int ring_smem(int stages, int K4) {
-  return kZeroBytes + stages * kChunk * 16 + (stages + 1) * K4 * 12;
+template <int WARPS>
+int ring_smem(int stages, int K4) {
+  return kZeroBytes + stages * Ring<WARPS>::kChunk * 16 + (stages + 1) * K4 * 12;
 }
 
 template <typename Kern>
@@ -2116,15 +2170,15 @@ int allow_smem(Kern kern, int bytes, std::atomic<uint64_t>& done) {
 }
 
 // Clusters of cs CTAs that are resident at once.
-template <typename Kern>
+template <int WARPS, typename Kern>
 int resident_clusters(Kern kern, int cs, int smem, int* out) {
-  static std::atomic<int> cache[64][4];  // by device and log2(cs); 2 CTAs an SM either way
-  const int dev = current_device(), slot = cs == 2 ? 1 : (cs == 4 ? 2 : 3);
-  int n = cache[dev][slot].load();
+  static std::atomic<int> cache[64][kMaxCluster + 1];  // Ring::kCtas an SM whatever the kernel
+  const int dev = current_device();
+  int n = cache[dev][cs].load();
   if (n == 0) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(cs));
-    cfg.blockDim = dim3(kRingThreads + 32);
+    cfg.blockDim = dim3((WARPS + 1) * 32);
     cfg.dynamicSmemBytes = static_cast<size_t>(smem);
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -2134,7 +2188,7 @@ int resident_clusters(Kern kern, int cs, int smem, int* out) {
     cfg.numAttrs = 1;
     LEMA_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
     if (n < 1) return set_error(LEMA_ERR_CUDA, "no cluster fits this device");
-    cache[dev][slot].store(n);
+    cache[dev][cs].store(n);
   }
   *out = n;
   return LEMA_OK;
@@ -2148,33 +2202,38 @@ int launch_count(const RowArgs& a, cudaStream_t s) {
                 static_cast<int32_t>(warps * 32));
 }
 
-template <typename T, int OBJ, bool SHORT>
+template <typename T, int OBJ, int WARPS, bool SHORT>
 int launch_ring(RowArgs a, int cs, int per, int stages, cudaStream_t s) {
-  auto kern = ring_kernel<T, OBJ, SHORT>;
+  auto kern = ring_kernel<T, OBJ, WARPS, SHORT>;
   static std::atomic<uint64_t> done{0};
-  int rc = allow_smem(kern, kRingSmem, done);
+  int rc = allow_smem(kern, Ring<WARPS>::kSmem, done);
   if (rc) return rc;
-  const int smem = ring_smem(stages, a.K4);
-  int clusters = std::min<int>(2 * device_sm_count(), kMaxRing);
-  if (cs > 1 && (rc = resident_clusters(kern, cs, smem, &clusters))) return rc;
+  const int smem = ring_smem<WARPS>(stages, a.K4);
+  int clusters = std::min<int>(Ring<WARPS>::kCtas * device_sm_count(), kMaxRing);
+  if (cs > 1 && (rc = resident_clusters<WARPS>(kern, cs, smem, &clusters))) return rc;
   const int64_t n = std::min<int64_t>(a.T, std::min<int64_t>(clusters, kMaxRing / cs)) * cs;
   a.self_count = a.T <= kOwnTotal && a.T <= kOwnRows * (n / cs) &&
                  (!a.per_sequence || a.n0 <= kOwnSeqs);
   if (!a.self_count && (rc = launch_count(a, s))) return rc;
-  rc = launch(!a.self_count, kern, n, kRingThreads + 32, smem, cs, s, a, cs, per, stages);
+  rc = launch(!a.self_count, kern, n, (WARPS + 1) * 32, smem, cs, s, a, cs, per, stages);
   return rc ? rc : launch(true, finish_kernel, 1, 256, 0, 1, s, a, static_cast<int>(n));
 }
 
-// 9 stages without a teacher, 8 with 64 entries, 3 with 1024. Only where those are fewer than a
-// row may have chunks are they freed one by one, which costs a few instructions a chunk: 8 x 512
-// rows of 32000 with 64 entries take 96.0 us without and 97.3 us with them.
-template <typename T, int OBJ>
-int launch_ring(const RowArgs& a, int cs, int per, cudaStream_t s) {
+// Seven warps: 9 stages without a teacher, 8 with 64 entries, 3 with 1024. Only where those are
+// fewer than a row may have chunks are they freed one by one, which costs a few instructions a
+// chunk: 8 x 512 rows of 32000 with 64 entries take 96.0 us without and 97.3 us with them.
+template <typename T, int OBJ, int WARPS>
+int launch_ring(const RowArgs& a, int cs, int nvec, cudaStream_t s) {
+  // few rows: spread each while SMs would be idle and every thread still has a vector
+  while (cs * 2 <= kMaxCluster && a.T * cs * 2 <= device_sm_count() &&
+         nvec >= cs * 2 * Ring<WARPS>::kThreads)
+    cs *= 2;
+  const int per = (nvec + cs - 1) / cs;
   int stages = kMaxStages;
-  while (ring_smem(stages, a.K4) > kRingSmem) --stages;
+  while (ring_smem<WARPS>(stages, a.K4) > Ring<WARPS>::kSmem) --stages;
   return OBJ == kDistill && stages < kRingVecs / kChunkVecs
-             ? launch_ring<T, OBJ, OBJ == kDistill>(a, cs, per, stages, s)
-             : launch_ring<T, OBJ, false>(a, cs, per, stages, s);
+             ? launch_ring<T, OBJ, WARPS, OBJ == kDistill>(a, cs, per, stages, s)
+             : launch_ring<T, OBJ, WARPS, false>(a, cs, per, stages, s);
 }
 
 template <typename T, int OBJ, int G, int NV>
@@ -2190,7 +2249,8 @@ int launch_direct(const RowArgs& a, int64_t grid, int smem, cudaStream_t s) {
 
 // How a row is held, by the vectors it spans. kNv vectors are the 64 elements that a thread
 // keeps as fp32. A warp a row while it holds it: policy over 65536 rows of 512 bf16 takes 47 us,
-// with 128 threads a row 124 us; over 16384 of 2000 it takes 38 and 48 us. Sets self_count for token_kernel, or *done where it is not needed.
+// with 128 threads a row 124 us; over 16384 of 2000 it takes 38 and 48 us. Sets self_count for
+// token_kernel, or *done where it is not needed.
 template <typename T, int OBJ>
 int launch_rows(RowArgs& a, int nvec, bool* done, cudaStream_t s) {
   constexpr int kNv = 64 / Vec<T>::kE;
@@ -2210,21 +2270,24 @@ int launch_rows(RowArgs& a, int nvec, bool* done, cudaStream_t s) {
     if (nvec <= 64 * kNv) return launch_direct<T, OBJ, 128, kNv / 2>(a, grid, smem, s);
     return launch_direct<T, OBJ, 128, kNv>(a, grid, smem, s);
   }
-  int cs = 1;
-  while (cs < kMaxCluster && nvec > cs * kRingCap) cs *= 2;
-  if (nvec > cs * kRingCap) {
+  // What an SM's CTAs hold at once is what keeps DRAM busy while each waits for its reductions: the
+  // fewest CTAs a row, of seven warps (two an SM) or of four (three an SM), whichever hold
+  // more. Of bf16 policy rows, a quarter not counted, 16000 elements reach 4.0 TB/s with
+  // seven warps and 4.6 with four, 32000 4.9 and 4.6, 32264 (two CTAs) 3.5 and 4.6, 50257 4.4
+  // (two CTAs) and 4.0 (four).
+  const int cs7 = (nvec + Ring<7>::kCap - 1) / Ring<7>::kCap,
+            cs4 = (nvec + Ring<4>::kCap - 1) / Ring<4>::kCap;
+  if (cs7 > kMaxCluster) {
     const int rc = launch_count(a, s);
     return rc ? rc
               : launch(true, stream_kernel<T, OBJ>,
                        std::min<int64_t>(a.T, device_sm_count()), kRowThreads, teacher, 1, s,
                        a);
   }
-  // few rows: spread each while SMs would be idle and every thread still has a vector
-  while (cs < kMaxCluster && a.T * cs * 2 <= device_sm_count() &&
-         nvec >= cs * 2 * kRingThreads)
-    cs *= 2;
   *done = true;
-  return launch_ring<T, OBJ>(a, cs, (nvec + cs - 1) / cs, s);
+  return cs4 > kMaxCluster || Ring<7>::kCtas * cs4 >= Ring<4>::kCtas * cs7
+             ? launch_ring<T, OBJ, 7>(a, cs7, nvec, s)
+             : launch_ring<T, OBJ, 4>(a, cs4, nvec, s);
 }
 
 // The list of rows, their statistics and gradients, the tokens' terms.

@@ -778,3 +778,58 @@ def test_far_rows(cuda_device, V):
             # k = -1/6/tau (mass - q); the bound on q counts exponents up to 150
             check_dx(dx, x, q, torch.full((1, 6), -1 / 6 / tau, dtype=torch.float64,
                                           device=x.device), onehot(t, V), tau)
+
+
+@pytest.mark.parametrize("V", [8201, 13001, 18440, 33000, 70001, 80000, 96777, 136001, 176008,
+                               208003, 258048])
+def test_row_lengths(cuda_device, V):
+    """Rows that one CTA of either size holds, and that two to eight share."""
+    dtype = "bf16"
+    for B, S in ((2, 2), (2, 75)):
+        x, t, g = make(cuda_device, B, S, V, dtype)
+        adv = torch.randn(B, S, device=x.device, generator=g)
+        loss, lps, _, dx = ops.policy_loss_grad(x, t, None, adv)
+        lp, q = ref_logps(x, t)
+        check_logps(lps, lp, V)
+        n = max(1, int((t != IGN).sum()))
+        check_dx(dx, x, q, torch.where(t == IGN, 0.0, -adv.double() / n), onehot(t, V))
+        val, ids = torch.topk(x.float(), 7, -1)
+        _, dx = ops.distill_loss_grad(x, ids, val, t != IGN)
+        _, k, mass, q = ref_distill(x, ids, val, t != IGN, 1.0)
+        # the weights' own errors: 7 u of their exponents, 2 u of ex2, 7 u of their sum, 2 u
+        check_dx(dx, x, q, k, mass, mass_err=18 * U)
+        del x, q, mass, dx
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", [5, 37, 300, 1999, 8000, 9001, 33000, 300001])
+def test_gradient_rows_at_other_phases(cuda_device, V, dtype):
+    """Gradient rows that start at every place within 16 bytes, whatever their logits' place; what
+    lies between them stays."""
+    x, t, g = make(cuda_device, 2, 9, V, dtype, ignore=0.2)
+    adv = torch.randn(2, 9, device=x.device, generator=g)
+    val, ids = torch.topk(x.float(), min(V, 5), -1)
+    w = torch.where(t == IGN, 0.0, adv).contiguous()
+    lead = x.requires_grad_(True)
+    want = [ops.policy_loss_grad(x.detach(), t, None, adv)[3],
+            ops.distill_loss_grad(x.detach(), ids, val, t != IGN)[1],
+            ops.preference_loss_grad(x.detach(), t)[2]]
+    lp = torch.autograd.grad(ops.token_logprobs(lead, t), lead, w)[0]
+    x = x.detach()
+    for gap in range(1, 9 if dtype == "bf16" else 5):
+        room = torch.full((2, 9, V + 16), 7.0, dtype=x.dtype, device=x.device)
+        out = room[..., gap:gap + V]
+        shut = (room[..., :gap], room[..., gap + V:])
+        for k, f in enumerate((lambda: ops.policy_loss_grad(x, t, None, adv, out=out),
+                               lambda: ops.distill_loss_grad(x, ids, val, t != IGN, out=out),
+                               lambda: ops.preference_loss_grad(x, t, out=out))):
+            f()
+            assert torch.equal(out, want[k])
+            assert all((s == 7.0).all() for s in shut)
+        # the same from logits at another place
+        apart = torch.empty(2, 9, V + 16, dtype=x.dtype, device=x.device)[..., gap:gap + V]
+        apart.copy_(x).requires_grad_(True)
+        got = torch.autograd.grad(ops.token_logprobs(apart, t), apart, w)[0]
+        # edges differ, and with them the order of a row's sum
+        assert ((got.double() - lp.double()).abs()
+                <= half_step(got.dtype) * 2.1 * lp.double().abs() + rel_s(V) * w[..., None].abs()).all()
