@@ -831,5 +831,39 @@ def test_gradient_rows_at_other_phases(cuda_device, V, dtype):
         apart.copy_(x).requires_grad_(True)
         got = torch.autograd.grad(ops.token_logprobs(apart, t), apart, w)[0]
         # edges differ, and with them the order of a row's sum
-        assert ((got.double() - lp.double()).abs()
-                <= half_step(got.dtype) * 2.1 * lp.double().abs() + rel_s(V) * w[..., None].abs()).all()
+        tol = half_step(got.dtype) * 2.1 * lp.double().abs() + rel_s(V) * w[..., None].abs()
+        assert ((got.double() - lp.double()).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("V", [130, 8500])
+def test_many_rows_in_graphs(cuda_device, V):
+    """Rows that a cluster lists, captured: what is counted at replay is what the targets say
+    then. Two streams replay two graphs at once."""
+    dev = cuda_device
+    data = [make(dev, 45, 200, V, "bf16", seed=s, ignore=0.2 + 0.3 * s) for s in range(2)]
+    adv = torch.randn(45, device=dev)
+
+    def both(x, t):
+        return (*ops.policy_loss_grad(x, t, None, adv, reduction="sequence"),
+                *ops.policy_loss_grad(x, t, None, adv))
+    want = [both(x, t) for x, t, _ in data]
+    graphs = []
+    for x, t, _ in data:
+        bufs = [x.clone(), t.clone()]
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = both(*bufs)
+        graphs.append((g, bufs, got))
+    streams = [torch.cuda.Stream(dev) for _ in graphs]
+    for swap in (1, 0):
+        for k, (_, bufs, _) in enumerate(graphs):
+            for b, src in zip(bufs, data[k ^ swap]):
+                b.copy_(src)
+        torch.cuda.synchronize()
+        for s, (g, _, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for k, (_, _, got) in enumerate(graphs):
+            for a, w in zip(got, want[k ^ swap]):
+                assert torch.equal(a, w)
