@@ -745,13 +745,13 @@ __device__ __forceinline__ void zero_row(const RowArgs& a, int64_t r, int tid) {
 // by DRAM's reads (4096 x 32000 bf16, three quarters of them counted: 36 us, 5.5 TB/s), short
 // ones by the latency of a row's chain of loads and reductions (65536 x 512: 26 us, 1.9 TB/s).
 // Several rows for each group, their targets loaded and logarithms taken together, gave nothing.
-constexpr int kStatThreads = 128;
+constexpr int stat_threads(int G) { return G > 128 ? G : 128; }
 template <typename T, int G, bool WHOLE, int U>
-__global__ void __launch_bounds__(kStatThreads) logprobs_kernel(RowArgs a) {
-  __shared__ float redf[kStatThreads / 32];
-  __shared__ double redd[kStatThreads / 32];
+__global__ void __launch_bounds__(stat_threads(G)) logprobs_kernel(RowArgs a) {
+  __shared__ float redf[G / 32];
+  __shared__ double redd[G / 32];
   const int tid = threadIdx.x % G;
-  const int64_t r = blockIdx.x * int64_t{kStatThreads / G} + threadIdx.x / G;
+  const int64_t r = blockIdx.x * int64_t{stat_threads(G) / G} + threadIdx.x / G;
   if (r >= a.T) return;
   if (r == 0 && tid == 0 && a.head) a.head->ticket = 0;  // pair_kernel's
   int64_t target;
@@ -2111,22 +2111,28 @@ bool warp_rows(int nvec) { return nvec <= 128; }
 
 template <typename T, int G, bool WHOLE, int U>
 int launch_logprobs_g(const RowArgs& a, cudaStream_t s) {
-  constexpr int64_t kRows = kStatThreads / G;
+  constexpr int64_t kRows = stat_threads(G) / G;
   logprobs_kernel<T, G, WHOLE, U>
-      <<<static_cast<unsigned>((a.T + kRows - 1) / kRows), kStatThreads, 0, s>>>(a);
+      <<<static_cast<unsigned>((a.T + kRows - 1) / kRows), stat_threads(G), 0, s>>>(a);
   LEMA_CUDA_TRY(cudaGetLastError());
   return LEMA_OK;
 }
 
 // As many vectors in flight as a thread has, 8 at most: with 8 for all, 65536 rows of 512 bf16
 // took 47 us instead of 26 and 16384 of 4096 took 44 instead of 31, most of their exponentials
-// those of absent vectors.
+// those of absent vectors. Few long rows get more threads: 100 rows of 128256 bf16 take 19.6 us
+// with 128, 13.4 with 256 and 11.2 with 512 threads, 450 take 30, 27 and 28; 1500 of 32000 take
+// 22, 22 and 28, 6250 of them 9 percent more with 256 than with 128.
 template <typename T, bool WHOLE>
 int launch_logprobs_t(const RowArgs& a, int nvec, cudaStream_t s) {
   if (nvec <= 32 * 2) return launch_logprobs_g<T, 32, WHOLE, 2>(a, s);
   if (warp_rows(nvec)) return launch_logprobs_g<T, 32, WHOLE, 4>(a, s);
-  if (nvec <= kStatThreads * 4) return launch_logprobs_g<T, kStatThreads, WHOLE, 4>(a, s);
-  return launch_logprobs_g<T, kStatThreads, WHOLE, 8>(a, s);
+  if (nvec <= 128 * 4) return launch_logprobs_g<T, 128, WHOLE, 4>(a, s);
+  if (nvec > 2 * 128 * 8) {  // two sweeps of 128 threads
+    if (a.T <= device_sm_count()) return launch_logprobs_g<T, 512, WHOLE, 8>(a, s);
+    if (a.T <= 4 * device_sm_count()) return launch_logprobs_g<T, 256, WHOLE, 8>(a, s);
+  }
+  return launch_logprobs_g<T, 128, WHOLE, 8>(a, s);
 }
 
 template <bool WHOLE>
