@@ -891,7 +891,9 @@ class _Logits:
     def grad_out(self, logits: torch.Tensor, out: torch.Tensor | None):
         """(gradient tensor, its pointer, its two row strides)."""
         if out is None:
-            out = torch.empty(logits.shape, dtype=logits.dtype, device=self.dev)
+            # the quickest of torch's allocations, here and below: a short call is their sum
+            out = (torch.empty_like(logits) if logits.is_contiguous()
+                   else torch.empty(logits.shape, dtype=logits.dtype, device=self.dev))
             return out, (out.data_ptr(), self.n1 * self.V, self.V)
         if out.shape != logits.shape or out.dtype != logits.dtype or out.device != self.dev:
             raise ValueError("out must have the logits' shape, type and device")
@@ -913,9 +915,13 @@ class _Logits:
             view = out[None]
         return out, (view.data_ptr(), view.stride(0), view.stride(1))
 
-    def workspace(self):
+    def workspace(self, more: int = 0):
+        """(scratch, its bytes for the call); `more` bytes behind those, 8-byte aligned."""
         n = _loss_workspace_bytes(self.n0, self.n1)
-        return torch.empty(n, dtype=torch.uint8, device=self.dev), n
+        return torch.empty(n + more, dtype=torch.uint8, device=self.dev), n
+
+    def scalar(self):
+        return torch.empty_strided((), (), dtype=torch.float32, device=self.dev)
 
     def call(self, name: str, *args) -> None:
         """One entry point on the logits' device and its current stream."""
@@ -984,7 +990,7 @@ def _first_order(backward):
 def _logprobs_fwd(logits, targets, temperature, ignore_index, want_stats):
     x = _Logits(logits)
     targets = _targets(x, targets)
-    logps = torch.empty(x.lead, dtype=torch.float32, device=x.dev)
+    logps = torch.empty_like(targets, dtype=torch.float32)
     stats = (torch.empty(x.n0, x.n1, 2, dtype=torch.float32, device=x.dev) if want_stats
              else None)
     x.call("lema_token_logprobs", targets.data_ptr(), ignore_index, temperature,
@@ -1028,14 +1034,15 @@ def _preference(logits, targets, ref_logps, beta, label_smoothing, ignore_index,
                          "their P rejected ones")
     targets = _targets(x, targets)
     ref = x.per_row(ref_logps, "ref_logps", torch.float32)
-    ws, n = x.workspace()
     T = x.n0 * x.n1
-    # statistics (pairs, 8-byte aligned), log-probabilities, coefficients
-    saved = torch.empty(4 * T, dtype=torch.float32, device=x.dev)
+    # statistics (pairs, 8-byte aligned), log-probabilities, coefficients: for a backward, or
+    # for this call alone
+    ws, n = x.workspace(16 * T if want_dx else 0)
+    saved = None if want_dx else torch.empty(4 * T, dtype=torch.float32, device=x.dev)
     rewards = torch.empty(x.n0, dtype=torch.float32, device=x.dev)
-    loss = torch.empty((), dtype=torch.float32, device=x.dev)
+    loss = x.scalar()
     dx, where = x.grad_out(logits, out) if want_dx else (None, _NO_GRAD)
-    at = saved.data_ptr()
+    at = ws.data_ptr() + n if want_dx else saved.data_ptr()
     x.call("lema_preference_loss", targets.data_ptr(), int(ignore_index), _ptr(ref), float(beta),
            float(label_smoothing), float(grad_scale), ws.data_ptr(), n, at + 8 * T, at,
            at + 12 * T, loss.data_ptr(), rewards.data_ptr(), *where)
@@ -1114,9 +1121,8 @@ def _policy(logits, targets, old_logps, advantages, ref_logps, clip, kl_coef, te
     else:
         raise ValueError(f"advantages must have shape {tuple(x.lead)}, or one per sequence")
     ws, n = x.workspace()
-    logps = torch.empty(x.lead, dtype=torch.float32, device=x.dev)
-    loss = torch.empty((), dtype=torch.float32, device=x.dev)
-    kl = torch.empty((), dtype=torch.float32, device=x.dev)
+    logps = torch.empty_like(targets, dtype=torch.float32)
+    loss, kl = x.scalar(), x.scalar()
     # statistics (pairs, 8-byte aligned), coefficients
     T = x.n0 * x.n1
     saved = torch.empty(3 * T, dtype=torch.float32, device=x.dev) if want_saved else None
@@ -1207,7 +1213,7 @@ def _teacher(x: _Logits, ids: torch.Tensor, logits: torch.Tensor, mask):
 def _distill(x, logits, ids, tl, mask, temperature, grad_scale, upstream, out, want_dx):
     """One call on checked teacher tensors: (loss, dlogits or None)."""
     ws, n = x.workspace()
-    loss = torch.empty((), dtype=torch.float32, device=x.dev)
+    loss = x.scalar()
     dx, where = x.grad_out(logits, out) if want_dx else (None, _NO_GRAD)
     x.call("lema_distill_loss", ids.data_ptr(), int(ids.dtype is torch.int32), tl.data_ptr(),
            int(tl.dtype is torch.float32), ids.shape[-1], _ptr(mask), float(temperature),
