@@ -888,7 +888,8 @@ __device__ __forceinline__ float teacher_coef(const TeacherSums& t, float share)
 
 // k of a token of the policy loss, for its gradient row alone. A bf16 row is rounded to 2^-9, so
 // the approximate logarithm and exponentials (2e-6 at worst here) serve it; they cut what every
-// thread of a row waits for from 1200 to 500 cycles.
+// thread of a row waits for from 1200 to 500 cycles. A ratio that close to an end of the clip range
+// may count as on its other side here.
 template <typename T>
 __device__ __forceinline__ float policy_coef(const RowArgs& a, const Token& tk, float xt, float m,
                                              float s, float w) {
