@@ -859,12 +859,31 @@ __device__ __forceinline__ TeacherSums teacher_weights(const RowArgs& a, int64_t
   return TeacherSums{warp_sum(d_sum), sum, static_cast<float>(sum), bad};
 }
 
-// The value of a gradient row at an entry's index: k (q - p), p the sum of the entries that hold
-// this index, always in the same order, so that entries which repeat it write the same value.
-// Four entries a read; those behind the last hold no index.
-__device__ __forceinline__ float teacher_value(const RowArgs& a, int32_t id, const float* s_p,
-                                               const int32_t* s_id, float q, float inv_t,
-                                               float k) {
+// Indices of a row seen once and seen again, by their low bits: an index that is not seen again is
+// held by one entry.
+template <int BITS>
+struct Seen {
+  uint32_t once[BITS / 32], twice[BITS / 32];
+  __device__ __forceinline__ void clear(int t, int threads) {
+    for (int i = t; i < BITS / 32; i += threads) once[i] = twice[i] = 0;
+  }
+  __device__ __forceinline__ void add(int32_t id) {
+    const uint32_t bit = 1u << (id & 31);
+    if (atomicOr(&once[id % BITS / 32], bit) & bit) atomicOr(&twice[id % BITS / 32], bit);
+  }
+  __device__ __forceinline__ bool again(int32_t id) const {
+    return twice[id % BITS / 32] >> (id & 31) & 1u;
+  }
+};
+
+// The value of a gradient row at entry j's index: k (q - p), p the sum of the entries that hold
+// this index (`alone`: no other), always in the same order, so that entries which repeat it write
+// the same value. Four entries a read; those behind the last hold no index.
+__device__ __forceinline__ float teacher_value(const RowArgs& a, int j, bool alone,
+                                               const float* s_p, const int32_t* s_id, float q,
+                                               float inv_t, float k) {
+  if (alone) return k * (q - s_p[j] * inv_t);
+  const int32_t id = s_id[j];
   float p0 = 0.f, p1 = 0.f, p2 = 0.f, p3 = 0.f;
 #pragma unroll 4
   for (int i = 0; i < a.K4; i += 4) {
@@ -913,8 +932,12 @@ __device__ __forceinline__ void note_bad_index(const RowArgs& a) {
 // token_kernel. G threads hold a row, kE * NV elements each: it is read once, its exponentials
 // stay in registers and are scaled and written once. Loads of many resident groups overlap:
 // 16384 policy rows of 4096 bf16, three quarters of them counted (235 MB), take 49 us, 4.8 TB/s;
-// 65536 of 512 (117 MB) 36 us, bound by the latency of a row's chain; with 64 teacher entries
-// each 65 and 81 us, bound by the entries (each lane compares its indices with all 64).
+// 65536 of 512 (117 MB) 36 us, bound by the latency of a row's chain. With 64 teacher entries a
+// row whole calls take 85 and 81 us instead of 60 and 48, for the latency of their loads.
+// Entries whose index another one may hold are told by a bit of it; comparing each with all took
+// 145 us over 12258 rows of 1802 fp32 with 244 entries, this 84. (The CTAs of ring_kernel have
+// the threads to compare; marking by its producer took longer: 66 and 74 us over 2000 rows of
+// 32000 with 200.)
 constexpr int kDirectThreads = 128;
 template <typename T, int OBJ, int G, int NV>
 __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
@@ -927,6 +950,9 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   float* s_x = s_p + a.K4;
   int32_t* s_id = reinterpret_cast<int32_t*>(s_x + a.K4);
   __shared__ int32_t s_count[kDirectThreads / 32], s_seq[kGroups];
+  // a bit for each element of a row, or nearly
+  __shared__ Seen<OBJ == kDistill ? G * NV * E : 32> seen[kGroups];
+  if (OBJ == kDistill) seen[group].clear(tid, G);
   ptx::griddep_wait();
   const int64_t r = blockIdx.x * int64_t{kGroups} + group;
   Counts counts = listed_counts(a);
@@ -982,6 +1008,9 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   } else {
     __syncwarp();
   }
+  if (OBJ == kDistill)
+    for (int j = tid; j < a.K; j += G)
+      if (s_id[j] >= 0) seen[group].add(s_id[j]);
   const bool far = far_max(m, a.c);
   if (far) {
 #pragma unroll
@@ -1061,8 +1090,8 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
     const float inv_t = 1.f / s_t[group].t_sum;
     for (int j = tid; j < a.K; j += G)
       if (s_id[j] >= 0)
-        put(dx + s_id[j], teacher_value(a, s_id[j], s_p, s_id, ex2((s_x[j] - m) * a.c) * inv_s,
-                                        inv_t, k));
+        put(dx + s_id[j], teacher_value(a, j, !seen[group].again(s_id[j]), s_p, s_id,
+                                        ex2((s_x[j] - m) * a.c) * inv_s, inv_t, k));
   }
 }
 
@@ -1631,7 +1660,7 @@ __global__ void __launch_bounds__((WARPS + 1) * 32, Ring<WARPS>::kCtas)
               if (s_id[j] >= 0 &&
                   in_share<T>(inf->head, inf->nvec, start, nv, rank, s_id[j]))
                 put(dx + s_id[j],
-                    teacher_value(a, s_id[j], s_p, s_id, ex2((s_x[j] - m_row) * a.c) * inv_s,
+                    teacher_value(a, j, false, s_p, s_id, ex2((s_x[j] - m_row) * a.c) * inv_s,
                                   inv_t, k));
           }
         }
@@ -1763,7 +1792,7 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
         const float inv_t = 1.f / s_t.t_sum;
         for (int j = tid; j < a.K; j += kRowThreads)
           if (s_id[j] >= 0)
-            put(dx + s_id[j], teacher_value(a, s_id[j], s_p, s_id,
+            put(dx + s_id[j], teacher_value(a, j, false, s_p, s_id,
                                             ex2((s_x[j] - m) * a.c) * inv_s, inv_t, k));
       }
     }
@@ -2145,8 +2174,12 @@ int launch_logprobs(const RowArgs& a, int x_f32, cudaStream_t s) {
 
 template <typename T>
 int launch_logprobs_bwd_t(const RowArgs& a, int nvec, bool after, cudaStream_t s) {
-  const int g = warp_rows(nvec) ? 32 : kBwdThreads;
-  const int chunks = std::max(1, (nvec + g * kBwdU - 1) / (g * kBwdU));
+  // A CTA a chunk, or a warp where more than a fifth of the CTAs' threads would have no vector: the
+  // preference loss over 15000 rows of 4296 bf16 takes 106 and 104 us, over 10000 of 9000 117 and
+  // 112, over 4096 of 32000 (no such waste) 116 and 125.
+  const auto chunks_of = [&](int g) { return std::max(1, (nvec + g * kBwdU - 1) / (g * kBwdU)); };
+  const bool waste = chunks_of(kBwdThreads) * (kBwdThreads * kBwdU) > nvec + nvec / 4;
+  const int g = waste ? 32 : kBwdThreads, chunks = chunks_of(g);
   const int64_t per = kBwdThreads / g, grid = (a.T * chunks + per - 1) / per;
   if (grid > INT32_MAX) return set_error(LEMA_ERR_UNSUPPORTED, "too many rows");
   const auto kern = g == 32 ? logprobs_bwd_kernel<T, 32> : logprobs_bwd_kernel<T, kBwdThreads>;

@@ -867,3 +867,22 @@ def test_many_rows_in_graphs(cuda_device, V):
         for k, (_, _, got) in enumerate(graphs):
             for a, w in zip(got, want[k ^ swap]):
                 assert torch.equal(a, w)
+
+
+@pytest.mark.parametrize("V,K,dtype", [(7, 300, "bf16"), (300, 1024, "fp32"), (520, 40, "bf16"),
+                                       (2055, 244, "bf16"), (1802, 64, "fp32"), (8190, 700, "bf16")])
+def test_repeated_entries_of_short_rows(cuda_device, V, K, dtype):
+    """Indices drawn with repetition, and all alike, in rows that a warp or 128 threads hold."""
+    x, _, g = make(cuda_device, 2, 21, V, dtype)
+    val = torch.randn(2, 21, K, device=x.device, generator=g)
+    ids = torch.randint(0, V, (2, 21, K), device=x.device, generator=g)
+    ids[0, 0] = V - 1
+    ids[1, 3] = V - 1 - (torch.arange(K, device=x.device) % 2)
+    for kind in (torch.int64, torch.int32):
+        loss, dx = ops.distill_loss_grad(x, ids.to(kind), val)
+        want, k, mass, q = ref_distill(x, ids, val, None, 1.0)
+        # a weight: exponents below 16 (16 u), ex2 and expf 4 u, a sum of 32 a lane and the lanes
+        # 37 u; repeated ones are added in fp32, K / 4 in a row: K / 4 u
+        err = (57 + K / 4) * U
+        check_dx(dx, x, q, k, mass, mass_err=err)
+        assert abs(loss.item() - want.item()) <= rel_s(V) + 8 * err + 2 * U * abs(want.item())
