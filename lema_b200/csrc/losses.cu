@@ -588,6 +588,8 @@ __global__ void __launch_bounds__(kCountThreads) count_kernel(RowArgs a, int32_t
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = blockIdx.x, ctas = gridDim.x;  // one cluster
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // a CTA's shared memory may be written only once it runs: waited for behind the counting
+  if (ctas > 1) ptx::cluster_arrive();
   const int64_t r0 = static_cast<int64_t>(rank) * chunk, r1 = min(a.T, r0 + chunk);
   bool in[kCountRows];
   const auto load = [&](int64_t at) {
@@ -617,6 +619,7 @@ __global__ void __launch_bounds__(kCountThreads) count_kernel(RowArgs a, int32_t
     __syncthreads();
     if (lane == 0) atomicAdd(&s_sum, n);
     __syncthreads();
+    ptx::cluster_wait();
     if (tid < ctas)
       asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(
                        ptx::mapa_shared(ptx::smem_u32(&s_cta[rank]), tid)),

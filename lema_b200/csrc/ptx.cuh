@@ -166,10 +166,17 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
   return r;
 }
 
-// All threads of all CTAs in the cluster.
+// All threads of all CTAs in the cluster, in two halves: what lies between them overlaps the
+// wait for the others.
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::
-                   : "memory");
+  cluster_arrive();
+  cluster_wait();
 }
 
 // Address of the same shared-memory location in CTA `rank` of the cluster.

@@ -118,3 +118,22 @@ def test_adapters_can_be_left_out():
     assert not torch.equal(m(x), base(x))
     m.enabled = False
     assert torch.equal(m(x), base(x)) and LoRALinear.enabled
+
+
+def test_cluster_memory_is_used_behind_a_cluster_barrier():
+    """Another CTA's shared memory exists once that CTA runs: every kernel that takes an
+    address in it (mapa) has waited at a cluster barrier before. Read from the sources, since
+    an access too early is undefined."""
+    import re
+    from lema_b200 import build
+    seen = 0
+    for path in build.sources():
+        text = re.sub(r"//[^\n]*", "", path.read_text())
+        for body in text.split("__global__")[1:]:
+            remote = body.find("mapa_shared(")
+            if remote < 0:
+                continue
+            seen += 1
+            head = body[:remote]
+            assert "cluster_sync()" in head or "cluster_wait()" in head, (path.name, body[:80])
+    assert seen >= 2
