@@ -571,9 +571,17 @@ def rmsnorm_bwd(x2d, g, rstd, dhn):
     return dx
 
 
+def _rope_tables(cos: torch.Tensor, sin: torch.Tensor, seq: int, d: int) -> None:
+    """The kernel reads rows 0 .. seq - 1 of both tables."""
+    if min(cos.numel(), sin.numel()) < seq * d:
+        raise ValueError(f"cos and sin must have [{seq}, {d}] elements at least, got "
+                         f"{tuple(cos.shape)} and {tuple(sin.shape)}")
+
+
 def rope(q2d, k2d, cos, sin, seq: int, hq: int, hk: int, d: int, mode: int = 0):
     """Rotary embedding of q [T, hq*d] and k [T, hk*d] rows (may be strided);
     cos/sin [seq, d] bf16. Returns contiguous (q_out, k_out)."""
+    _rope_tables(cos, sin, seq, d)
     dev = _require_cuda(q2d, k2d, cos, sin)
     T = q2d.shape[0]
     qo = torch.empty(T, hq * d, dtype=torch.bfloat16, device=dev)
@@ -744,6 +752,7 @@ class MLPFn(torch.autograd.Function):
 def rope_qkv(q2d, k2d, v2d, q_add, k_add, v_add, cos, sin, seq, hq, hk, d):
     """Forward RoPE of q and k plus the contiguous copy of v, each after adding its
     optional LoRA output (bf16 rounding). Returns contiguous (q_out, k_out, v_out)."""
+    _rope_tables(cos, sin, seq, d)
     dev = _require_cuda(q2d, k2d, v2d, cos, sin)
     T = q2d.shape[0]
     qo = torch.empty(T, hq * d, dtype=torch.bfloat16, device=dev)

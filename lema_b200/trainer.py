@@ -310,10 +310,17 @@ class StreamedLoraTrainer:
                        adapters: bool = True, temperature: float = 1.0) -> torch.Tensor:
         """Log-probabilities [batch, seq] fp32 that the model gives the next token of
         each position (0 where it has none or its label is -100), by one streamed
-        forward. ``adapters=False`` leaves the LoRA adapters out: the frozen model
-        that preference and policy objectives refer to."""
+        forward. Any batch, and up to the trainer's ``seq`` positions.
+        ``adapters=False`` leaves the LoRA adapters out: the frozen model that
+        preference and policy objectives refer to."""
+        if ids.dim() != 2 or not 1 <= ids.shape[1] <= self.seq:
+            raise ValueError(f"ids must be [batch, 1 .. {self.seq}], got {tuple(ids.shape)}")
+        if labels is not None and labels.shape != ids.shape:
+            raise ValueError(f"labels must have the shape of ids, {tuple(ids.shape)}, got "
+                             f"{tuple(labels.shape)}")
         self.errors.check()
         dev = self.device
+        cos, sin = (t[:, :ids.shape[1]] for t in (self.cos, self.sin))
         ids = ids.to(dev, non_blocking=True)
         labels = ids if labels is None else labels.to(dev, non_blocking=True)
         lora = [m for blk in self.blocks for m in blk.modules() if isinstance(m, LoRALinear)]
@@ -327,7 +334,7 @@ class StreamedLoraTrainer:
             for i in range(self.L):
                 if i + ahead < self.L:
                     self._ensure(i + ahead)
-                h = self._bind(i)(h, self.cos, self.sin)
+                h = self._bind(i)(h, cos, sin)
                 self._release(i)
             logps = ops.token_logprobs(self.head(h), next_targets(labels),
                                        temperature=temperature)

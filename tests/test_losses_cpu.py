@@ -137,3 +137,28 @@ def test_cluster_memory_is_used_behind_a_cluster_barrier():
             head = body[:remote]
             assert "cluster_sync()" in head or "cluster_wait()" in head, (path.name, body[:80])
     assert seen >= 2
+
+
+def test_scores_refuse_longer_sequences():
+    """Positions behind the trainer's rotary tables would be read past their end."""
+    from types import SimpleNamespace
+    from lema_b200.trainer import StreamedLoraTrainer
+    tr = SimpleNamespace(seq=8)                 # refused before anything else is touched
+    for shape in ((2, 9), (2, 0), (8,), (1, 2, 4)):
+        with pytest.raises(ValueError, match="ids"):
+            StreamedLoraTrainer.token_logprobs(tr, torch.zeros(shape, dtype=torch.int64))
+    ids = torch.zeros(2, 8, dtype=torch.int64)
+    with pytest.raises(ValueError, match="labels"):
+        StreamedLoraTrainer.token_logprobs(tr, ids, ids[:, 1:])
+
+
+def test_rope_refuses_short_tables():
+    q = torch.zeros(12, 32, dtype=torch.bfloat16)
+    table, short = torch.zeros(6, 16), torch.zeros(1, 5, 16)
+    for cos, sin in ((short, table), (table, short)):
+        with pytest.raises(ValueError, match="cos and sin"):
+            ops.rope(q, q, cos, sin, 6, 2, 2, 16)
+        with pytest.raises(ValueError, match="cos and sin"):
+            ops.rope_qkv(q, q, q, None, None, None, cos, sin, 6, 2, 2, 16)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):     # long enough: the next check
+        ops.rope(q, q, table, table, 6, 2, 2, 16)

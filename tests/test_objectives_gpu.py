@@ -236,3 +236,24 @@ def test_bad_label_stops_training(cuda_device):
         tr.train_step(ids)
     tr.train_step(ids)
     tr.close()
+
+
+def test_scores_of_shorter_sequences(cuda_device):
+    """Sequences shorter than the trainer's and other batches, through the fused blocks and (an
+    adapter on o_proj) the others: the bits of a trainer built for that length, which runs the
+    same kernels on the same bytes. Longer ones are refused and the trainer goes on."""
+    for targets in (("q_proj", "v_proj"), ("q_proj", "o_proj")):
+        tr = _trainer(cuda_device, targets=targets)
+        ids, labels = _batch(cuda_device)
+        want = tr.token_logprobs(ids, labels)
+        for b, s in ((4, 31), (1, 48), (3, 1)):
+            one = _trainer(cuda_device, batch=b, seq=s, targets=targets)
+            got = tr.token_logprobs(ids[:b, :s], labels[:b, :s])
+            assert got.shape == (b, s)
+            assert torch.equal(got, one.token_logprobs(ids[:b, :s], labels[:b, :s]))
+            one.close()
+        for bad in (torch.cat([ids, ids], 1), torch.cat([ids, ids[:, :1]], 1), ids[:, :0], ids[0]):
+            with pytest.raises(ValueError, match="ids"):
+                tr.token_logprobs(bad)
+        assert torch.equal(want, tr.token_logprobs(ids, labels))
+        tr.close()
