@@ -313,9 +313,10 @@ LEMA_API int lema_attn_set_wait_budget(int64_t cycles);
 /* What stands beside the reference's shifted cross entropy (src/lema/_trainer.py:
  * 151-157) in a trainer that aligns or distils a model; the reference has no such
  * loss. Logits are n0 sequences of n1 rows of V values, bf16 (x_f32 = 0) or fp32,
- * row (b, t) at x + b*ld0 + t*ld1 elements, unit stride along V, any alignment.
- * targets [n0, n1] int64: a row whose target is ignore_index is not read, counts
- * for nothing and gets a zero gradient row. A target (or a teacher index with a
+ * row (b, t) at x + b*ld0 + t*ld1 elements, unit stride along V, starting at any
+ * element (a pointer off its own type's boundary is LEMA_ERR_MISALIGNED). targets
+ * [n0, n1] int64: a row whose target is ignore_index is not read, counts for
+ * nothing and gets a zero gradient row. A target (or a teacher index with a
  * weight) outside [0, V) records device error 0x106 and makes its row's outputs
  * NaN. q = softmax(x / temperature). Sums of exponentials are fp32, per-token
  * terms and sums over tokens fp64, every output is rounded once. Gradients dx have

@@ -25,6 +25,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <initializer_list>
 
 #include "internal.h"
 #include "ptx.cuh"
@@ -2033,14 +2034,25 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
 
 int bad(const char* what) { return set_error(LEMA_ERR_INVALID_ARGUMENT, what); }
 
+// Whether p lies on a multiple of n bytes (null does).
+bool on(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Every per-token array of 8-byte and of 4-byte values on its own type's boundary.
+int check_aligned(std::initializer_list<const void*> p8, std::initializer_list<const void*> p4) {
+  bool ok = true;
+  for (const void* p : p8) ok &= on(p, 8);
+  for (const void* p : p4) ok &= on(p, 4);
+  return ok ? LEMA_OK : set_error(LEMA_ERR_MISALIGNED, "a pointer lies off its type's boundary");
+}
+
 // Whether n rows `ld` elements apart stay inside 64-bit offsets.
 bool span_ok(int64_t n, int64_t ld) {
   return ld >= 0 && ld <= (int64_t{1} << 60) / std::max<int64_t>(n, 1);
 }
 
 // Sizes, strides and temperature shared by every entry point; fills the common fields.
-int make_rows(RowArgs& a, const void* x, int64_t n0, int64_t n1, int64_t ld0, int64_t ld1,
-              int64_t V, double temperature) {
+int make_rows(RowArgs& a, const void* x, int x_f32, int64_t n0, int64_t n1, int64_t ld0,
+              int64_t ld1, int64_t V, double temperature) {
   a = RowArgs{};
   if (n0 < 0 || n1 < 0) return bad("negative row count");
   if (V <= 0 || V > (1 << 30)) return bad("vocabulary size must be in [1, 2^30]");
@@ -2049,6 +2061,8 @@ int make_rows(RowArgs& a, const void* x, int64_t n0, int64_t n1, int64_t ld0, in
   if (n0 > 0 && n1 > INT32_MAX / n0)
     return set_error(LEMA_ERR_UNSUPPORTED, "more than 2^31 - 1 rows");
   if (n0 * n1 > 0 && x == nullptr) return bad("null logits");
+  if (!on(x, x_f32 ? 4 : 2))
+    return set_error(LEMA_ERR_MISALIGNED, "logits lie off their type's boundary");
   if (!span_ok(n0, ld0) || !span_ok(n1, ld1)) return bad("row stride negative or past 64 bits");
   a.x = x;
   a.in = RowMap{std::max<int64_t>(n1, 1), ld0, ld1};
@@ -2065,8 +2079,10 @@ int make_rows(RowArgs& a, const void* x, int64_t n0, int64_t n1, int64_t ld0, in
   return LEMA_OK;
 }
 
-int set_out(RowArgs& a, void* dx, int64_t ldd0, int64_t ldd1) {
+int set_out(RowArgs& a, void* dx, int x_f32, int64_t ldd0, int64_t ldd1) {
   if (dx == nullptr) return LEMA_OK;
+  if (!on(dx, x_f32 ? 4 : 2))
+    return set_error(LEMA_ERR_MISALIGNED, "gradient rows lie off their type's boundary");
   if (!span_ok(a.n0, ldd0) || !span_ok(a.in.n1, ldd1))
     return bad("gradient row stride negative or past 64 bits");
   // rows inside a sequence and sequences, either of them outermost
@@ -2352,7 +2368,7 @@ int launch_loss(RowArgs a, int x_f32, cudaStream_t s) {
 
 // Statistics are read and written as pairs.
 int set_stats(RowArgs& a, const float* stats) {
-  if ((reinterpret_cast<uintptr_t>(stats) & 7u) != 0) return bad("stats: 8-byte alignment");
+  if (!on(stats, 8)) return bad("stats: 8-byte alignment");
   a.stats = reinterpret_cast<float2*>(const_cast<float*>(stats));
   return LEMA_OK;
 }
@@ -2382,10 +2398,11 @@ extern "C" int lema_token_logprobs(const void* x, int32_t x_f32, int64_t n0, int
                                    float* stats, void* stream) {
   clear_error();
   RowArgs a;
-  int rc = make_rows(a, x, n0, n1, ld0, ld1, V, temperature);
+  int rc = make_rows(a, x, x_f32, n0, n1, ld0, ld1, V, temperature);
   if (rc) return rc;
   if (a.T == 0) return LEMA_OK;
   if (!targets || !logps) return bad("null targets or logps");
+  if ((rc = check_aligned({targets}, {logps}))) return rc;
   if ((rc = need_err(a))) return rc;
   a.targets = targets;
   a.ignore = ignore_index;
@@ -2402,11 +2419,12 @@ extern "C" int lema_token_logprobs_bwd(const void* x, int32_t x_f32, int64_t n0,
                                        int64_t ldd0, int64_t ldd1, void* stream) {
   clear_error();
   RowArgs a;
-  int rc = make_rows(a, x, n0, n1, ld0, ld1, V, temperature);
+  int rc = make_rows(a, x, x_f32, n0, n1, ld0, ld1, V, temperature);
   if (rc) return rc;
   if (a.T == 0) return LEMA_OK;
   if (!targets || !stats || !dlogps || !dx) return bad("null pointer");
-  if ((rc = set_out(a, dx, ldd0, ldd1))) return rc;
+  if ((rc = check_aligned({targets}, {dlogps, upstream}))) return rc;
+  if ((rc = set_out(a, dx, x_f32, ldd0, ldd1))) return rc;
   a.targets = targets;
   a.ignore = ignore_index;
   if ((rc = set_stats(a, stats))) return rc;
@@ -2424,7 +2442,7 @@ extern "C" int lema_preference_loss(const void* x, int32_t x_f32, int64_t n0, in
                                     int64_t ldd1, void* stream) {
   clear_error();
   RowArgs a;
-  int rc = make_rows(a, x, n0, n1, ld0, ld1, V, 1.0);
+  int rc = make_rows(a, x, x_f32, n0, n1, ld0, ld1, V, 1.0);
   if (rc) return rc;
   if (n0 == 0 || n0 % 2 != 0) return bad("preference_loss needs chosen and rejected sequences");
   if (!(beta > 0.0) || !std::isfinite(beta)) return bad("beta must be positive");
@@ -2432,7 +2450,9 @@ extern "C" int lema_preference_loss(const void* x, int32_t x_f32, int64_t n0, in
     return bad("label_smoothing must be in [0, 0.5)");
   if (!loss || !rewards || (a.T > 0 && (!targets || !logps || !stats || !coef)))
     return bad("null pointer");
-  if ((rc = set_ws(a, ws, ws_bytes)) || (rc = set_out(a, dx, ldd0, ldd1)) || (rc = need_err(a)))
+  if ((rc = check_aligned({targets}, {ref_logps, logps, coef, loss, rewards}))) return rc;
+  if ((rc = set_ws(a, ws, ws_bytes)) || (rc = set_out(a, dx, x_f32, ldd0, ldd1)) ||
+      (rc = need_err(a)))
     return rc;
   a.targets = targets;
   a.ignore = ignore_index;
@@ -2468,13 +2488,16 @@ extern "C" int lema_policy_loss(const void* x, int32_t x_f32, int64_t n0, int64_
                                 void* stream) {
   clear_error();
   RowArgs a;
-  int rc = make_rows(a, x, n0, n1, ld0, ld1, V, temperature);
+  int rc = make_rows(a, x, x_f32, n0, n1, ld0, ld1, V, temperature);
   if (rc) return rc;
   if (!(clip_lo >= 0.0 && clip_lo <= 1.0) || !(clip_hi >= 0.0) || !std::isfinite(clip_hi))
     return bad("clip must be in [0, 1] below and finite, >= 0 above");
   if (!(kl_coef >= 0.0) || !std::isfinite(kl_coef)) return bad("kl_coef must be >= 0");
   if (!loss || !kl || (a.T > 0 && (!targets || !advantages || !logps))) return bad("null pointer");
-  if ((rc = set_ws(a, ws, ws_bytes)) || (rc = set_out(a, dx, ldd0, ldd1)) || (rc = need_err(a)))
+  if ((rc = check_aligned({targets}, {old_logps, advantages, ref_logps, logps, coef, loss, kl})))
+    return rc;
+  if ((rc = set_ws(a, ws, ws_bytes)) || (rc = set_out(a, dx, x_f32, ldd0, ldd1)) ||
+      (rc = need_err(a)))
     return rc;
   a.targets = targets;
   a.ignore = ignore_index;
@@ -2505,13 +2528,17 @@ extern "C" int lema_distill_loss(const void* x, int32_t x_f32, int64_t n0, int64
                                  int64_t ldd1, void* stream) {
   clear_error();
   RowArgs a;
-  int rc = make_rows(a, x, n0, n1, ld0, ld1, V, temperature);
+  int rc = make_rows(a, x, x_f32, n0, n1, ld0, ld1, V, temperature);
   if (rc) return rc;
   if (!loss) return bad("null loss");
   if (K < 1 || K > kMaxTeacher)
     return set_error(LEMA_ERR_UNSUPPORTED, "between 1 and 1024 teacher entries a row");
   if (a.T > 0 && (!teacher_ids || !teacher_logits)) return bad("null teacher indices or logits");
-  if ((rc = set_ws(a, ws, ws_bytes)) || (rc = set_out(a, dx, ldd0, ldd1)) || (rc = need_err(a)))
+  if ((rc = check_aligned({}, {loss, upstream}))) return rc;
+  if (!on(teacher_ids, ids_i32 ? 4 : 8) || !on(teacher_logits, tl_f32 ? 4 : 2))
+    return set_error(LEMA_ERR_MISALIGNED, "teacher entries lie off their type's boundary");
+  if ((rc = set_ws(a, ws, ws_bytes)) || (rc = set_out(a, dx, x_f32, ldd0, ldd1)) ||
+      (rc = need_err(a)))
     return rc;
   a.teacher_ids = teacher_ids;
   a.ids_i32 = ids_i32;

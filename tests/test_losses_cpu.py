@@ -162,3 +162,37 @@ def test_rope_refuses_short_tables():
             ops.rope_qkv(q, q, q, None, None, None, cos, sin, 6, 2, 2, 16)
     with pytest.raises(RuntimeError, match="no CPU fallback"):     # long enough: the next check
         ops.rope(q, q, table, table, 6, 2, 2, 16)
+
+
+def test_pointers_off_their_types_are_refused():
+    """Each array moved off its element's boundary in turn, which a kernel would fault on."""
+    lib = N.lib()
+    rows = [FAKE, 0, 2, 3, 300, 100, 100]
+
+    def each(name, args, places):
+        for i, by in places:
+            moved = list(args)
+            moved[i] = FAKE + by
+            assert getattr(lib, name)(*moved) == N.LEMA_ERR_MISALIGNED, (name, i)
+
+    lp = rows + [FAKE, -100, 1.0, FAKE, None, None]
+    each("lema_token_logprobs", lp, [(0, 1), (7, 4), (10, 2)])
+    each("lema_token_logprobs", [FAKE, 1] + lp[2:], [(0, 2)])       # fp32 logits
+    bwd = rows + [FAKE, -100, 1.0, FAKE, FAKE, FAKE, FAKE, 300, 100, None]
+    each("lema_token_logprobs_bwd", bwd, [(0, 1), (7, 4), (11, 2), (12, 1), (13, 1)])
+    each("lema_token_logprobs_bwd", [FAKE, 1] + bwd[2:], [(13, 2)])
+    pref = rows + [FAKE, -100, FAKE, 0.1, 0.0, 1.0, FAKE, 1 << 20, FAKE, FAKE, FAKE, FAKE, FAKE,
+                   FAKE, 300, 100, None]
+    each("lema_preference_loss", pref, [(0, 1), (7, 4), (9, 2), (15, 1), (17, 3), (18, 2), (19, 1),
+                                        (20, 1)])
+    pol = rows + [FAKE, -100, 1.0, FAKE, FAKE, 3, 1, FAKE, 0.2, 0.2, 0.0, 0, 1.0, FAKE, 1 << 20,
+                  FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 300, 100, None]
+    each("lema_policy_loss", pol, [(0, 1), (7, 4), (10, 2), (11, 1), (14, 2), (22, 3), (24, 1),
+                                   (25, 2), (26, 1), (27, 1)])
+    dist = rows + [FAKE, 0, FAKE, 1, 3, None, 1.0, 1.0, FAKE, FAKE, 1 << 20, FAKE, FAKE, 300, 100,
+                   None]
+    each("lema_distill_loss", dist, [(0, 1), (7, 4), (9, 2), (15, 1), (18, 2), (19, 1)])
+    ids32, tl16 = list(dist), list(dist)
+    ids32[8], tl16[10] = 1, 0
+    each("lema_distill_loss", ids32, [(7, 2)])
+    each("lema_distill_loss", tl16, [(9, 1)])
