@@ -253,6 +253,22 @@ __device__ __forceinline__ float exp2_whole(float n) {
 __device__ __forceinline__ bool far_max(float m, float c) {
   return fabsf(m * c) > 2048.f && m != -INFINITY;
 }
+// What takes a partial sum of a row whose maximum is `from` to the larger maximum `to` (neither
+// of them -inf). A sum is about its maximum; with WHOLE it is about whole_max while the maximum is
+// near, and only a far one is about itself, so where one of the two is near the factor goes by
+// the two references that the sums have: 2^(from c - n) or 2^(n - to c), c with what its rounding
+// left, since 2048 times that is 2e-5.
+__device__ __forceinline__ float rescale_far(float from, float to, float c, float c_lo) {
+  if (!far_max(to, c)) return ex2(fmaf(from, c, -whole_max(to, c)) + from * c_lo);
+  if (!far_max(from, c)) return ex2(fmaf(-to, c, whole_max(from, c)) - to * c_lo);
+  return ex2((from - to) * c);
+}
+template <bool WHOLE>
+__device__ __forceinline__ float rescale(float from, float to, float c, float c_lo) {
+  if (!WHOLE) return ex2((from - to) * c);
+  if (far_max(from, c) || far_max(to, c)) return rescale_far(from, to, c, c_lo);
+  return exp2_whole(whole_max(from, c) - whole_max(to, c));
+}
 __device__ __forceinline__ uint64_t exp_pair(uint64_t x, const ExpScale& k) {
   float lo, hi;
   f2_unpack(f2_fma(x, k.c, k.mc), lo, hi);
@@ -396,8 +412,8 @@ __device__ __forceinline__ void group_sync() {
 }
 
 // Maximum of a row and sum of exp((x - m) / tau) from the (m, s) of a group's threads, for every
-// thread. WHOLE: the sums are about whole_max of their own maxima (about the maximum itself
-// when far_max), and the row's is about its own: see about_max. Sums meet in fp64.
+// thread. WHOLE: each sum is about the reference of its own maximum (rescale), the row's about
+// that of the row's: see about_max. Sums meet in fp64.
 template <int G, bool WHOLE>
 __device__ __forceinline__ void group_combine(float& m, double& s, const RowArgs& a, float* redf,
                                               double* redd) {
@@ -413,11 +429,7 @@ __device__ __forceinline__ void group_combine(float& m, double& s, const RowArgs
     for (int w = 1; w < G / 32; ++w) m = fmaxf(m, redf[w]);
   }
   // a thread that saw only -inf adds nothing
-  const bool far = !WHOLE || far_max(m, a.c);
-  const float n = whole_max(m, a.c);
-  const float f = far || far_max(mt, a.c) ? ex2((mt - m) * a.c)
-                                          : exp2_whole(whole_max(mt, a.c) - n);
-  s *= mt == -INFINITY ? 0.0 : static_cast<double>(f);
+  s *= mt == -INFINITY ? 0.0 : static_cast<double>(rescale<WHOLE>(mt, m, a.c, a.c_lo));
   s = warp_sum(s);
   if (G > 32) {
     if ((threadIdx.x & 31) == 0) redd[warp] = s;
@@ -470,9 +482,7 @@ __device__ __forceinline__ void thread_stats(const T* x, const Span<T>& sp, int 
     }
     const bool far = far_max(mx, c);
     const float n = far ? 0.f : whole_max(mx, c);
-    if (m != -INFINITY)  // the sum so far, about the new maximum
-      sum *= !WHOLE || far || far_max(m, c) ? ex2((m - mx) * c)
-                                            : exp2_whole(whole_max(m, c) - n);
+    if (m != -INFINITY) sum *= rescale<WHOLE>(m, mx, c, c_lo);  // the sum so far
     m = mx;
     if (far) {
 #pragma unroll

@@ -886,3 +886,67 @@ def test_repeated_entries_of_short_rows(cuda_device, V, K, dtype):
         err = (57 + K / 4) * U
         check_dx(dx, x, q, k, mass, mass_err=err)
         assert abs(loss.item() - want.item()) <= rel_s(V) + 8 * err + 2 * U * abs(want.item())
+
+
+def _straddling_rows(dev, dtype, V, seed):
+    """Rows around |x log2 e| = 2048 (|x| = 1419.565), where the statistics of a preference row
+    change their reference, on both sides of zero; rows short of it and wholly beyond."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    rows = []
+    for sign in (1.0, -1.0):
+        for mean, std in ((1300.0, 2.0), (1412.0, 2.0), (1416.0, 4.0), (1418.75, 0.3),
+                          (1419.5, 0.1), (1420.5, 0.3), (1427.0, 2.0), (1500.0, 2.0),
+                          (3e4, 2.0)):
+            rows.append(sign * mean + std * torch.randn(V, device=dev, generator=g))
+        # two values, the higher one rare: at the front, at the end, anywhere
+        low, high = sorted((sign * 1416.0, sign * 1424.0)) if dtype is torch.bfloat16 else \
+            sorted((sign * 1419.25, sign * 1419.75))
+        for at in (0, V - 1, V // 3):
+            row = torch.full((V,), low, device=dev)
+            row[at] = high
+            rows.append(row)
+        ramp = torch.linspace(low - 8, high + 8, V, device=dev)   # every step a new maximum
+        rows += [ramp, ramp.flip(0)]
+    return torch.stack(rows).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", [300, 2000, 7001, 16001, 40000])
+def test_preference_rows_across_the_far_border(cuda_device, V, dtype):
+    """Maxima on both sides of the border between the threads of a row and between their
+    sweeps (rows held by a warp, by 128 threads in one and in two sweeps, by 512). Sequences
+    of one token, so that each reward is a log-probability. A partial sum crosses the border
+    once within its thread and once when the threads meet: each multiplies by a power of two
+    whose exponent e is rounded to u |e| (weighted by 2^-|e|, less than u) and taken by
+    ex2.approx (4 u): 10 u beside the bound of any row."""
+    x = _straddling_rows(cuda_device, DT[dtype], V, V)
+    n = x.shape[0]
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    t = torch.where(torch.arange(n, device=x.device) % 2 == 0, x.float().argmax(-1),
+                    torch.randint(0, V, (n,), device=x.device, generator=g))[:, None]
+    x = torch.cat([x, x.flip(0)])[:, None]          # each row chosen once and rejected once
+    t = torch.cat([t, t.flip(0)])
+    P = n
+    lp, q = ref_logps(x, t)
+    ref = (lp + 0.3 * torch.randn(lp.shape, device=x.device, generator=g,
+                                  dtype=torch.float64)).float()
+    lp_err = rel_s(V) + 10 * U
+    a_max = min((x.double().amax(-1) - x.double().amin(-1)).max().item() * 1.4427, 150.0)
+    mass = onehot(t, V)
+    for r, e in ((None, 0.0), (ref, 0.1)):
+        loss, rewards, dx = ops.preference_loss_grad(x, t, r, beta=1.0, label_smoothing=e)
+        want, R, k, _ = ref_preference(x, t, r, 1.0, e)
+        assert ((rewards.double() - R).abs() <= lp_err + U * R.abs()).all(), \
+            (rewards.double() - R).abs().max().item()
+        assert abs(loss.item() - want.item()) <= 2 * lp_err + 2 * U * abs(want.item())
+        # dL/dh moves by at most a quarter of h's error
+        slack = 2 * lp_err / 4 / P
+        wantx = k[..., None] * (mass - q)
+        tol = (half_step(x.dtype) + 8 * U) * wantx.abs() \
+            + k.abs()[..., None] * (q * (lp_err + (4 + 2.1 * a_max) * U) + 2 * U * mass) \
+            + slack * (mass - q).abs() + 1e-37
+        assert ((dx.double() - wantx).abs() <= tol).all()
+        xr = x.clone().requires_grad_(True)
+        l2, rw2 = ops.preference_loss(xr, t, r, beta=1.0, label_smoothing=e)
+        assert torch.equal(l2.detach(), loss) and torch.equal(rw2, rewards)
+        assert torch.equal(torch.autograd.grad(l2, xr)[0], dx)
