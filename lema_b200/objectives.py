@@ -32,7 +32,8 @@ def next_targets(labels: torch.Tensor) -> torch.Tensor:
 class Preference:
     """Pairs of answers: the first half of the batch chosen, the second half the
     rejected ones of the same prompts. ``ref_logps`` [batch, seq] are the frozen
-    model's (``token_logprobs(ids, labels, adapters=False)``; None: reference-free).
+    model's (``token_logprobs(ids, labels, adapters=False)``, before the first step where
+    whole layers are fine-tuned; None: reference-free).
     ``rewards`` [batch] of the last call: beta * summed log ratios."""
 
     ref_logps: torch.Tensor | None = None

@@ -312,12 +312,19 @@ class StreamedLoraTrainer:
         each position (0 where it has none or its label is -100), by one streamed
         forward. Any batch, and up to the trainer's ``seq`` positions.
         ``adapters=False`` leaves the LoRA adapters out: the frozen model that
-        preference and policy objectives refer to."""
+        preference and policy objectives refer to. Selective full fine-tuning steps
+        the streamed weights themselves: from its first step on there is no frozen
+        model to score with and ``adapters=False`` is refused, so take the reference
+        scores before it."""
         if ids.dim() != 2 or not 1 <= ids.shape[1] <= self.seq:
             raise ValueError(f"ids must be [batch, 1 .. {self.seq}], got {tuple(ids.shape)}")
         if labels is not None and labels.shape != ids.shape:
             raise ValueError(f"labels must have the shape of ids, {tuple(ids.shape)}, got "
                              f"{tuple(labels.shape)}")
+        if not adapters and self.full_ft is not None and self.full_ft.layer_steps:
+            raise RuntimeError("adapters=False: full fine-tuning has changed the weights under the "
+                               "adapters, so they are not the frozen model any more; score the "
+                               "reference before the first step")
         self.errors.check()
         dev = self.device
         cos, sin = (t[:, :ids.shape[1]] for t in (self.cos, self.sin))

@@ -196,3 +196,24 @@ def test_pointers_off_their_types_are_refused():
     ids32[8], tl16[10] = 1, 0
     each("lema_distill_loss", ids32, [(7, 2)])
     each("lema_distill_loss", tl16, [(9, 1)])
+
+
+def test_scores_refuse_a_reference_that_has_been_trained():
+    from types import SimpleNamespace
+    from lema_b200.trainer import StreamedLoraTrainer
+
+    class Reached(Exception):
+        pass
+
+    def check():
+        raise Reached
+    ids = torch.zeros(2, 8, dtype=torch.int64)
+    errors = SimpleNamespace(check=check)            # what comes next
+    stepped = SimpleNamespace(layer_steps={1: 1})
+    with pytest.raises(RuntimeError, match="full fine-tuning"):
+        StreamedLoraTrainer.token_logprobs(
+            SimpleNamespace(seq=8, full_ft=stepped, errors=errors), ids, adapters=False)
+    for ft, adapters in ((stepped, True), (SimpleNamespace(layer_steps={}), False), (None, False)):
+        with pytest.raises(Reached):
+            StreamedLoraTrainer.token_logprobs(
+                SimpleNamespace(seq=8, full_ft=ft, errors=errors), ids, adapters=adapters)

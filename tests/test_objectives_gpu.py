@@ -257,3 +257,21 @@ def test_scores_of_shorter_sequences(cuda_device):
                 tr.token_logprobs(bad)
         assert torch.equal(want, tr.token_logprobs(ids, labels))
         tr.close()
+
+
+def test_reference_scores_and_full_fine_tuning(cuda_device):
+    """The reference is scored before the first full fine-tuning step, of an accumulated
+    one too, and refused behind it; scores with the adapters go on."""
+    tr = _trainer(cuda_device, full_ft_layers=(1,), lr=1e-3, grad_accum=2)
+    ids, labels = _batch(cuda_device)
+    ref = tr.token_logprobs(ids, labels, adapters=False)
+    tr.train_step(ids, labels, objective=Preference(ref))
+    assert torch.equal(ref, tr.token_logprobs(ids, labels, adapters=False))
+    before = tr.token_logprobs(ids, labels)
+    tr.train_step(ids, labels, objective=Preference(ref))
+    with pytest.raises(RuntimeError, match="full fine-tuning"):
+        tr.token_logprobs(ids, labels, adapters=False)
+    assert not torch.equal(before, tr.token_logprobs(ids, labels))
+    tr.train_step(ids, labels, objective=Preference(ref))
+    tr.check_device_errors()
+    tr.close()
