@@ -740,7 +740,7 @@ __device__ __forceinline__ double2 token_terms(const RowArgs& a, const Counts& n
   const double coef = policy_token<double, true>(a, load_token(a, r), lp, &loss, &kl);
   a.logps[r] = static_cast<float>(lp);
   if (a.coef) a.coef[r] = static_cast<float>(w * coef);
-  if (a.stats) a.stats[r] = make_float2(st.m, 1.f / st.s);
+  if (a.stats) a.stats[r] = make_float2(st.m, isnan(st.x) ? NAN : 1.f / st.s);
   return make_double2(w * loss, w * kl);
 }
 
@@ -794,7 +794,8 @@ __global__ void __launch_bounds__(stat_threads(G)) logprobs_kernel(RowArgs a) {
     a.logps[r] = static_cast<float>(lp);
     if (a.lp64) a.lp64[r] = lp;
     if (a.stats)
-      a.stats[r] = make_float2(m, static_cast<float>(1.0 / s) * expf(static_cast<float>(-up)));
+      a.stats[r] =
+          make_float2(m, ok ? static_cast<float>(1.0 / s) * expf(static_cast<float>(-up)) : NAN);
   }
 }
 
@@ -1984,7 +1985,9 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
       if (v0 + u * G < sp.nvec) w[u] = ld16(xv + v0 + u * G);
   }
   ptx::griddep_wait();
-  const float k = counts ? a.g[r] * grad_factor(a) * static_cast<float>(a.inv_tau) : 0.f;
+  const bool ok = target >= 0 && target < a.V;  // a row of NaN otherwise
+  const float k =
+      counts ? (ok ? a.g[r] * grad_factor(a) * static_cast<float>(a.inv_tau) : NAN) : 0.f;
   if (k == 0.f) {
     // zeros need no input: whole vectors of the output's own phase
     const Span<T> so(dx, a.V);
@@ -2003,7 +2006,6 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
   const bool same = same_phase<T>(x, dx);
   uint4* dv = reinterpret_cast<uint4*>(dx + sp.head);
   // the target's value, by the thread that has just written what the others hold there
-  const bool ok = target >= 0 && target < a.V;
   const int tv = ok ? static_cast<int>(target) - sp.head : -1;  // its place behind the head
   const float xt = ok ? to_f(x[target]) : 0.f;
   const auto scaled = [&](uint4 x16) {

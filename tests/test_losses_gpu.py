@@ -950,3 +950,37 @@ def test_preference_rows_across_the_far_border(cuda_device, V, dtype):
         l2, rw2 = ops.preference_loss(xr, t, r, beta=1.0, label_smoothing=e)
         assert torch.equal(l2.detach(), loss) and torch.equal(rw2, rewards)
         assert torch.equal(torch.autograd.grad(l2, xr)[0], dx)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", [3, 400, 9001])
+def test_gradient_of_an_out_of_range_target(cuda_device, V, dtype):
+    """Under autograd, too, a bad target's outputs are NaN: its log-probability, statistics and
+    gradient row (whatever its upstream gradient), and no other row's."""
+    for bad in (V, -1, 2 ** 40):
+        x, t, _ = make(cuda_device, 2, 5, V, dtype, ignore=0)
+        t[0, 1] = bad
+        t[1, 4] = IGN
+        hit = torch.zeros(2, 5, dtype=torch.bool, device=x.device)
+        hit[0, 1] = True
+        adv = torch.ones(2, 5, device=x.device)
+        for f in (lambda v: ops.token_logprobs(v, t).nansum(),
+                  lambda v: ops.token_logprobs(v, t).sum(),
+                  lambda v: ops.policy_loss(v, t, None, adv)[0]):
+            xr = x.clone().requires_grad_(True)
+            loss = f(xr)
+            assert _native.device_error() == 0x106
+            (dx,) = torch.autograd.grad(loss, xr)
+            assert dx[hit].isnan().all() and torch.isfinite(dx[~hit]).all()
+            assert (dx[1, 4] == 0).all()
+        xr = x.clone().requires_grad_(True)
+        (dx,) = torch.autograd.grad(ops.token_logprobs(xr, t), xr, torch.zeros_like(adv))
+        assert _native.device_error() == 0x106
+        assert dx[hit].isnan().all() and (dx[~hit] == 0).all()
+        stats = torch.zeros(2, 5, 2, device=x.device)
+        lp = torch.zeros(2, 5, device=x.device)
+        _native.call("lema_token_logprobs", x.data_ptr(), int(dtype == "fp32"), 2, 5, 5 * V, V, V,
+                     t.data_ptr(), IGN, 1.0, lp.data_ptr(), stats.data_ptr(),
+                     torch.cuda.current_stream().cuda_stream)
+        assert _native.device_error() == 0x106
+        assert stats[..., 1][hit].isnan().all() and torch.isfinite(stats[~hit]).all()
