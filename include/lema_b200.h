@@ -318,14 +318,18 @@ LEMA_API int lema_attn_set_wait_budget(int64_t cycles);
  * [n0, n1] int64: a row whose target is ignore_index is not read, counts for
  * nothing and gets a zero gradient row. A target (or a teacher index with a
  * weight) outside [0, V) records device error 0x106 and makes its row's outputs
- * NaN. q = softmax(x / temperature). Sums of exponentials are fp32, per-token
- * terms and sums over tokens fp64, every output is rounded once. Gradients dx have
- * the logits' type, row (b, t) at dx + b*ldd0 + t*ldd1, and may be written over x
- * itself (same pointer and strides); they may not overlap it otherwise. NULL dx
- * computes no gradient. grad_scale multiplies the gradient alone. `upstream` (may
- * be NULL) is one fp32 device value that multiplies the gradient. `ws` is a
- * 16-byte aligned scratch of lema_loss_workspace_bytes(n0, n1) bytes that no other
- * call in flight uses; it needs no initial value. With no counted row a loss is 0.
+ * NaN. q = softmax(x / temperature). Exponentials of logits (relative error 2^-22)
+ * and their sums are fp32; log-probabilities, their differences, returned losses
+ * and KL terms and sums over tokens are fp64. A gradient row is its token's
+ * coefficient times (onehot - q): the coefficient follows from the same fp64
+ * differences, with their exponentials in fp32 (2^-22 relative; for bf16 logits
+ * 1e-5), q is fp32. Every output is rounded once. Gradients dx have the logits'
+ * type, row (b, t) at dx + b*ldd0 + t*ldd1, and may be written over x itself (same
+ * pointer and strides); they may not overlap it otherwise. NULL dx computes no
+ * gradient. grad_scale multiplies the gradient alone. `upstream` (may be NULL) is
+ * one fp32 device value that multiplies the gradient. `ws` is a 16-byte aligned
+ * scratch of lema_loss_workspace_bytes(n0, n1) bytes that no other call in flight
+ * uses; it needs no initial value. With no counted row a loss is 0.
  * 1e-6 <= temperature <= 1e6. */
 
 /* Scratch bytes of the loss calls on n0 sequences of n1 rows (-1: too many rows). */

@@ -17,9 +17,12 @@
 // and the row of q = exp((x - m) / tau) / s written once. Rows that do not count (a target of
 // ignore_index, a false mask) are not read; their gradient row is zero.
 //
-// Precision: exponentials and their sum in fp32; what is computed once per token (the
-// log-probability, ratios, KL terms, sums over tokens) in fp64, since losses are differences
-// of nearly equal log-probabilities; every output rounded once.
+// Precision: exponentials (ex2.approx, 2^-22) and their sum in fp32; what is computed once per
+// token (the log-probability, its differences from the old and the reference one, the side of a
+// clip end, sums over tokens) in fp64, since losses are differences of nearly equal log-
+// probabilities, and with it ratios and KL terms where they are returned. A gradient row's
+// coefficient takes their exponentials in fp32 (for bf16 rows approximate ones) of the same fp64
+// differences. Every output is rounded once.
 #include <cuda_bf16.h>
 
 #include <algorithm>
@@ -96,6 +99,7 @@ struct RowArgs {
   int64_t adv_s0, adv_s1;
   const float* ref_logps;
   double clip_lo, clip_hi, kl_coef;
+  double log_lo, log_hi;         // log(1 - clip_lo), log(1 + clip_hi)
   int32_t per_sequence;
   int64_t n0;
   // distill
@@ -552,30 +556,66 @@ __device__ __forceinline__ Token load_token(const RowArgs& a, int64_t r) {
                a.ref_logps ? a.ref_logps[r] : 0.f};
 }
 
+// log(s) of a row's sum, to 1e-12: a row's threads wait for it (policy over 3 x 611 rows of
+// 100277 bf16 takes 158.5 us, with log() 161.9; over 8 x 1024 of 8000 60.8 and 61.6). s = 2^e f,
+// f in [sqrt(1/2), sqrt(2)), and with t = (f - 1) / (f + 1), |t| < 0.172,
+//   log f = 2 artanh t = 2 t + 2 t^3 (1/3 + t^2 / 5 + ... + t^10 / 13),
+// whose remainder is 5e-13. t is a quotient in fp32, corrected once by its residual in fp64. A sum
+// holds its maximum's 1, or it is NaN, and so is its logarithm. Every rounding is written
+// out, so that all who call it with one s get the same bits.
+__device__ __forceinline__ double log_sum(float s) {
+  const uint32_t bits = __float_as_uint(s);
+  const int e = static_cast<int>(bits - 0x3f3504f3u) >> 23;  // sqrt(1/2)
+  const float f = __uint_as_float(bits - (static_cast<uint32_t>(e) << 23));
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(f, 1.f)));
+  const double fd = f, rd = r, num = __dsub_rn(fd, 1.0), den = __dadd_rn(fd, 1.0);
+  const double q = __fmul_rn(__fsub_rn(f, 1.f), r);
+  const double t = __fma_rn(__fma_rn(-q, den, num), rd, q);
+  const double t2 = __dmul_rn(t, t), t4 = __dmul_rn(t2, t2), two_t = __dadd_rn(t, t);
+  const double p0 = __fma_rn(t2, 1.0 / 5, 1.0 / 3), p1 = __fma_rn(t2, 1.0 / 9, 1.0 / 7),
+               p2 = __fma_rn(t2, 1.0 / 13, 1.0 / 11);
+  const double p = __fma_rn(t4, __fma_rn(t4, p2, p1), p0);
+  const double y = __fma_rn(__dmul_rn(two_t, t2), p, __fma_rn(e, 0.6931471805599453, two_t));
+  return bits - 0x00800000u < 0x7f000000u ? y : NAN;
+}
+// A token's log-probability from what its row left.
+__device__ __forceinline__ double token_lp(const RowArgs& a, float x, float m, float s) {
+  return __fma_rn(__dsub_rn(x, m), a.inv_tau, -log_sum(s));
+}
+
+// e^d - 1 to 8e-6 of itself: beside a bf16 step of 2^-9 nothing, but e^d - 1 as it stands would
+// keep 2e-7 of 1 and so nothing of a small d.
+__device__ __forceinline__ float expm1_fast(float d) {
+  return fabsf(d) < 0.03125f ? d * fmaf(d, fmaf(d, 1.f / 6, 0.5f), 1.f) : __expf(d) - 1.f;
+}
+
 // dL/dlp of one token of the clipped policy loss over its weight, and (LOSS) its loss and KL.
-// F = double for what is returned, float for the gradient's coefficient.
+// F = double for what is returned, float for the gradient's coefficient (FAST: of a bf16 row). Both
+// take differences of log-probabilities, and the side of a clip end, from the same fp64 numbers:
+// a gradient row is clipped exactly where the returned loss is, and a KL term keeps the digits of
+// a small d.
 template <typename F, bool LOSS, bool FAST = false>
-__device__ __forceinline__ F policy_token(const RowArgs& a, const Token& tk, F lp, F* loss,
+__device__ __forceinline__ F policy_token(const RowArgs& a, const Token& tk, double lp, F* loss,
                                           F* kl) {
   const F A = tk.adv;
   // on-policy the ratio is 1, and NaN for a log-probability that is not finite
-  const F up = lp - (a.old_logps ? static_cast<F>(tk.old) : lp);
-  const F ratio = FAST ? static_cast<F>(__expf(static_cast<float>(up))) : exp(up);
-  const F lo = static_cast<F>(1.0 - a.clip_lo), hi = static_cast<F>(1.0 + a.clip_hi);
-  const F bent = ratio < lo ? lo : (ratio > hi ? hi : ratio);  // a NaN ratio stays NaN
-  const F plain = ratio * A, clipped = bent * A;
-  const bool use_plain = !(clipped < plain);
-  F coef = use_plain ? -plain : F(0);
+  const double up = __dsub_rn(lp, a.old_logps ? static_cast<double>(tk.old) : lp);
+  const F ratio = FAST ? static_cast<F>(__expf(static_cast<float>(up))) : exp(static_cast<F>(up));
+  // min(r A, clip(r) A) is the clipped one; not for a NaN ratio
+  const bool clipped = A > F(0) ? up > a.log_hi : A < F(0) && up < a.log_lo;
+  F coef = clipped ? F(0) : -ratio * A;
   F d_kl = F(0);
   if (a.ref_logps) {
-    const F d = static_cast<F>(tk.ref) - lp;
-    const F e = FAST ? static_cast<F>(__expf(static_cast<float>(d)) - 1.f) : expm1(d);
-    d_kl = e - d;
+    const double d = __dsub_rn(tk.ref, lp);
+    const F e = FAST ? static_cast<F>(expm1_fast(static_cast<float>(d))) : expm1(static_cast<F>(d));
+    d_kl = e - static_cast<F>(d);
     coef -= static_cast<F>(a.kl_coef) * e;
   }
   if (LOSS) {
     *kl = d_kl;
-    *loss = static_cast<F>(a.kl_coef) * d_kl - (use_plain ? plain : clipped);
+    *loss = static_cast<F>(a.kl_coef) * d_kl -
+            (clipped ? static_cast<F>(A > F(0) ? 1.0 + a.clip_hi : 1.0 - a.clip_lo) : ratio) * A;
   }
   return coef;
 }
@@ -725,17 +765,15 @@ __device__ __forceinline__ void zero_outputs(const RowArgs& a, int64_t r) {
 template <int OBJ>
 __device__ __forceinline__ double2 token_terms(const RowArgs& a, const Counts& n, int64_t r) {
   const RowStat st = a.row[r];
-  const double log_s = log(static_cast<double>(st.s));
   if (OBJ == kDistill) {
     // sum_k p_k (log p_k - log q_k), p_k = p'_k / t
-    const double t = st.x;
+    const double t = st.x, log_s = log(static_cast<double>(st.s));
     if (t == 0.0) return make_double2(0.0, 0.0);
     return make_double2((st.a / t * a.inv_tau - log(t) + log_s) /
                             (static_cast<double>(n.total) * a.inv_tau * a.inv_tau),
                         0.0);
   }
-  const double w = token_weight(a, n, r),
-               lp = (static_cast<double>(st.x) - st.m) * a.inv_tau - log_s;
+  const double w = token_weight(a, n, r), lp = token_lp(a, st.x, st.m, st.s);
   double loss, kl;
   const double coef = policy_token<double, true>(a, load_token(a, r), lp, &loss, &kl);
   a.logps[r] = static_cast<float>(lp);
@@ -920,17 +958,14 @@ __device__ __forceinline__ float teacher_coef(const TeacherSums& t, float share)
   return t.bad ? NAN : (t.t_sum == 0.f ? 0.f : share);
 }
 
-// k of a token of the policy loss, for its gradient row alone. A bf16 row is rounded to 2^-9, so
-// the approximate logarithm and exponentials (2e-6 at worst here) serve it; they cut what every
-// thread of a row waits for from 1200 to 500 cycles. A ratio that close to an end of the clip range
-// may count as on its other side here.
+// k of a token of the policy loss, for its gradient row: the log-probability and its differences
+// as the loss has them, their exponentials in fp32. A bf16 row is rounded to 2^-9, so approximate
+// exponentials (8e-6 at worst) serve it.
 template <typename T>
 __device__ __forceinline__ float policy_coef(const RowArgs& a, const Token& tk, float xt, float m,
                                              float s, float w) {
-  const float d = (xt - m) * static_cast<float>(a.inv_tau);
-  if (sizeof(T) == 4)
-    return policy_token<float, false>(a, tk, d - logf(s), nullptr, nullptr) * w;
-  return policy_token<float, false, true>(a, tk, d - __logf(s), nullptr, nullptr) * w;
+  return policy_token<float, false, sizeof(T) == 2>(a, tk, token_lp(a, xt, m, s), nullptr,
+                                                    nullptr) * w;
 }
 
 __device__ __forceinline__ float grad_factor(const RowArgs& a) {
@@ -957,7 +992,7 @@ constexpr int kDirectThreads = 128;
 template <typename T, int OBJ, int G, int NV>
 __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   constexpr int E = Vec<T>::kE, kGroups = kDirectThreads / G;
-  __shared__ float redf[2][kDirectThreads / 32];
+  __shared__ float redf[2][kDirectThreads / 32], s_k;
   __shared__ TeacherSums s_t[kGroups];
   extern __shared__ __align__(16) char smem[];
   const int tid = threadIdx.x % G, group = threadIdx.x / G, warp = tid >> 5;
@@ -1055,7 +1090,7 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
   }
   if (m == -INFINITY) s = NAN;
   const float inv_s = 1.f / s;
-  float k;
+  float k = 0.f;
   if (OBJ == kDistill) {
     const TeacherSums t = s_t[group];
     k = teacher_coef(t, row_share(a, counts));
@@ -1064,7 +1099,13 @@ __global__ void __launch_bounds__(kDirectThreads) direct_kernel(RowArgs a) {
       a.row[r] = RowStat{m, s, t.t_sum, 0.f, t.about(m)};
     }
   } else {
-    k = policy_coef<T>(a, tk, xt, m, s, weight);
+    // by one warp: conversions to and from fp64 share a pipe with 2^x
+    if (warp == 0) k = policy_coef<T>(a, tk, xt, m, s, weight);
+    if (G > 32) {
+      if (tid == 0) s_k = k;
+      __syncthreads();
+      k = s_k;
+    }
     if (tid == 0) {
       if (!ok) note_bad_index(a);
       a.row[r] = RowStat{m, s, xt, 0.f, 0.0};
@@ -1725,6 +1766,7 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
   __shared__ float redf[kRowThreads / 32];
   __shared__ double redd[kRowThreads / 32];
   __shared__ TeacherSums s_t;
+  __shared__ float s_k;
   const int tid = threadIdx.x;
   ptx::griddep_wait();
   const Counts counts = listed_counts(a);
@@ -1750,7 +1792,7 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
     thread_stats<T, kRowThreads, 4, false>(x, sp, tid, a.c, a.c_lo, m, sd);
     group_combine<kRowThreads, false>(m, sd, a, redf, redd);
     const float s = static_cast<float>(sd), inv_s = 1.f / s;
-    float k;
+    float k = 0.f;
     if (OBJ == kDistill) {
       k = teacher_coef(s_t, row_share(a, counts));
       if (tid == 0) {
@@ -1758,8 +1800,12 @@ __global__ void __launch_bounds__(kRowThreads) stream_kernel(RowArgs a) {
         a.row[r] = RowStat{m, s, s_t.t_sum, 0.f, s_t.about(m)};
       }
     } else {
-      k = policy_coef<T>(a, load_token(a, r), xt, m, s,
-                         static_cast<float>(token_weight(a, counts, r) * a.inv_tau));
+      if (tid < 32)  // one warp's conversions from and to fp64, not those of 32
+        k = policy_coef<T>(a, load_token(a, r), xt, m, s,
+                           static_cast<float>(token_weight(a, counts, r) * a.inv_tau));
+      if (tid == 0) s_k = k;
+      __syncthreads();
+      k = s_k;
       if (tid == 0) {
         if (!ok) note_bad_index(a);
         a.row[r] = RowStat{m, s, xt, 0.f, 0.0};
@@ -2520,6 +2566,8 @@ extern "C" int lema_policy_loss(const void* x, int32_t x_f32, int64_t n0, int64_
   a.ref_logps = ref_logps;
   a.clip_lo = clip_lo;
   a.clip_hi = clip_hi;
+  a.log_lo = std::log(1.0 - clip_lo);
+  a.log_hi = std::log(1.0 + clip_hi);
   a.kl_coef = kl_coef;
   a.per_sequence = per_sequence;
   a.logps = logps;

@@ -984,3 +984,99 @@ def test_gradient_of_an_out_of_range_target(cuda_device, V, dtype):
                      torch.cuda.current_stream().cuda_stream)
         assert _native.device_error() == 0x106
         assert stats[..., 1][hit].isnan().all() and torch.isfinite(stats[~hit]).all()
+
+
+# rows held by a warp, by 128 threads, by a CTA and by a cluster, and swept
+POLICY_LENGTHS = [300, 5000, 9001, 70000, 300001]
+
+
+def _even_rows(dev, B, S, V, dtype):
+    """Rows of one value. Their sum is V (exact below 2^24) and each log-probability -log V, so
+    that what the loss makes of it can be held to fp64 without the rows' own rounding."""
+    x = torch.zeros(B, S, V, dtype=DT[dtype], device=dev)
+    t = torch.randint(0, V, (B, S), device=dev, generator=torch.Generator(dev).manual_seed(V))
+    return x, t, torch.full((B, S), -math.log(V), dtype=torch.float64, device=dev)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", POLICY_LENGTHS)
+def test_kl_slope_of_a_policy_near_its_reference(cuda_device, V, dtype):
+    """Advantages of 0 and |ref - lp| from 1e-5 to 0.2: the row is -kl_coef (e^d - 1) w alone.
+    Relative bound: for fp32 rows d and e^d - 1 round once each (2 u and 2 u), kl_coef, w and
+    three products 5 u, 1 / s and two products behind it 4 u: 16 u in all with the stored
+    value's; for bf16 e^d - 1 is 8e-6 off (the remainder d^3 / 24 below 1/32, 2.4e-7 of
+    e^d above), 1e-5 with the rest."""
+    x, t, lp = _even_rows(cuda_device, 4, 12, V, dtype)
+    g = torch.Generator(device=cuda_device).manual_seed(2)
+    size = 10.0 ** (-5 + 4.3 * torch.rand(4, 12, device=x.device, generator=g))
+    sign = torch.where(torch.rand(4, 12, device=x.device, generator=g) < 0.5, -1.0, 1.0)
+    ref = (lp + (size * sign).double()).float()
+    d = ref.double() - lp
+    adv = torch.zeros(4, device=x.device)
+    k = -0.3 * torch.expm1(d) / 48
+    mass = onehot(t, V)
+    want = k[..., None] * (mass - 1.0 / V)
+    rel = half_step(x.dtype) + 1e-5 if dtype == "bf16" else 16 * U
+    old = (lp + 0.05).float()
+    for o in (None, old):
+        dx = ops.policy_loss_grad(x, t, o, adv, ref, kl_coef=0.3)[3]
+        assert ((dx.double() - want).abs() <= rel * want.abs()).all(), \
+            ((dx.double() - want).abs() / want.abs()).max().item()
+        xr = x.clone().requires_grad_(True)
+        (dx,) = torch.autograd.grad(ops.policy_loss(xr, t, o, adv, ref, kl_coef=0.3)[0], xr)
+        assert ((dx.double() - want).abs() <= rel * want.abs()).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", POLICY_LENGTHS)
+def test_ratios_next_to_the_clip_ends(cuda_device, V, dtype):
+    """Ratios a few last places of an old log-probability on either side of the clip range's
+    ends: both forms clip those that the fp64 formula clips, and no others."""
+    x, t, lp = _even_rows(cuda_device, 2, 42, V, dtype)
+    up = torch.arange(42, device=x.device)
+    for tau in (1.0, 0.7):
+        for clip in ((0.2, 0.3), (0.05, 0.28)):
+            edge = torch.tensor([math.log(1 - clip[0]), math.log(1 + clip[1])], device=x.device,
+                                dtype=torch.float64)[:, None]
+            # 21 steps of fp32 below and 21 above
+            step = 2.0 ** (math.floor(math.log2(math.log(V))) - 23)
+            old = ((lp - edge).float().double() + (up - 21) * step).float()
+            r = lp - old.double() - edge              # above 0: past the upper end, inside the lower
+            assert r.abs().min() > 1e-11              # log_sum is good to 1e-13
+            adv = torch.where(torch.arange(2, device=x.device) == 0, -1.0, 1.0)   # per sequence
+            gone = torch.stack([r[0] < 0, r[1] > 0])
+            dx = ops.policy_loss_grad(x, t, old, adv, clip=clip, temperature=tau)[3]
+            assert torch.equal((dx == 0).all(-1), gone)
+            xr = x.clone().requires_grad_(True)
+            (dx,) = torch.autograd.grad(
+                ops.policy_loss(xr, t, old, adv, clip=clip, temperature=tau)[0], xr)
+            assert torch.equal((dx == 0).all(-1), gone)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", POLICY_LENGTHS)
+def test_both_forms_of_the_policy_gradient(cuda_device, V, dtype):
+    """One call and autograd on ordinary rows, ratios anywhere and the reference near: the same
+    row statistics and the same fp64 differences, so what is between them is the rounding of the
+    coefficient (1e-5 for bf16 rows, 16 u) and of each stored value."""
+    x, t, g = make(cuda_device, 2, 14, V, dtype)
+    lp, _ = ref_logps(x, t, 0.9)
+    shape = lp.shape
+    noise = torch.randn(shape, device=x.device, generator=g, dtype=torch.float64)
+    old = (lp - 0.3 * noise).float()
+    ref = (lp + 3e-4 * noise.flip(0)).float()
+    adv = torch.randn(shape, device=x.device, generator=g)
+    adv[:, ::2] = 0.0
+    coef = 1e-5 if dtype == "bf16" else 16 * U
+    for kl in (0.0, 0.5):
+        kw = dict(kl_coef=kl, temperature=0.9, reduction="sequence")
+        dx = ops.policy_loss_grad(x, t, old, adv, ref, **kw)[3]
+        xr = x.clone().requires_grad_(True)
+        (gx,) = torch.autograd.grad(ops.policy_loss(xr, t, old, adv, ref, **kw)[0], xr)
+        assert torch.equal((dx == 0).all(-1), (gx == 0).all(-1))
+        a, b = dx.double(), gx.double()
+        # the target's own value is a difference of k and k q: its bound goes by the row's largest
+        top = torch.maximum(a.abs(), b.abs()).amax(-1, keepdim=True)
+        tol = (2 * half_step(x.dtype) + 2 * coef) * torch.maximum(a.abs(), b.abs()) \
+            + 8 * U * onehot(t, V) * top + 1e-37
+        assert ((a - b).abs() <= tol).all()
