@@ -609,12 +609,13 @@ __device__ __forceinline__ F policy_token(const RowArgs& a, const Token& tk, dou
   if (a.ref_logps) {
     const double d = __dsub_rn(tk.ref, lp);
     const F e = FAST ? static_cast<F>(expm1_fast(static_cast<float>(d))) : expm1(static_cast<F>(d));
-    d_kl = e - static_cast<F>(d);
-    coef -= static_cast<F>(a.kl_coef) * e;
+    d_kl = e == static_cast<F>(INFINITY) ? e : e - static_cast<F>(d);
+    // with a coefficient of 0 the KL is returned alone: it may be infinite
+    if (a.kl_coef != 0.0) coef -= static_cast<F>(a.kl_coef) * e;
   }
   if (LOSS) {
     *kl = d_kl;
-    *loss = static_cast<F>(a.kl_coef) * d_kl -
+    *loss = (a.kl_coef != 0.0 ? static_cast<F>(a.kl_coef) * d_kl : F(0)) -
             (clipped ? static_cast<F>(A > F(0) ? 1.0 + a.clip_hi : 1.0 - a.clip_lo) : ratio) * A;
   }
   return coef;
@@ -1983,7 +1984,9 @@ __global__ void __launch_bounds__(kPairThreads) pair_kernel(RowArgs a, int64_t P
     const double won = beta * sum.x, lost = beta * sum.y, h = won - lost;
     rewards[p] = static_cast<float>(won);
     rewards[p + P] = static_cast<float>(lost);
-    loss.x = ((1.0 - smooth) * softplus(-h) + smooth * softplus(h)) / static_cast<double>(P);
+    // no smoothing: no second term, which is infinite for a rejected token without probability
+    loss.x = ((1.0 - smooth) * softplus(-h) + (smooth > 0.0 ? smooth * softplus(h) : 0.0)) /
+             static_cast<double>(P);
     // sigma(-h) = 1 / (1 + e^h)
     s_dh = static_cast<float>((smooth / (1.0 + exp(-h)) - (1.0 - smooth) / (1.0 + exp(h))) * beta /
                               static_cast<double>(P));

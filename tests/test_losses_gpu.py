@@ -1080,3 +1080,66 @@ def test_both_forms_of_the_policy_gradient(cuda_device, V, dtype):
         tol = (2 * half_step(x.dtype) + 2 * coef) * torch.maximum(a.abs(), b.abs()) \
             + 8 * U * onehot(t, V) * top + 1e-37
         assert ((a - b).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", [130, 2000, 9001, 40000])
+def test_preference_of_infinities_and_lowest_values(cuda_device, V, dtype):
+    """Masked vocabularies through the preference loss's own statistics, each row a sequence of
+    its own beside an ordinary one, chosen and rejected."""
+    low = torch.finfo(DT[dtype]).min
+    x, _, _ = make(cuda_device, 1, 8, V, dtype, ignore=0)
+    x = x[0][:, None]
+    x[0, 0, 10:] = float("-inf")
+    x[1] = low
+    x[2] = low
+    x[2, 0, 3] = 0.0
+    x[3, 0, 3] = float("-inf")           # the target itself masked
+    x[4] = float("-inf")
+    x[5, 0, 7] = float("nan")
+    x[6, 0, 5] = float("inf")
+    plain, _, _ = make(cuda_device, 8, 1, V, dtype, seed=5, ignore=0)
+    t = torch.full((16, 1), 3, device=x.device)
+    for both in (torch.cat([x, plain]), torch.cat([plain, x])):
+        z = both.double()
+        lsm = torch.log_softmax(z - z.amax(-1, keepdim=True), -1)
+        want = lsm[..., 3].sum(1)
+        _, rewards, dx = ops.preference_loss_grad(both, t, beta=1.0)
+        got = rewards.double()
+        assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isinf(), want.isinf())
+        ok = torch.isfinite(want)
+        assert ((got - want).abs()[ok] <= (rel_s(V) + U * want.abs())[ok]).all()
+        bad = want[:8].isnan() | want[8:].isnan()
+        assert dx[torch.cat([bad, bad])].isnan().all()
+        h = want[:8] - want[8:]
+        k = torch.cat([-torch.sigmoid(-h), torch.sigmoid(-h)]) / 8
+        for r in (~torch.cat([bad, bad])).nonzero().flatten().tolist():
+            q = lsm[r, 0].exp()
+            mass = torch.zeros_like(q)
+            mass[3] = 1
+            w = k[r] * (mass - q)
+            tol = (half_step(x.dtype) + 8 * U) * w.abs() \
+                + k[r].abs() * (q * (rel_s(V) + 300 * U) + 2 * U * mass) \
+                + 2 * rel_s(V) / 8 * (mass - q).abs() + 1e-37
+            assert ((dx[r, 0].double() - w).abs() <= tol).all(), r
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("V", [130, 5000, 9001, 70000, 300001])
+def test_terms_without_weight(cuda_device, V, dtype):
+    """A target without probability (its logit -inf) where its infinite term has weight 0:
+    a rejected token without smoothing, the KL with a coefficient of 0."""
+    x, t, _ = make(cuda_device, 2, 3, V, dtype, ignore=0)
+    x[1, 1, t[1, 1]] = float("-inf")
+    loss, rewards, dx = ops.preference_loss_grad(x, t)
+    assert loss.item() == 0.0 and rewards[1].item() == -math.inf and not dx.any()
+    loss, _, _ = ops.preference_loss_grad(x, t, label_smoothing=0.1)
+    assert loss.item() == math.inf
+    old = ref = torch.full((2, 3), -2.0, device=x.device)
+    adv = torch.ones(2, device=x.device)
+    loss, lps, kl, dx = ops.policy_loss_grad(x, t, old, adv, ref)
+    plain = ops.policy_loss_grad(x, t, old, adv)
+    assert kl.item() == math.inf and torch.isfinite(loss) and torch.isfinite(dx).all()
+    assert torch.equal(loss, plain[0]) and torch.equal(dx, plain[3]) and not dx[1, 1].any()
+    loss, _, _, dx = ops.policy_loss_grad(x, t, old, adv, ref, kl_coef=0.1)
+    assert loss.item() == math.inf and not torch.isfinite(dx[1, 1]).any()
