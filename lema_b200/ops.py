@@ -873,7 +873,7 @@ class _Logits:
         if len(shape) == 2:
             t = t[None]
         elif len(shape) > 3:
-            t = t.reshape(-1, shape[-2], V)
+            t = t.reshape(math.prod(shape[:-2]), shape[-2], V)
         st = t.stride()
         if st[2] != 1 and V > 1:
             t = t.contiguous()
@@ -919,7 +919,7 @@ class _Logits:
         torch.autograd.graph.increment_version(out)
         view = out
         if out.dim() > 3:
-            view = out.view(-1, out.shape[-2], self.V)
+            view = out.view(self.n0, self.n1, self.V)
         elif out.dim() == 2:
             view = out[None]
         return out, (view.data_ptr(), view.stride(0), view.stride(1))

@@ -1143,3 +1143,20 @@ def test_terms_without_weight(cuda_device, V, dtype):
     assert torch.equal(loss, plain[0]) and torch.equal(dx, plain[3]) and not dx[1, 1].any()
     loss, _, _, dx = ops.policy_loss_grad(x, t, old, adv, ref, kl_coef=0.1)
     assert loss.item() == math.inf and not torch.isfinite(dx[1, 1]).any()
+
+
+def test_no_rows_of_any_shape(cuda_device):
+    for lead in ((0,), (2, 0), (0, 3), (2, 2, 0), (0, 2, 3), (2, 0, 3)):
+        x = torch.zeros(*lead, 50, device=cuda_device, dtype=torch.bfloat16)
+        t = torch.zeros(lead, dtype=torch.int64, device=cuda_device)
+        ids = torch.zeros(*lead, 3, dtype=torch.int64, device=cuda_device)
+        assert ops.token_logprobs(x, t).shape == lead
+        adv = torch.zeros(lead, device=cuda_device)
+        for out in (None, x):
+            loss, lps, kl, dx = ops.policy_loss_grad(x, t, None, adv, out=out)
+            assert loss.item() == 0 and kl.item() == 0 and lps.shape == lead and dx.shape == x.shape
+            loss, dx = ops.distill_loss_grad(x, ids, ids.float(), out=out)
+            assert loss.item() == 0 and dx.shape == x.shape
+        xr = x.clone().requires_grad_(True)
+        (g,) = torch.autograd.grad(ops.token_logprobs(xr, t).sum(), xr)
+        assert g.shape == x.shape
