@@ -298,8 +298,9 @@ __device__ __forceinline__ void shift_vec(uint4& w, float m) {
 // added up: a preference reward sums hundreds of them and keeps little, so what shifts them all
 // the same way shows (it was 2e-5 off with exp_vec). That is c's own rounding, 1e-8 of x - m,
 // added back here with a second multiply-add; and ex2.approx, which is 5e-8 low on average but 1e-8
-// on [-1/2, 1/2], where its argument is brought here. Elements are kept above n - 120, which
-// is nothing beside the maximum. NaNs are looked for apart.
+// on [-1/2, 1/2], where its argument is brought here: Cody and Waite's reduction, by a constant in
+// two parts. Elements are kept above n - 120, which is nothing beside the maximum. NaNs are
+// looked for apart.
 struct WholeScale {
   uint64_t c, c_lo, up;  // 1.5 * 2^23 - n, added and taken off: rounds to a whole number
   __device__ __forceinline__ WholeScale(float n, float c_, float c_lo_)

@@ -19,7 +19,8 @@ repetitions), printing one JSON line per case.
         reduce kernels) a single time, untimed, for an ncu capture
     python -m lema_b200.kernel_bench losses
         the losses over vocabulary logits (log-probabilities, preference, clipped
-        policy, distillation with their gradients) at the training batch, at short
+        policy, distillation: the value alone, its gradient by autograd and in the
+        same call; 64 and 1024 teacher entries) at the training batch, at short
         rows and at rows longer than a cluster holds; GB/s over the counted rows
         read once and every gradient row written once
 """
@@ -196,17 +197,39 @@ def losses() -> None:
         adv = torch.randn(B, device=dev)
         val, idx = torch.topk(x[..., :256].float(), 64, -1)
         once, both = (t != -100).sum().item() * V * x.element_size(), B * S * V * x.element_size()
-        for name, fn, nbytes in (
-                ("token_logprobs", lambda: ops.token_logprobs(x, t), once),
-                ("preference_loss_grad", lambda: ops.preference_loss_grad(x, t), once + both),
-                ("policy_loss_grad", lambda: ops.policy_loss_grad(x, t, None, adv), once + both),
-                ("distill_loss_grad", lambda: ops.distill_loss_grad(x, idx, val, t != -100),
-                 once + both)):
+        leaf, one = x.detach().requires_grad_(True), torch.ones((), device=dev)
+        up = torch.ones(B, S, device=dev)
+
+        def autograd(loss, upstream):
+            return torch.autograd.grad(loss, leaf, upstream)
+        cases = [
+            ("token_logprobs", lambda: ops.token_logprobs(x, t), once),
+            ("token_logprobs autograd", lambda: autograd(ops.token_logprobs(leaf, t), up),
+             once + both),
+            ("preference_loss", lambda: ops.preference_loss(x, t), once),
+            ("preference_loss autograd", lambda: autograd(ops.preference_loss(leaf, t)[0], one),
+             once + both),
+            ("preference_loss_grad", lambda: ops.preference_loss_grad(x, t), once + both),
+            ("policy_loss", lambda: ops.policy_loss(x, t, None, adv), once),
+            ("policy_loss autograd", lambda: autograd(ops.policy_loss(leaf, t, None, adv)[0], one),
+             once + both),
+            ("policy_loss_grad", lambda: ops.policy_loss_grad(x, t, None, adv), once + both),
+            ("distill_loss", lambda: ops.distill_loss(x, idx, val, t != -100), once),
+            ("distill_loss autograd",
+             lambda: autograd(ops.distill_loss(leaf, idx, val, t != -100), one), once + both),
+            ("distill_loss_grad", lambda: ops.distill_loss_grad(x, idx, val, t != -100),
+             once + both)]
+        if V >= 4096:
+            many, ids = torch.topk(x[..., :4096].float(), 1024, -1)
+            cases.append(("distill_loss_grad K 1024",
+                          lambda: ops.distill_loss_grad(x, ids, many, t != -100), once + both))
+        for name, fn, nbytes in cases:
             us = _time_us(fn, 9, flush)
             print(json.dumps({"case": f"{name} {B} x {S} x {V} {str(dtype)[6:]}",
                               "us": round(us, 1), "GBps": round(nbytes / us / 1e3, 1),
                               "bytes": nbytes}), flush=True)
-        del x, t, val, idx
+        del x, t, val, idx, leaf
+        many = ids = None
 
 
 def main(argv: list[str]) -> None:

@@ -1041,7 +1041,7 @@ def test_ratios_next_to_the_clip_ends(cuda_device, V, dtype):
             # 21 steps of fp32 below and 21 above
             step = 2.0 ** (math.floor(math.log2(math.log(V))) - 23)
             old = ((lp - edge).float().double() + (up - 21) * step).float()
-            r = lp - old.double() - edge              # above 0: past the upper end, inside the lower
+            r = lp - old.double() - edge   # above 0: past the upper end, inside the lower
             assert r.abs().min() > 1e-11              # log_sum is good to 1e-13
             adv = torch.where(torch.arange(2, device=x.device) == 0, -1.0, 1.0)   # per sequence
             gone = torch.stack([r[0] < 0, r[1] > 0])
