@@ -2024,7 +2024,12 @@ __global__ void __launch_bounds__(kBwdThreads) logprobs_bwd_kernel(RowArgs a, in
   T* dx = static_cast<T*>(a.dx) + a.out.at(r);
   const int64_t target = a.targets[r];
   const bool counts = target != a.ignore;
-  if (a.zeros_done && !counts) return;
+  if (a.zeros_done && !counts) {
+    // With no other rows the grid would end before pair_kernel, which whatever comes behind it on
+    // the stream then would not wait for: one CTA does.
+    if (blockIdx.x == 0) ptx::griddep_wait();
+    return;
+  }
   const Span<T> sp(x, a.V);
   const uint4* xv = sp.vecs(x);
   uint4 w[kBwdU];

@@ -217,3 +217,26 @@ def test_scores_refuse_a_reference_that_has_been_trained():
         with pytest.raises(Reached):
             StreamedLoraTrainer.token_logprobs(
                 SimpleNamespace(seq=8, full_ft=ft, errors=errors), ids, adapters=adapters)
+
+
+def test_kernels_that_overlap_the_one_before_wait_before_they_end():
+    """A kernel that may begin while its predecessor runs must not end before that does, or
+    what comes next on the stream follows this one alone: each such kernel waits, at least in
+    one CTA, before any of its threads may return. Read from the sources, since the order is
+    otherwise a matter of chance."""
+    import re
+    from lema_b200 import build
+    seen = 0
+    for path in build.sources():
+        text = re.sub(r"//[^\n]*", "", path.read_text())
+        for body in text.split("__global__")[1:]:
+            wait = body.find("griddep_wait()")
+            if wait < 0:
+                continue
+            seen += 1
+            # threads behind the last piece of work are never all of a CTA that waits
+            body = re.sub(r"if \(unit >= [^;]*\) return;", "", body)
+            wait = body.find("griddep_wait()")
+            first = re.search(r"\breturn\b", body)
+            assert first is None or wait < first.start(), (path.name, body[:120])
+    assert seen >= 10

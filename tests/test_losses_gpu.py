@@ -1160,3 +1160,25 @@ def test_no_rows_of_any_shape(cuda_device):
         xr = x.clone().requires_grad_(True)
         (g,) = torch.autograd.grad(ops.token_logprobs(xr, t).sum(), xr)
         assert g.shape == x.shape
+
+
+def test_preference_without_counted_rows_in_a_graph(cuda_device):
+    """Many pairs and no counted token, captured with what reads the loss behind it: no row of
+    the gradient has anything to do, and the loss is still complete when it is read."""
+    dev = cuda_device
+    x = torch.zeros(6000, 40, 8, dtype=torch.bfloat16, device=dev)
+    t = torch.full((6000, 40), IGN, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    got = torch.zeros(20, device=dev)
+    with torch.cuda.graph(graph):
+        for i in range(20):
+            loss, rewards, dx = ops.preference_loss_grad(x, t)
+            got[i].copy_(loss)
+            loss.fill_(7.0)
+            rewards.fill_(7.0)
+    for _ in range(5):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert ((got - math.log(2)).abs() <= U).all()
+        assert loss.item() == 7.0 and (rewards == 7.0).all() and not dx.any()
